@@ -49,6 +49,7 @@ enum {
   B2G_DTYPE_E4M3 = 2, /* fp8 e4m3 (OCP / NVIDIA __nv_fp8_e4m3) */
   B2G_DTYPE_E5M2 = 3, /* fp8 e5m2 */
   B2G_DTYPE_F32 = 4,  /* IEEE binary32: output (C) type only */
+  B2G_DTYPE_I8 = 5,   /* signed 8-bit integer: the 8-bit operators (b2g_*_q8) only */
 };
 
 /* Which kernel the calling thread's last successful compute call ran. */
@@ -331,6 +332,88 @@ int b2g_contract5d_batched(const void* A, const int64_t a_shape[5], const int64_
 int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t M, int64_t N,
                      int64_t K, int64_t lda, int64_t ldb, int64_t ldc, int64_t stride_a,
                      int64_t stride_b, int64_t stride_c, void* stream);
+
+/*
+ * The 8-bit linear layer: rows put into 8 bits with scales, their matrix product, and the
+ * backward passes that read them again.  No reference counterpart (the reference is fp16 only).
+ *
+ * Conventions of the b2g_*_q8 entry points:
+ *   - An 8-bit matrix is row-major, B2G_DTYPE_I8 (qmax 127) or B2G_DTYPE_E4M3 (qmax 448), with
+ *     one fp32 scale per row; element (m, n) stands for Q[m*ldq + n] * scale[m].
+ *   - Any leading dimension >= the row length (in elements) and any alignment of the element type
+ *     are accepted.  Row pitches and base addresses that are multiples of 16 bytes run fastest:
+ *     elsewhere the row kernels load elements one by one and the products copy the operand into
+ *     an aligned workspace first.  Elements between the row length and the pitch are neither
+ *     read nor written.
+ *   - Pointers belong to the current device.  Every pointer the call needs has to be non-null
+ *     unless it is said to be optional.  M == 0 is valid everywhere.
+ *   - Outputs may not overlap inputs or each other, except where said.
+ *
+ * b2g_quantize_q8: rows of X (dtype F16, BF16 or F32) into Q.  Per row, with a = max|x|:
+ *   scale = max(a / qmax, 2^-126), q = round(x * qmax / a) (to nearest, ties to even; x / scale
+ *   where the scale is at its least).  pow2 != 0: the scale is rounded up to a power of two
+ *   and q = round(x / scale).  A row that holds a NaN or an infinity gets the scale NaN and
+ *   q = 0, so that everything computed from it is NaN.  N >= 1.
+ *   Power-of-two scales are what b2g_wgrad_q8 wants: q * scale is then exact in bf16.
+ * b2g_dequantize_q8: X = Q * scale, rounded once to dtype (F16, BF16 or F32), saturating to
+ *   its largest finite value; a NaN scale gives NaN.
+ */
+int b2g_quantize_q8(const void* X, void* Q, float* scale, int64_t M, int64_t N, int64_t ldx,
+                    int64_t ldq, int dtype, int q_dtype, int pow2, void* stream);
+int b2g_dequantize_q8(const void* Q, const float* scale, void* X, int64_t M, int64_t N, int64_t ldq,
+                      int64_t ldx, int q_dtype, int dtype, void* stream);
+
+/*
+ * RMS norm with the residual's addition and an 8-bit output: per row
+ *   h = x + r,  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * w,  Q, scale = y in 8 bits
+ * (the rule of b2g_quantize_q8).  All sums are fp32, and y is computed from the unrounded h.
+ * R is optional (NULL: h = x); H is optional and receives h rounded to dtype; H may be X or R
+ * itself (same leading dimension), for a residual stream updated in place.  rstd is optional
+ * (M values, for b2g_rmsnorm_bwd_q8).  X, R and H have type dtype (F16, BF16 or F32), W (N
+ * values) w_dtype (the same three).  The sum of squares of a row has to stay below 2^128.
+ */
+int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void* H, void* Q, float* scale,
+                   float* rstd, int64_t M, int64_t N, int64_t ldx, int64_t ldr, int64_t ldh,
+                   int64_t ldq, int dtype, int w_dtype, int q_dtype, float eps, int pow2,
+                   void* stream);
+
+/*
+ * Scaled 8-bit matrix product: C[m,n] = (sum_k A[m*lda+k] * B[n*ldb+k]) * a_scale[m] * b_scale[n]
+ * + bias[n].  A is M x K (tokens), B is N x K (one row of weights per output channel), both
+ * `dtype` (I8 or E4M3).  int8 products are summed exactly in int32 (K <= 131071, so that no sum
+ * overflows), e4m3 products in fp32.  a_scale (M), b_scale (N) and bias (N) are optional fp32
+ * vectors (NULL: 1, 1 and 0).  C is F32, F16 or BF16, rounded once.
+ */
+int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
+                int64_t ldb, int64_t ldc, int dtype, const float* a_scale, const float* b_scale,
+                const float* bias, int c_dtype, void* stream);
+
+/*
+ * Weight gradient of C = X.W^T from an 8-bit checkpoint of X:
+ *   dW[n*ldw + k] = sum_{m < M} dY[m*ldy + n] * (Q[m*ldq + k] * scale[m])   (+ dW if accumulate)
+ * dY is M x N (dtype F16 or BF16), Q M x K (q_dtype) with its row scales, dW N x K of type
+ * c_dtype: F32, or (accumulate == 0 only) F16 or BF16.  Q * scale is rounded to dY's type
+ * (saturating): with power-of-two scales it is exact in BF16, and in F16 while it lies in
+ * F16's range.  Products are exact in fp32 and summed in fp32; an fp32 dW sums at most 4096
+ * tokens in one tensor-core accumulator, and such partial sums in fp32.
+ */
+int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, void* dW, int64_t M, int64_t N,
+                 int64_t K, int64_t ldy, int64_t ldq, int64_t ldw, int dtype, int q_dtype,
+                 int accumulate, int c_dtype, void* stream);
+
+/*
+ * Backward pass of the RMS norm, the rounding to 8 bits passed straight through:
+ *   xh = x * rstd,  g = dy * w,  dx = rstd * (g - xh * mean(g * xh)) (+ dr),  dw = sum_m dy * xh
+ * with x = X * x_scale the checkpoint of the norm's input h: x_dtype I8 or E4M3 with x_scale (M
+ * values), or F16, BF16 or F32 with x_scale NULL.  dY, dR and dX have type dtype (F16, BF16 or
+ * F32).  dR (the gradient that reaches h past the norm) and dw (N fp32 values, overwritten) are
+ * optional; dX may be dY or dR itself (same leading dimension).  All sums are fp32 in a fixed
+ * order, so results do not change from run to run.
+ */
+int b2g_rmsnorm_bwd_q8(const void* dY, const void* X, const float* x_scale, const void* W,
+                       const float* rstd, const void* dR, void* dX, float* dw, int64_t M, int64_t N,
+                       int64_t ldy, int64_t ldx, int64_t ldr, int64_t lddx, int dtype, int x_dtype,
+                       int w_dtype, void* stream);
 
 /* Balanced contiguous row partition: rank r gets M/world rows, the first M%world ranks one more.
  * No reference counterpart (the reference is single-GPU). */

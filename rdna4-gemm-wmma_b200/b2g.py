@@ -24,7 +24,7 @@ ERR_CUDA = 3
 ERR_TIMEOUT = 4
 ERR_NCCL = 5
 
-DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_E5M2, DTYPE_F32 = 0, 1, 2, 3, 4
+DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_E5M2, DTYPE_F32, DTYPE_I8 = 0, 1, 2, 3, 4, 5
 
 PATH_NONE, PATH_TC_1CTA, PATH_TC_2CTA, PATH_GENERIC, PATH_ZERO, PATH_EMPTY = range(6)
 PATH_NAMES = {0: "none", 1: "tc_1cta", 2: "tc_2cta", 3: "generic", 4: "zero", 5: "empty"}
@@ -140,6 +140,19 @@ def load(path=None):
     L.b2g_comm_destroy.argtypes = [vp]
     L.b2g_comm_check.restype = ctypes.c_int
     L.b2g_comm_check.argtypes = [vp, i64, vp]
+    c_int = ctypes.c_int
+    L.b2g_quantize_q8.restype = c_int
+    L.b2g_quantize_q8.argtypes = [vp] * 3 + [i64] * 4 + [c_int] * 3 + [vp]
+    L.b2g_dequantize_q8.restype = c_int
+    L.b2g_dequantize_q8.argtypes = [vp] * 3 + [i64] * 4 + [c_int] * 2 + [vp]
+    L.b2g_rmsnorm_q8.restype = c_int
+    L.b2g_rmsnorm_q8.argtypes = [vp] * 7 + [i64] * 6 + [c_int] * 3 + [ctypes.c_float, c_int, vp]
+    L.b2g_gemm_q8.restype = c_int
+    L.b2g_gemm_q8.argtypes = [vp] * 3 + [i64] * 6 + [c_int, vp, vp, vp, c_int, vp]
+    L.b2g_wgrad_q8.restype = c_int
+    L.b2g_wgrad_q8.argtypes = [vp] * 4 + [i64] * 6 + [c_int] * 4 + [vp]
+    L.b2g_rmsnorm_bwd_q8.restype = c_int
+    L.b2g_rmsnorm_bwd_q8.argtypes = [vp] * 8 + [i64] * 6 + [c_int] * 3 + [vp]
     if path is None:
         _lib = L
     return L
@@ -434,6 +447,125 @@ def contract5d_batched(A, a_shape, a_stride, B, b_shape, b_stride, b_batch_strid
                                          _arr(b_shape, 3), _arr(b_stride, 3), b_batch_stride,
                                          _ptr(C), _arr(c_shape, 4), _arr(c_stride, 4), dtype,
                                          float(alpha), float(beta), _stream(stream)))
+
+
+_TORCH_NAMES = {DTYPE_F16: ("torch.float16",), DTYPE_BF16: ("torch.bfloat16",),
+                DTYPE_F32: ("torch.float32",), DTYPE_I8: ("torch.int8",),
+                DTYPE_E4M3: ("torch.float8_e4m3fn", "torch.uint8")}
+_torch_types = None  # type code -> torch dtypes, filled in at the first tensor
+
+
+def _operand(x, dtype, what, rows=None, cols=None, ld=None):
+    """(pointer, leading dimension) of an operand of the 8-bit operators.  A raw pointer is taken
+    as it is (its leading dimension defaults to `cols`).  A torch tensor has to be of the type
+    that the call names, on the current device, and, with rows and cols, a row-major matrix of
+    that size at least, whose row stride is the default leading dimension."""
+    if x is None:
+        return None, (cols or 1) if ld is None else ld
+    if not hasattr(x, "stride"):
+        return _ptr(x), (cols or 1) if ld is None else ld
+    global _torch_types
+    import torch
+    if _torch_types is None:
+        _torch_types = {c: [getattr(torch, n.split(".")[1]) for n in names if hasattr(torch, n.split(".")[1])]
+                        for c, names in _TORCH_NAMES.items()}
+    if dtype in _torch_types and x.dtype not in _torch_types[dtype]:
+        raise B2GError(ERR_INVALID_ARG, "%s is %s, not of type code %r" % (what, x.dtype, dtype))
+    if not x.is_cuda:
+        raise B2GError(ERR_INVALID_ARG, "%s is not on a GPU" % what)
+    if x.get_device() != torch.cuda.current_device():
+        raise B2GError(ERR_INVALID_ARG, "%s is on another device than the current one" % what)
+    if rows is None:  # a vector
+        if cols and (x.numel() < cols or not x.is_contiguous()):
+            raise B2GError(ERR_INVALID_ARG, "%s has fewer than %d contiguous values" % (what, cols))
+        return x.data_ptr(), 1
+    if not rows or not cols:
+        return x.data_ptr(), (cols or 1) if ld is None else ld
+    if x.dim() == 2 and ld is None:
+        if x.shape[0] < rows or x.shape[1] < cols or (x.stride(1) != 1 and x.shape[1] > 1):
+            raise B2GError(ERR_INVALID_ARG, "%s is no row-major matrix of %d x %d" % (what, rows, cols))
+        return x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), cols)
+    return x.data_ptr(), cols if ld is None else ld
+
+
+def quantize_q8(X, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, pow2=False, ldx=None,
+                ldq=None, stream=None):
+    """Q, scale = rows of X (M x N, type dtype) in 8 bits: scale = max|x| / qmax, with pow2
+    rounded up to a power of two.  Leading dimensions default to the tensors' row strides."""
+    x, ldx = _operand(X, dtype, "X", M, N, ldx)
+    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
+    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
+    _check(load().b2g_quantize_q8(x, q, s, M, N, ldx, ldq, dtype, q_dtype, 1 if pow2 else 0,
+                                  _stream(stream)))
+
+
+def dequantize_q8(Q, scale, X, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, ldq=None, ldx=None,
+                  stream=None):
+    """X (M x N, type dtype) = Q * scale (one scale per row)."""
+    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
+    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
+    x, ldx = _operand(X, dtype, "X", M, N, ldx)
+    _check(load().b2g_dequantize_q8(q, s, x, M, N, ldq, ldx, q_dtype, dtype, _stream(stream)))
+
+
+def rmsnorm_q8(X, W, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, R=None, H=None, rstd=None,
+               w_dtype=None, eps=1e-6, pow2=False, ldx=None, ldr=None, ldh=None, ldq=None,
+               stream=None):
+    """h = X + R, Q, scale = (h / sqrt(mean(h^2) + eps) * W) in 8 bits.  Optional outputs: H = h
+    in type dtype (may be X or R itself), rstd (M fp32 values, for rmsnorm_bwd_q8)."""
+    w_dtype = dtype if w_dtype is None else w_dtype
+    x, ldx = _operand(X, dtype, "X", M, N, ldx)
+    r, ldr = _operand(R, dtype, "R", M, N, ldr)
+    w, _ = _operand(W, w_dtype, "W", None, N)
+    h, ldh = _operand(H, dtype, "H", M, N, ldh)
+    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
+    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
+    rs, _ = _operand(rstd, DTYPE_F32, "rstd", None, M)
+    _check(load().b2g_rmsnorm_q8(x, r, w, h, q, s, rs, M, N, ldx, ldr, ldh, ldq, dtype, w_dtype,
+                                 q_dtype, float(eps), 1 if pow2 else 0, _stream(stream)))
+
+
+def gemm_q8(A, B, C, M, N, K, dtype=DTYPE_I8, a_scale=None, b_scale=None, bias=None,
+            c_dtype=DTYPE_F32, lda=None, ldb=None, ldc=None, stream=None):
+    """C = (A . B^T) * a_scale[:, None] * b_scale + bias with A M x K and B N x K of 8-bit type
+    dtype (int32 sums for DTYPE_I8) and C of type c_dtype."""
+    a, lda = _operand(A, dtype, "A", M, K, lda)
+    b, ldb = _operand(B, dtype, "B", N, K, ldb)
+    c, ldc = _operand(C, c_dtype, "C", M, N, ldc)
+    sa, _ = _operand(a_scale, DTYPE_F32, "a_scale", None, M)
+    sb, _ = _operand(b_scale, DTYPE_F32, "b_scale", None, N)
+    bi, _ = _operand(bias, DTYPE_F32, "bias", None, N)
+    _check(load().b2g_gemm_q8(a, b, c, M, N, K, lda, ldb, ldc, dtype, sa, sb, bi, c_dtype,
+                              _stream(stream)))
+
+
+def wgrad_q8(dY, Q, scale, dW, M, N, K, dtype=DTYPE_BF16, q_dtype=DTYPE_I8, accumulate=False,
+             c_dtype=DTYPE_F32, ldy=None, ldq=None, ldw=None, stream=None):
+    """dW (N x K) = dY^T . (Q * scale) from the 8-bit checkpoint Q (M x K) of a linear layer's
+    input and the gradient dY (M x N) of its output; accumulate adds into an fp32 dW."""
+    y, ldy = _operand(dY, dtype, "dY", M, N, ldy)
+    q, ldq = _operand(Q, q_dtype, "Q", M, K, ldq)
+    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
+    w, ldw = _operand(dW, c_dtype, "dW", N, K, ldw)
+    _check(load().b2g_wgrad_q8(y, q, s, w, M, N, K, ldy, ldq, ldw, dtype, q_dtype,
+                               1 if accumulate else 0, c_dtype, _stream(stream)))
+
+
+def rmsnorm_bwd_q8(dY, X, x_scale, W, rstd, dX, dw, M, N, dtype=DTYPE_BF16, x_dtype=DTYPE_I8,
+                   w_dtype=None, dres=None, ldy=None, ldx=None, ldr=None, lddx=None, stream=None):
+    """Backward pass of rmsnorm_q8: dX = rstd * (dY*W - xh * mean(dY*W*xh)) (+ dres) and
+    dw = sum over rows of dY * xh, xh = (the checkpoint X * x_scale of h) * rstd.  dw may be None."""
+    w_dtype = dtype if w_dtype is None else w_dtype
+    y, ldy = _operand(dY, dtype, "dY", M, N, ldy)
+    x, ldx = _operand(X, x_dtype, "X", M, N, ldx)
+    xs, _ = _operand(x_scale, DTYPE_F32, "x_scale", None, M)
+    w, _ = _operand(W, w_dtype, "W", None, N)
+    rs, _ = _operand(rstd, DTYPE_F32, "rstd", None, M)
+    r, ldr = _operand(dres, dtype, "dres", M, N, ldr)
+    d, lddx = _operand(dX, dtype, "dX", M, N, lddx)
+    g, _ = _operand(dw, DTYPE_F32, "dw", None, N)
+    _check(load().b2g_rmsnorm_bwd_q8(y, x, xs, w, rs, r, d, g, M, N, ldy, ldx, ldr, lddx, dtype,
+                                     x_dtype, w_dtype, _stream(stream)))
 
 
 def version():

@@ -26,6 +26,7 @@
 
 #include "../../include/b2g_gemm.h"
 #include "errors.h"
+#include "host.h"
 #include "plan.h"
 #include "gemm_sm100.cuh"
 
@@ -40,7 +41,7 @@ static thread_local int64_t t_split_ws = 0;
 // Set while run() plans a call again without half-height pair tiles (see there).
 static thread_local bool t_no_half = false;
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
@@ -51,8 +52,10 @@ static int fail(int code, const char* fmt, ...) {
 }
 
 void set_error(const char* msg) { t_err = msg; }
+void clear_error() { t_err.clear(); }
+void set_path(int path) { t_path = path; }
 
-static int cuda_fail(cudaError_t e, const char* what) {
+int cuda_fail(cudaError_t e, const char* what) {
   return fail(B2G_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
@@ -80,6 +83,22 @@ int64_t comm_timeout_ms() { return opt_comm_timeout_ms.load(); }
 bool comm_nonblocking() { return opt_comm_nonblocking.load() != 0; }
 static std::atomic<int64_t> opt_cluster_fixup{1};  // split-K fix-up through distributed smem
 static std::atomic<int64_t> opt_serial_fixup{0};  // 1 = always the last-arriver fix-up
+
+LaunchOptions launch_options() {
+  LaunchOptions o;
+  o.cta_group = (int)opt_cta_group.load();
+  o.tile_n = (int)opt_tile_n.load();
+  o.split_k = (int)opt_split_k.load();
+  o.raster_group = (int)opt_raster_group.load();
+  o.force_generic = (int)opt_force_generic.load();
+  o.fault_flags = (int)opt_fault_flags.load();
+  o.tail_split = opt_tail_split.load() != 0;
+  o.pdl = opt_pdl.load() != 0;
+  o.cluster_fixup = opt_cluster_fixup.load() != 0;
+  o.serial_fixup = opt_serial_fixup.load() != 0;
+  o.timeout_ns = opt_timeout_ns.load();
+  return o;
+}
 
 // ------------------------------------------------------------------ driver entry point
 static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
@@ -114,10 +133,9 @@ struct MapKeyHash {
 static std::mutex g_map_mu;
 static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> g_map_cache;
 
-static CUresult encode_cached(CUtensorMap* out, CUtensorMapDataType dt, cuuint32_t rank, void* addr,
-                              const cuuint64_t* dims, const cuuint64_t* strides,
-                              const cuuint32_t* box, CUtensorMapSwizzle swz,
-                              CUtensorMapL2promotion l2) {
+CUresult encode_cached(CUtensorMap* out, CUtensorMapDataType dt, cuuint32_t rank, void* addr,
+                       const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                       CUtensorMapSwizzle swz, CUtensorMapL2promotion l2) {
   MapKey key;
   std::memset(key.w, 0, sizeof(key.w));
   key.w[0] = (uint64_t)(uintptr_t)addr;
@@ -173,6 +191,17 @@ static int device_state(int dev, DevState** out) {
     cudaDeviceGetAttribute(&d.cc_minor, cudaDevAttrComputeCapabilityMinor, dev);
   }
   *out = &d;
+  return B2G_OK;
+}
+
+int current_device(int* dev, int* sm_count, int* cc_major) {
+  const cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  DevState* ds = nullptr;
+  const int rc = device_state(*dev, &ds);
+  if (rc != B2G_OK) return rc;
+  *sm_count = ds->sm_count;
+  *cc_major = ds->cc_major;
   return B2G_OK;
 }
 
@@ -283,7 +312,7 @@ __global__ void fill_uniform_kernel(void* __restrict__ dst, int64_t n, uint64_t 
 // Stream-ordered pool of the split-K workspaces, one per device, that keeps freed memory for
 // reuse (release threshold: unlimited) instead of returning it to the driver at every
 // synchronisation as the default pool does.
-static int split_pool(cudaMemPool_t* out) {
+int split_pool(cudaMemPool_t* out) {
   static std::mutex mu;
   static cudaMemPool_t pools[64] = {};
   int dev = 0;

@@ -10,6 +10,8 @@ void count_launch();
 // Device error word of the multi-GPU kernels (b2g_shard.cu), merged into b2g_device_status():
 // reads it and, with clear != 0, resets it; returns 0 or a cudaError_t.
 int shard_device_error(int clear, int* value);
+// The same for the kernels of the 8-bit linear layer (b2g_q8.cu).
+int q8_device_error(int clear, int* value);
 // Options of the multi-GPU entry points (b2g_set_option "comm_timeout_ms", "comm_nonblocking").
 int64_t comm_timeout_ms();
 bool comm_nonblocking();

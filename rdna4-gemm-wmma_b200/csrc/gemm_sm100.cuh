@@ -31,8 +31,8 @@
 namespace b2g {
 
 // Device-side error word: 0 = fine, otherwise the code of the first bounded wait that gave up.
-// Read and cleared by b2g_device_status().
-__device__ int g_device_error;
+// Read and cleared by b2g_device_status().  One word per translation unit that has these kernels.
+static __device__ int g_device_error;
 
 enum : int {
   ERR_WAIT_EMPTY = 1,   // producer waiting for a free pipeline stage
@@ -107,6 +107,20 @@ struct GemmParams {
   int add_self;
   const unsigned* add_status;
   unsigned add_epoch;
+  // The 8-bit linear layer's instances (Q != Q_NONE; plain row-major C, one M mode):
+  const float* row_scale;  // Q_I8, Q_FP8: C = A.B * row_scale[row] * col_scale[col] + bias[col]
+  const float* col_scale;  // (null: 1)
+  void* c_direct;          // non-null: C (row pitch ldc elements) is stored with ordinary stores,
+  long long ldc;           // all of it (direct_all: a base or pitch that TMA does not take) or
+  int direct_all;          // only chunks that pass the last column (N not whole 16-byte pieces)
+};
+
+// What an instance of the kernel computes beside the plain product.
+enum : int {
+  Q_NONE = 0,
+  Q_I8 = 1,     // int8 operands, int32 accumulators, row and column scales
+  Q_FP8 = 2,    // fp8 operands, row and column scales
+  Q_WGRAD = 3,  // 16-bit operands, A stored with its rows contiguous ([k][m], as B is [k][n])
 };
 
 constexpr int kBM = 128;  // rows per CTA (UMMA M per CTA)
@@ -189,6 +203,39 @@ __host__ __device__ constexpr uint32_t make_idesc(int M, int N, bool b_mn_major,
          ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// kind::i8: D int32 (2 at bit 4), A and B signed 8-bit (1 at bits 7 and 10), both K-major.
+__host__ __device__ constexpr uint32_t make_idesc_i8(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// a + b of two accumulator words: fp32, or (I8) int32 held in a float's bits.
+template <bool I8>
+__device__ __forceinline__ float acc_add(float a, float b) {
+  if constexpr (I8)
+    return __int_as_float(__float_as_int(a) + __float_as_int(b));
+  else
+    return a + b;
+}
+
+// v[j] = p[col + j] for the 32 columns from col (the same for every lane: broadcast loads), without
+// touching columns past n.
+__device__ __forceinline__ void load_cols(const float* p, int col, int n, float (&v)[32]) {
+  if (col + 32 <= n && (reinterpret_cast<uintptr_t>(p + col) & 15) == 0) {
+    const float4* q = reinterpret_cast<const float4*>(p + col);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 x = __ldg(q + j);
+      v[4 * j] = x.x;
+      v[4 * j + 1] = x.y;
+      v[4 * j + 2] = x.z;
+      v[4 * j + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = col + j < n ? __ldg(p + col + j) : 0.0f;
+  }
+}
+
 // Unit u -> (tile, split index, number of splits of that tile, K-block range).
 __device__ __forceinline__ void unit_info(const GemmParams& p, int u, int& t, int& sp, int& ns,
                                           int& kb_lo, int& kb_hi) {
@@ -223,11 +270,15 @@ __device__ __forceinline__ void m_tile_origin(const GemmParams& p, int mt, int& 
 // ESZ: operand element size in bytes (2 = fp16/bf16 via kind::f16, 1 = fp8 via kind::f8f6f4).
 // A K block is 128 bytes of K (64 or 128 elements), consumed by 4 UMMAs of 32 bytes of K each.
 template <int CG, int BN, bool B_KMAJOR, bool C_MCONTIG, int ESZ, int BMC = kBM, int EW = 4,
-          bool ADD = false>
+          bool ADD = false, int Q = Q_NONE>
 __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
   using C = Cfg<CG, BN, BMC, EW>;
+  static_assert(Q == Q_NONE || (!C_MCONTIG && !ADD && BMC == kBM), "8-bit layer instances");
+  static_assert((Q != Q_I8 && Q != Q_FP8) || (ESZ == 1 && B_KMAJOR), "8-bit operands are K-major");
+  static_assert(Q != Q_WGRAD || (ESZ == 2 && !B_KMAJOR), "weight gradient: both operands MN-major");
+  constexpr bool I8 = Q == Q_I8;
   constexpr int KB = kRowBytes / ESZ;                 // K elements per stage
   constexpr int ATOM = kRowBytes / ESZ;               // MN-major swizzle atom width (elements)
   constexpr uint32_t ATOM_BYTES = (uint32_t)kRowBytes * KB;  // one atom: ATOM x KB elements
@@ -348,7 +399,14 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
           if (p.fault_flags & 1) continue;
           const int jj = kb / p.k_blocks_per_j;
           const int kc = (kb - jj * p.k_blocks_per_j) * KB;
-          ptx::tma_load_5d<CG>(base + s * C::A_BYTES, &tmA, fb, kc, jj, i0, b0, a0);
+          if constexpr (Q == Q_WGRAD) {
+#pragma unroll
+            for (int c = 0; c < BMC / ATOM; ++c)
+              ptx::tma_load_3d<CG>(base + s * C::A_BYTES + (uint32_t)c * ATOM_BYTES, &tmA, fb,
+                                   i0 + ATOM * c, kc, jj);
+          } else {
+            ptx::tma_load_5d<CG>(base + s * C::A_BYTES, &tmA, fb, kc, jj, i0, b0, a0);
+          }
           issue_b(base + C::OFF_B + s * C::B_BYTES, fb, n0, kc, jj, a0);
         }
       }
@@ -369,7 +427,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (leader && lane == 0) {
-      const uint32_t idesc = make_idesc(BMC * CG, C::UN, !B_KMAJOR, (uint32_t)p.ab_format);
+      const uint32_t idesc = I8 ? make_idesc_i8(BMC * CG, C::UN)
+                                : make_idesc(BMC * CG, C::UN, !B_KMAJOR, (uint32_t)p.ab_format) |
+                                      (Q == Q_WGRAD ? 1u << 15 : 0u);  // bit 15: A is MN-major
       int it = 0, tc = 0;
       bool ok = true;
       // Issue the MMAs of K block kb from stage s into N-halves [h_lo, h_hi).
@@ -378,14 +438,18 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         const uint32_t sb = base + C::OFF_B + s * C::B_BYTES;
 #pragma unroll
         for (int k16 = 0; k16 < 4; ++k16) {  // 4 UMMAs of 32 bytes of K
-          const uint64_t ad = ptx::smem_desc_sw128(sa + 32u * k16, 16u, 1024u);
+          const uint64_t ad = Q == Q_WGRAD ? ptx::smem_desc_sw128(sa + MN_STEP * k16, ATOM_BYTES, 1024u)
+                                           : ptx::smem_desc_sw128(sa + 32u * k16, 16u, 1024u);
 #pragma unroll
           for (int h = 0; h < C::NH; ++h) {
             if (h < h_lo || h >= h_hi) continue;
             const uint32_t bh = sb + (uint32_t)h * C::HALF_BYTES;
             const uint64_t bd = B_KMAJOR ? ptx::smem_desc_sw128(bh + 32u * k16, 16u, 1024u)
                                          : ptx::smem_desc_sw128(bh + MN_STEP * k16, ATOM_BYTES, 1024u);
-            ptx::umma<CG, ESZ>(d + (uint32_t)h * C::UN_COLS, ad, bd, idesc, (kb | k16) != 0 ? 1u : 0u);
+            if constexpr (I8)
+              ptx::umma_i8<CG>(d + (uint32_t)h * C::UN_COLS, ad, bd, idesc, (kb | k16) != 0 ? 1u : 0u);
+            else
+              ptx::umma<CG, ESZ>(d + (uint32_t)h * C::UN_COLS, ad, bd, idesc, (kb | k16) != 0 ? 1u : 0u);
           }
         }
       };
@@ -515,6 +579,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
       ptx::tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)acc * C::ACC_COLS;
       const int n0 = tn * BN + col_off;
+      float row_scale = 1.0f;  // this lane's row
+      if constexpr (Q == Q_I8 || Q == Q_FP8)
+        if (p.row_scale && rows_valid && ci + lane < p.i_size) row_scale = __ldg(p.row_scale + ci + lane);
 
       // Stage chunk `ch` (32 columns of this warp's 32 rows) and TMA-store it.
       auto store_chunk = [&](const uint32_t (&v)[32], int ch) {
@@ -580,6 +647,51 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) w[j] = v[j];
         }
+        if constexpr (Q == Q_I8 || Q == Q_FP8) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            w[j] = __float_as_uint((I8 ? (float)(int)w[j] : __uint_as_float(w[j])) * row_scale);
+          if (p.col_scale) {
+            float cs[32];
+            load_cols(p.col_scale, gcol, p.n_size, cs);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) * cs[j]);
+          }
+          if (p.bias) {
+            float b[32];
+            load_cols(p.bias, gcol, p.n_size, b);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(__uint_as_float(w[j]) + b[j]);
+          }
+        }
+        if constexpr (Q != Q_NONE) {
+          if (p.c_direct && (p.direct_all || gcol + 32 > p.n_size)) {
+            // turn the 32 x 32 chunk in shared memory (word j of row r at r * 32 + (j ^ r): no bank
+            // is hit twice either way) and store it row by row, 32 columns at a time
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              ptx::st_shared_b32(buf + 4u * (uint32_t)(lane * 32 + (j ^ lane)), w[j]);
+            __syncwarp();
+            const int nrows = min(32, p.i_size - ci), col = gcol + lane;
+            for (int r = 0; r < nrows; ++r) {
+              const float x = __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r))));
+              if (col < p.n_size) {
+                const long long at = (long long)(ci + r) * p.ldc + col;
+                if (p.c_type == 0) {
+                  float* c = static_cast<float*>(p.c_direct) + at;
+                  *c = p.accumulate ? *c + x : x;
+                } else if (p.c_type == 1) {
+                  static_cast<__half*>(p.c_direct)[at] = __float2half_rn(x);
+                } else {
+                  static_cast<__nv_bfloat16*>(p.c_direct)[at] = __float2bfloat16_rn(x);
+                }
+              }
+            }
+            __syncwarp();
+            return;
+          }
+        }
+        if constexpr (Q == Q_NONE) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           w[j] = p.alpha == 1.0f ? w[j] : __float_as_uint(__uint_as_float(w[j]) * p.alpha);
@@ -602,6 +714,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
               if (gcol + j < p.n_size)
                 w[j] = __float_as_uint(__uint_as_float(w[j]) + __ldg(p.bias + gcol + j));
           }
+        }
         }
         if (p.c_type != 0) {
           // 16-bit C: row `lane` as 4 16-byte chunks (32 values rounded to nearest), 64-byte
@@ -726,10 +839,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
                 if (r0 + c >= ns) break;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                  a[4 * j] += x[c][j].x;
-                  a[4 * j + 1] += x[c][j].y;
-                  a[4 * j + 2] += x[c][j].z;
-                  a[4 * j + 3] += x[c][j].w;
+                  a[4 * j] = acc_add<I8>(a[4 * j], x[c][j].x);
+                  a[4 * j + 1] = acc_add<I8>(a[4 * j + 1], x[c][j].y);
+                  a[4 * j + 2] = acc_add<I8>(a[4 * j + 2], x[c][j].z);
+                  a[4 * j + 3] = acc_add<I8>(a[4 * j + 3], x[c][j].w);
                 }
               }
             }
@@ -849,27 +962,27 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
               for (int j = 0; j < 8; ++j) y[j] = __ldcg(src + (sp + 1) * split_stride + 32 * j);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                a[4 * j] += x[j].x;
-                a[4 * j + 1] += x[j].y;
-                a[4 * j + 2] += x[j].z;
-                a[4 * j + 3] += x[j].w;
+                a[4 * j] = acc_add<I8>(a[4 * j], x[j].x);
+                a[4 * j + 1] = acc_add<I8>(a[4 * j + 1], x[j].y);
+                a[4 * j + 2] = acc_add<I8>(a[4 * j + 2], x[j].z);
+                a[4 * j + 3] = acc_add<I8>(a[4 * j + 3], x[j].w);
               }
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                a[4 * j] += y[j].x;
-                a[4 * j + 1] += y[j].y;
-                a[4 * j + 2] += y[j].z;
-                a[4 * j + 3] += y[j].w;
+                a[4 * j] = acc_add<I8>(a[4 * j], y[j].x);
+                a[4 * j + 1] = acc_add<I8>(a[4 * j + 1], y[j].y);
+                a[4 * j + 2] = acc_add<I8>(a[4 * j + 2], y[j].z);
+                a[4 * j + 3] = acc_add<I8>(a[4 * j + 3], y[j].w);
               }
             }
             if (sp < p.k_splits) {
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
                 const float4 x = __ldcg(src + sp * split_stride + 32 * j);
-                a[4 * j] += x.x;
-                a[4 * j + 1] += x.y;
-                a[4 * j + 2] += x.z;
-                a[4 * j + 3] += x.w;
+                a[4 * j] = acc_add<I8>(a[4 * j], x.x);
+                a[4 * j + 1] = acc_add<I8>(a[4 * j + 1], x.y);
+                a[4 * j + 2] = acc_add<I8>(a[4 * j + 2], x.z);
+                a[4 * j + 3] = acc_add<I8>(a[4 * j + 3], x.w);
               }
             }
             uint32_t vv[32];

@@ -48,9 +48,189 @@ struct NormArgs {
   bool norm, pow2;
 };
 
-// One block per row, two passes over it: sum of squares and largest |h * w| (|x| without the
-// norm), then the 8-bit values.  The largest |y| is rstd * max|h * w|, so one pass serves both.
-__global__ void __launch_bounds__(kRowThreads) rows_to_q8_kernel(const NormArgs a) {
+// ------------------------------------------------------------------ vectors of a row
+// VEC consecutive elements, loaded and stored as one piece.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Vec {
+  T e[VEC];
+};
+
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ void from_f(__half* d, float v) { *d = __float2half_rn(v); }
+__device__ __forceinline__ void from_f(__nv_bfloat16* d, float v) { *d = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f(float* d, float v) { *d = v; }
+
+// Elements [n, n + VEC) of a row of N; elements past the row are not touched and read as zero.
+template <typename T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> load_vec(const T* row, int64_t n, int64_t N) {
+  Vec<T, VEC> v;
+  if (n + VEC <= N) {
+    if constexpr (sizeof(v) == 16) {  // read once: do not displace the weights from L1
+      *reinterpret_cast<uint4*>(&v) = __ldcs(reinterpret_cast<const uint4*>(row + n));
+    } else {
+      v = *reinterpret_cast<const Vec<T, VEC>*>(row + n);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      v.e[j] = n + j < N ? row[n + j] : T(0.0f);
+    }
+  }
+  return v;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* row, int64_t n, int64_t N, const Vec<T, VEC>& v) {
+  if (n + VEC <= N) {
+    *reinterpret_cast<Vec<T, VEC>*>(row + n) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (n + j < N) row[n + j] = v.e[j];
+  }
+}
+
+// VEC weights as fp32 (any type; cached in L1 for the block's next row).
+template <int VEC>
+__device__ __forceinline__ void load_weights(const void* W, int w_dtype, int64_t n, int64_t N, float (&w)[VEC]) {
+  const int size = w_dtype == B2G_DTYPE_F32 ? 4 : 2;
+  if (VEC >= 4 && n + VEC <= N && (reinterpret_cast<uintptr_t>(W) & (4 * size - 1)) == 0) {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 4) {  // four at a time: 16 bytes of fp32, 8 of the 16-bit types
+      if (size == 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(W) + n + j));
+        w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
+      } else {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(W) + n + j));
+        const uint32_t b[2] = {x.x, x.y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (w_dtype == B2G_DTYPE_BF16) {
+            w[j + 2 * k] = __uint_as_float(b[k] << 16);
+            w[j + 2 * k + 1] = __uint_as_float(b[k] & 0xffff0000u);
+          } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[k]));
+            w[j + 2 * k] = f.x;
+            w[j + 2 * k + 1] = f.y;
+          }
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[j] = n + j < N ? load_elem(W, n + j, w_dtype) : 0.0f;
+  }
+}
+
+// (sum, integer maximum) over the threads of a row: a warp, or the block.  `buf` holds two words
+// per warp for each parity of the row count, so consecutive rows need one barrier each.
+template <bool WARP>
+__device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, float* buf, int parity) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if constexpr (!WARP) {
+    float2* b = reinterpret_cast<float2*>(buf) + parity * 32;
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = make_float2(sum, __uint_as_float(top));
+    __syncthreads();
+    const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
+    const float2 x = lane < warps ? b[lane] : make_float2(0.0f, 0.0f);
+    sum = x.x;
+    top = __float_as_uint(x.y);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  }
+}
+
+// Rows into 8 bits, each row held in registers: one pass over the data.  A row belongs to a warp
+// (WARP: short rows) or to the block; a thread holds V vectors of VEC elements of it, `threads`
+// vectors apart.  Blocks stride over the rows; where registers allow (AHEAD: blocks of up to 256
+// threads) a row's loads are issued before the previous row is reduced, so that the reduction's
+// barrier is not waited out with the memory idle.
+//
+// Per row: sum of squares and largest |h * w| (|x| without the norm).  The largest |y| is rstd
+// times that, so one reduction serves both; rstd cancels from the 8-bit values (row_quant).
+template <typename T, bool NORM, int VEC, int V, bool WARP, bool AHEAD>
+__global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AHEAD ? 2 : 1)
+    rows_to_q8_kernel(const NormArgs a) {
+  __shared__ float buf[128];
+  const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+  const int threads = WARP ? 32 : (int)blockDim.x;
+  const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  const T* X = static_cast<const T*>(a.X);
+  const T* R = static_cast<const T*>(a.R);
+  const int64_t N = a.N;
+  Vec<T, VEC> x[V], r[V];
+  auto fetch = [&](int64_t m) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = load_vec<T, VEC>(X + m * a.ldx, ((int64_t)i * threads + tid) * VEC, N);
+    if (NORM && R)
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = load_vec<T, VEC>(R + m * a.ldr, ((int64_t)i * threads + tid) * VEC, N);
+  };
+  if (AHEAD && first < a.M) fetch(first);
+  int parity = 0;
+  for (int64_t m = first; m < a.M; m += step, parity ^= 1) {
+    if (!AHEAD) fetch(m);
+    float v[V][VEC];
+    float ss = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int64_t n = ((int64_t)i * threads + tid) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = to_f(x[i].e[j]);
+      if constexpr (NORM) {
+        if (R) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] += to_f(r[i].e[j]);
+        }
+        if (a.H) {
+          Vec<T, VEC> h;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) from_f(&h.e[j], v[i][j]);
+          store_vec<T, VEC>(static_cast<T*>(a.H) + m * a.ldh, n, N, h);
+        }
+        float w[VEC];
+        load_weights<VEC>(a.W, a.w_dtype, n, N, w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          ss = fmaf(v[i][j], v[i][j], ss);
+          v[i][j] *= w[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+    }
+    if (AHEAD && m + step < a.M) fetch(m + step);
+    row_reduce<WARP>(ss, top, buf, parity);
+    const float rstd = NORM ? 1.0f / sqrtf(ss / (float)N + a.eps) : 1.0f;
+    const RowQuant rq = row_quant(top, rstd, q_max(a.q_dtype), a.pow2);
+    if (tid == 0) {
+      a.scale[m] = rq.scale;
+      if (NORM && a.rstd) a.rstd[m] = rstd;
+    }
+    const bool bad = rq.scale != rq.scale;
+    uint8_t* q = static_cast<uint8_t*>(a.Q) + m * a.ldq;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      Vec<uint8_t, VEC> o;
+      pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
+      store_vec<uint8_t, VEC>(q, ((int64_t)i * threads + tid) * VEC, N, o);
+    }
+  }
+}
+
+// The same for rows too long for a block's registers: two passes over the row, element by element.
+__global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const NormArgs a) {
   __shared__ float buf[kRowThreads / 32];
   for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
     auto value = [&](int64_t n) {
@@ -84,13 +264,30 @@ __global__ void __launch_bounds__(kRowThreads) rows_to_q8_kernel(const NormArgs 
   }
 }
 
+// Rows out of 8 bits: VEC values a thread and piece, pieces of a row `gridDim`-strided over the whole
+// matrix.  Memory-bound: 1 byte in, 2 or 4 out.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kRowThreads)
-    dequantize_kernel(const void* Q, const float* scale, void* X, int64_t M, int64_t N, int64_t ldq,
-                      int64_t ldx, int q_dtype, int dtype) {
-  for (int64_t m = blockIdx.x; m < M; m += gridDim.x) {
-    const float s = scale[m];
-    for (int64_t n = threadIdx.x; n < N; n += blockDim.x) {
-      store_elem(X, m * ldx + n, dtype, clamp_to(load_elem(Q, m * ldq + n, q_dtype) * s, largest(dtype)));
+    dequantize_kernel(const uint8_t* Q, const float* scale, T* X, int64_t M, int64_t N, int64_t ldq,
+                      int64_t ldx, int q_dtype, float top) {
+  const int64_t per_row = (N + VEC - 1) / VEC;
+  const int64_t bpr = (per_row + kRowThreads - 1) / kRowThreads;  // block pieces of a row
+  for (int64_t b = blockIdx.x; b < M * bpr; b += gridDim.x) {
+    const int64_t m = b / bpr, n = ((b - m * bpr) * kRowThreads + threadIdx.x) * VEC;
+    if (n >= N) continue;
+    const float s = __ldg(scale + m);
+    const Vec<uint8_t, VEC> q = load_vec<uint8_t, VEC>(Q + m * ldq, n, N);
+    constexpr int OUT = VEC < 16 / (int)sizeof(T) ? VEC : 16 / (int)sizeof(T);  // values per store
+#pragma unroll
+    for (int i = 0; i < VEC; i += OUT) {
+      Vec<T, OUT> o;
+#pragma unroll
+      for (int j = 0; j < OUT; ++j) {
+        const uint8_t c = q.e[i + j];
+        const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c));
+        from_f(&o.e[j], clamp_to(v * s, top));
+      }
+      if (n + i < N) store_vec<T, OUT>(X + m * ldx, n + i, N, o);
     }
   }
 }
@@ -152,12 +349,72 @@ int check_rows(int64_t M, int64_t N, std::initializer_list<int64_t> lds) {
   return B2G_OK;
 }
 
+bool aligned(const void* p, int64_t pitch_bytes, int64_t rows, int to) {
+  return ((uintptr_t)p % to) == 0 && (rows == 1 || pitch_bytes % to == 0);
+}
+
+// One launch of rows_to_q8_kernel: as many resident blocks as the GPU holds, at most one a row.
+template <typename T, bool NORM, int VEC, int V, bool WARP, bool AHEAD = true>
+int launch_rows(const NormArgs& a, int threads, int sms, cudaStream_t s) {
+  const int per_block = WARP ? threads / 32 : 1;
+  const int64_t need = (a.M + per_block - 1) / per_block;
+  const int64_t cap = (int64_t)sms * std::max(1, 1024 / threads);
+  rows_to_q8_kernel<T, NORM, VEC, V, WARP, AHEAD><<<(unsigned)std::min(need, cap), threads, 0, s>>>(a);
+  return launched("rows_to_q8_kernel");
+}
+
+// Vectors of 16 bytes where every address and pitch allows, else single elements; short rows one a
+// warp.  A thread holds as many vectors as keep the block at 256 threads, up to 4 of them.
+template <typename T, bool NORM>
+int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int es = (int)sizeof(T);
+  const bool vec = aligned(a.X, a.ldx * es, a.M, 16) && (!a.R || aligned(a.R, a.ldr * es, a.M, 16)) &&
+                   (!a.H || aligned(a.H, a.ldh * es, a.M, 16)) && aligned(a.Q, a.ldq, a.M, VEC);
+  if (vec) {
+    const int64_t nv = (a.N + VEC - 1) / VEC;
+    if (nv <= 32) return launch_rows<T, NORM, VEC, 1, true>(a, 128, sms, s);
+    if (nv <= 64) return launch_rows<T, NORM, VEC, 2, true>(a, 128, sms, s);
+    if (nv <= 128) return launch_rows<T, NORM, VEC, 4, true>(a, 128, sms, s);
+    if (nv <= 256) return launch_rows<T, NORM, VEC, 1, false>(a, (int)(nv + 31) / 32 * 32, sms, s);
+    if (nv <= 512) return launch_rows<T, NORM, VEC, 2, false>(a, (int)(nv + 63) / 64 * 32, sms, s);
+    if (nv <= 1024) return launch_rows<T, NORM, VEC, 4, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
+    if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, false, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
+  } else {
+    if (a.N <= 32 * 16) return launch_rows<T, NORM, 1, 16, true>(a, 128, sms, s);
+    if (a.N <= 256 * 16) return launch_rows<T, NORM, 1, 16, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
+    if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, false, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
+  }
+  long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
+  return launched("long_rows_to_q8_kernel");
+}
+
 int rows_to_q8(const NormArgs& a, cudaStream_t s) {
   int dev = 0, sms = 0, cc = 0;
   const int rc = current_device(&dev, &sms, &cc);
   if (rc != B2G_OK) return rc;
-  rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
-  return launched("rows_to_q8_kernel");
+  switch (a.dtype) {
+    case B2G_DTYPE_F16:
+      return a.norm ? rows_of<__half, true>(a, sms, s) : rows_of<__half, false>(a, sms, s);
+    case B2G_DTYPE_BF16:
+      return a.norm ? rows_of<__nv_bfloat16, true>(a, sms, s) : rows_of<__nv_bfloat16, false>(a, sms, s);
+    default:
+      return a.norm ? rows_of<float, true>(a, sms, s) : rows_of<float, false>(a, sms, s);
+  }
+}
+
+template <typename T>
+int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N, int64_t ldq, int64_t ldx,
+                  int q_dtype, float top, int sms, cudaStream_t s) {
+  const uint8_t* q = static_cast<const uint8_t*>(Q);
+  const bool vec = aligned(Q, ldq, M, 16) && aligned(X, ldx * (int64_t)sizeof(T), M, 16);
+  const int64_t per_row = (N + (vec ? 15 : 0)) / (vec ? 16 : 1);
+  const int64_t blocks = std::min<int64_t>(M * ((per_row + kRowThreads - 1) / kRowThreads), (int64_t)sms * 1024);
+  if (vec)
+    dequantize_kernel<T, 16><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
+  else
+    dequantize_kernel<T, 1><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
+  return launched("dequantize_kernel");
 }
 
 }  // namespace
@@ -167,9 +424,16 @@ int dequantize_rows(const void* Q, const float* scale, void* X, int64_t M, int64
   int dev = 0, sms = 0, cc = 0;
   const int rc = current_device(&dev, &sms, &cc);
   if (rc != B2G_OK) return rc;
-  dequantize_kernel<<<row_blocks(M, sms), kRowThreads, 0, s>>>(Q, scale, X, M, N, ldq, ldx, q_dtype,
-                                                               dtype);
-  return launched("dequantize_kernel");
+  switch (dtype) {
+    case B2G_DTYPE_F16:
+      return dequantize_to(Q, scale, static_cast<__half*>(X), M, N, ldq, ldx, q_dtype, 65504.0f, sms, s);
+    case B2G_DTYPE_BF16:
+      return dequantize_to(Q, scale, static_cast<__nv_bfloat16*>(X), M, N, ldq, ldx, q_dtype,
+                           0x1.fep127f, sms, s);
+    default:
+      return dequantize_to(Q, scale, static_cast<float*>(X), M, N, ldq, ldx, q_dtype, 0x1.fffffep127f,
+                           sms, s);
+  }
 }
 
 }  // namespace b2g

@@ -1447,12 +1447,14 @@ extern "C" int b2g_device_status(int clear) {
     return -1;
   }
   if (v == 0) v = vs;
-  const int qe = q8_device_error(clear, &vs);  // the 8-bit layer's kernels
-  if (qe != 0) {
-    fail(B2G_ERR_CUDA, "read 8-bit layer error word: %s", cudaGetErrorString((cudaError_t)qe));
-    return -1;
+  for (auto word : {q8_device_error, rows_device_error}) {  // the 8-bit layer's kernels
+    const int qe = word(clear, &vs);
+    if (qe != 0) {
+      fail(B2G_ERR_CUDA, "read 8-bit layer error word: %s", cudaGetErrorString((cudaError_t)qe));
+      return -1;
+    }
+    if (v == 0) v = vs;
   }
-  if (v == 0) v = vs;
   if (clear) {
     if (v != 0) ring_mark_dirty();  // a kernel that gave up may have left counters set
     const int z = 0;

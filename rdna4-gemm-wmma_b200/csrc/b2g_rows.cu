@@ -3,16 +3,33 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/b2g_gemm.h"
 #include "errors.h"
 #include "host.h"
+#include "ptx.cuh"
 #include "q8.cuh"
 
 namespace b2g {
+
+// First bounded wait of the row kernels that gave up (0: none), merged into b2g_device_status().
+static __device__ int g_rows_error;
+
+int rows_device_error(int clear, int* value) {
+  cudaError_t e = cudaMemcpyFromSymbol(value, g_rows_error, sizeof(int));
+  if (e == cudaSuccess && clear) {
+    const int z = 0;
+    e = cudaMemcpyToSymbol(g_rows_error, &z, sizeof(int));
+  }
+  return (int)e;
+}
+
 namespace {
 
 using namespace q8;
+
+constexpr int ERR_WAIT_ROW = 8;  // a row's bulk copy did not arrive
 
 constexpr int kRowThreads = 256;
 
@@ -62,66 +79,80 @@ __device__ __forceinline__ void from_f(__half* d, float v) { *d = __float2half_r
 __device__ __forceinline__ void from_f(__nv_bfloat16* d, float v) { *d = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_f(float* d, float v) { *d = v; }
 
-// Elements [n, n + VEC) of a row of N; elements past the row are not touched and read as zero.
+// Elements [n, n + VEC) of a row of N (a multiple of VEC), zeros past the row.  One predicated load: a
+// branch with an element-wise end would make every load wait for the one before it.
 template <typename T, int VEC>
-__device__ __forceinline__ Vec<T, VEC> load_vec(const T* row, int64_t n, int64_t N) {
+__device__ __forceinline__ Vec<T, VEC> load_vec(const T* row, int n, int N) {
   Vec<T, VEC> v;
-  if (n + VEC <= N) {
-    if constexpr (sizeof(v) == 16) {  // read once: do not displace the weights from L1
-      *reinterpret_cast<uint4*>(&v) = __ldcs(reinterpret_cast<const uint4*>(row + n));
-    } else {
-      v = *reinterpret_cast<const Vec<T, VEC>*>(row + n);
-    }
+  if constexpr (sizeof(v) == 16) {  // read once: do not displace the weights from L1
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (n < N) u = __ldcs(reinterpret_cast<const uint4*>(row + n));
+    *reinterpret_cast<uint4*>(&v) = u;
+  } else if constexpr (sizeof(v) == 8) {
+    uint2 u = make_uint2(0, 0);
+    if (n < N) u = __ldcs(reinterpret_cast<const uint2*>(row + n));
+    *reinterpret_cast<uint2*>(&v) = u;
   } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      v.e[j] = n + j < N ? row[n + j] : T(0.0f);
+    static_assert(VEC == 1 || sizeof(v) == 4, "vector size");
+    if constexpr (sizeof(v) == 4) {
+      uint32_t u = 0;
+      if (n < N) u = *reinterpret_cast<const uint32_t*>(row + n);
+      *reinterpret_cast<uint32_t*>(&v) = u;
+    } else if constexpr (sizeof(v) == 2) {
+      uint16_t u = 0;
+      if (n < N) u = *reinterpret_cast<const uint16_t*>(row + n);
+      *reinterpret_cast<uint16_t*>(&v) = u;
+    } else {
+      uint8_t u = 0;
+      if (n < N) u = *reinterpret_cast<const uint8_t*>(row + n);
+      *reinterpret_cast<uint8_t*>(&v) = u;
     }
   }
   return v;
 }
 
 template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* row, int64_t n, int64_t N, const Vec<T, VEC>& v) {
-  if (n + VEC <= N) {
-    *reinterpret_cast<Vec<T, VEC>*>(row + n) = v;
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (n + j < N) row[n + j] = v.e[j];
-  }
+__device__ __forceinline__ void store_vec(T* row, int n, int N, const Vec<T, VEC>& v) {
+  if (n < N) *reinterpret_cast<Vec<T, VEC>*>(row + n) = v;
 }
 
 // VEC weights as fp32 (any type; cached in L1 for the block's next row).
 template <int VEC>
-__device__ __forceinline__ void load_weights(const void* W, int w_dtype, int64_t n, int64_t N, float (&w)[VEC]) {
-  const int size = w_dtype == B2G_DTYPE_F32 ? 4 : 2;
-  if (VEC >= 4 && n + VEC <= N && (reinterpret_cast<uintptr_t>(W) & (4 * size - 1)) == 0) {
+__device__ __forceinline__ void load_weights(const void* W, int w_dtype, bool vec, int n, int N, float (&w)[VEC]) {
+  if constexpr (VEC >= 4) {
+    if (vec) {
 #pragma unroll
-    for (int j = 0; j < VEC; j += 4) {  // four at a time: 16 bytes of fp32, 8 of the 16-bit types
-      if (size == 4) {
-        const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(W) + n + j));
-        w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
-      } else {
-        const uint2 x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(W) + n + j));
-        const uint32_t b[2] = {x.x, x.y};
+      for (int j = 0; j < VEC; j += 4) {  // four at a time: 16 bytes of fp32, 8 of the 16-bit types
+        if (w_dtype == B2G_DTYPE_F32) {
+          float4 x = make_float4(0, 0, 0, 0);
+          if (n < N) x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(W) + n + j));
+          w[j] = x.x; w[j + 1] = x.y; w[j + 2] = x.z; w[j + 3] = x.w;
+        } else {
+          uint2 x = make_uint2(0, 0);
+          if (n < N) x = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(W) + n + j));
+          const uint32_t b[2] = {x.x, x.y};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          if (w_dtype == B2G_DTYPE_BF16) {
-            w[j + 2 * k] = __uint_as_float(b[k] << 16);
-            w[j + 2 * k + 1] = __uint_as_float(b[k] & 0xffff0000u);
-          } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[k]));
-            w[j + 2 * k] = f.x;
-            w[j + 2 * k + 1] = f.y;
+          for (int k = 0; k < 2; ++k) {
+            if (w_dtype == B2G_DTYPE_BF16) {
+              w[j + 2 * k] = __uint_as_float(b[k] << 16);
+              w[j + 2 * k + 1] = __uint_as_float(b[k] & 0xffff0000u);
+            } else {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[k]));
+              w[j + 2 * k] = f.x;
+              w[j + 2 * k + 1] = f.y;
+            }
           }
         }
       }
+      return;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[j] = n + j < N ? load_elem(W, n + j, w_dtype) : 0.0f;
   }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) w[j] = n + j < N ? load_elem(W, n + j, w_dtype) : 0.0f;
+}
+
+__device__ __forceinline__ bool weights_vec(const void* W, int w_dtype) {
+  return (reinterpret_cast<uintptr_t>(W) & (w_dtype == B2G_DTYPE_F32 ? 15 : 7)) == 0;
 }
 
 // (sum, integer maximum) over the threads of a row: a warp, or the block.  `buf` holds two words
@@ -167,14 +198,15 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
   const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
   const T* X = static_cast<const T*>(a.X);
   const T* R = static_cast<const T*>(a.R);
-  const int64_t N = a.N;
+  const int N = (int)a.N;
+  const bool wvec = NORM && weights_vec(a.W, a.w_dtype);
   Vec<T, VEC> x[V], r[V];
   auto fetch = [&](int64_t m) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = load_vec<T, VEC>(X + m * a.ldx, ((int64_t)i * threads + tid) * VEC, N);
+    for (int i = 0; i < V; ++i) x[i] = load_vec<T, VEC>(X + m * a.ldx, (i * threads + tid) * VEC, N);
     if (NORM && R)
 #pragma unroll
-      for (int i = 0; i < V; ++i) r[i] = load_vec<T, VEC>(R + m * a.ldr, ((int64_t)i * threads + tid) * VEC, N);
+      for (int i = 0; i < V; ++i) r[i] = load_vec<T, VEC>(R + m * a.ldr, (i * threads + tid) * VEC, N);
   };
   if (AHEAD && first < a.M) fetch(first);
   int parity = 0;
@@ -185,7 +217,7 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int64_t n = ((int64_t)i * threads + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[i][j] = to_f(x[i].e[j]);
       if constexpr (NORM) {
@@ -200,7 +232,7 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
           store_vec<T, VEC>(static_cast<T*>(a.H) + m * a.ldh, n, N, h);
         }
         float w[VEC];
-        load_weights<VEC>(a.W, a.w_dtype, n, N, w);
+        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           ss = fmaf(v[i][j], v[i][j], ss);
@@ -224,9 +256,158 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
     for (int i = 0; i < V; ++i) {
       Vec<uint8_t, VEC> o;
       pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
-      store_vec<uint8_t, VEC>(q, ((int64_t)i * threads + tid) * VEC, N, o);
+      store_vec<uint8_t, VEC>(q, (i * threads + tid) * VEC, N, o);
     }
   }
+}
+
+// VEC 16-byte-aligned elements from shared memory as fp32.
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const uint8_t* p, float (&v)[VEC]) {
+  const Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(p);
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[j] = to_f(x.e[j]);
+}
+
+// A ring of row buffers in shared memory, filled by bulk copies: one ring a row owner (a warp, or the
+// block).  `full` barriers count the bytes of each buffer; the owner's leader refills a buffer once
+// every thread of the owner has read it.  Copies run ahead of the rows by up to `stages`, which
+// keeps the memory busy however long a row's reduction takes, and costs no registers.  A wait that
+// runs out marks the CTA, later waits return at once, and its rows come out as NaN.
+struct Ring {
+  uint32_t base, bars, stage_bytes;
+  int stages;
+  volatile int* abort_flag;
+  uint64_t limit_ns;
+  __device__ __forceinline__ uint32_t stage(int k) const { return base + (uint32_t)(k % stages) * stage_bytes; }
+  __device__ __forceinline__ uint32_t bar(int k) const { return bars + 8u * (uint32_t)(k % stages); }
+  __device__ __forceinline__ bool wait(int k) const {
+    return ptx::mbar_wait(bar(k), (uint32_t)(k / stages) & 1u, abort_flag, &g_rows_error, ERR_WAIT_ROW, limit_ns);
+  }
+};
+
+// Sets up `owners` rings of `stages` buffers in dynamic shared memory and returns this thread's.
+__device__ __forceinline__ Ring make_ring(uint8_t* smem, int owners, int owner, int stages,
+                                          uint32_t stage_bytes, uint64_t limit_ns, int* abort_flag) {
+  const uint32_t base = ptx::smem_u32(smem), bars = base + (uint32_t)(owners * stages) * stage_bytes;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < owners * stages; ++i) ptx::mbar_init(bars + 8u * i, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  __syncthreads();
+  return {base + (uint32_t)(owner * stages) * stage_bytes, bars + 8u * (uint32_t)(owner * stages), stage_bytes,
+          stages, abort_flag, limit_ns};
+}
+
+constexpr int kRingThreads = 256;
+
+// rows_to_q8_kernel with its rows in a ring (16-byte rows, at least a few rows an owner).  A thread
+// holds V vectors of a row; the norm's weights stay in its registers where V <= 4.
+template <typename T, bool NORM, int V, bool WARP>
+__global__ void __launch_bounds__(kRingThreads, 2)
+    rows_ring_kernel(const NormArgs a, int stages, uint32_t row_bytes, uint64_t limit_ns) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr bool WREG = NORM && V <= 4;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float buf[128];
+  __shared__ int abort_flag;
+  const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
+  const int threads = WARP ? 32 : kRingThreads;
+  const int owners = WARP ? kRingThreads / 32 : 1, owner = WARP ? (int)(threadIdx.x >> 5) : 0;
+  const int64_t first = (int64_t)blockIdx.x * owners + owner, step = (int64_t)gridDim.x * owners;
+  const T* X = static_cast<const T*>(a.X);
+  const T* R = NORM ? static_cast<const T*>(a.R) : nullptr;
+  const int N = (int)a.N;
+  const uint32_t r_off = row_bytes;  // R's row follows X's in a stage
+  const Ring ring = make_ring(smem, owners, owner, stages, R ? 2 * row_bytes : row_bytes, limit_ns, &abort_flag);
+  const uint8_t* const ring_ptr = smem + (ring.base - ptx::smem_u32(smem));
+  auto fill = [&](int64_t m, int k) {
+    const uint32_t bar = ring.bar(k), dst = ring.stage(k);
+    ptx::mbar_arrive_expect_tx(bar, R ? 2 * row_bytes : row_bytes);
+    ptx::bulk_load(dst, X + m * a.ldx, row_bytes, bar);
+    if (R) ptx::bulk_load(dst + r_off, R + m * a.ldr, row_bytes, bar);
+  };
+  int issued = 0;
+  if (tid == 0)
+    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+  const bool wvec = NORM && weights_vec(a.W, a.w_dtype);
+  float wreg[WREG ? V : 1][VEC];
+  if constexpr (WREG)
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, wreg[i]);
+  int k = 0;
+  for (int64_t m = first; m < a.M; m += step, ++k) {
+    const bool ok = ring.wait(k);
+    const uint8_t* st = ring_ptr + (uint32_t)(k % stages) * ring.stage_bytes;
+    float v[V][VEC];
+    F2 ss = f2(0.0f, 0.0f);
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = (i * threads + tid) * VEC;
+      if (n < N) {
+        unpack<T, VEC>(st + n * (int)sizeof(T), v[i]);
+        if constexpr (NORM) {
+          if (R) {
+            float r[VEC];
+            unpack<T, VEC>(st + r_off + n * (int)sizeof(T), r);
+#pragma unroll
+            for (int j = 0; j < VEC; j += 2)
+              f2_get(f2_add(f2(v[i][j], v[i][j + 1]), f2(r[j], r[j + 1])), v[i][j], v[i][j + 1]);
+          }
+          if (a.H) {
+            Vec<T, VEC> h;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) from_f(&h.e[j], v[i][j]);
+            *reinterpret_cast<Vec<T, VEC>*>(static_cast<T*>(a.H) + m * a.ldh + n) = h;
+          }
+          float wl[VEC];
+          if constexpr (!WREG) load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, wl);
+#pragma unroll
+          for (int j = 0; j < VEC; j += 2) {
+            const F2 h = f2(v[i][j], v[i][j + 1]);
+            ss = f2_fma(h, h, ss);
+            const F2 w = WREG ? f2(wreg[WREG ? i : 0][j], wreg[WREG ? i : 0][j + 1]) : f2(wl[j], wl[j + 1]);
+            f2_get(f2_mul(h, w), v[i][j], v[i][j + 1]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) top = max_abs(top, v[i][j]);
+      }
+    }
+    float s0, s1;
+    f2_get(ss, s0, s1);
+    float sum = s0 + s1;
+    uint32_t bits = ok ? __float_as_uint(top) : 0x7fffffffu;
+    row_reduce<WARP>(sum, bits, buf, k & 1);
+    if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
+      fill(m + step * stages, k + stages);  // every thread has read this row (row_reduce)
+      ++issued;
+    }
+    const float rstd = NORM ? 1.0f / sqrtf(sum / (float)N + a.eps) : 1.0f;
+    const RowQuant rq = row_quant(bits, rstd, q_max(a.q_dtype), a.pow2);
+    if (tid == 0) {
+      a.scale[m] = rq.scale;
+      if (NORM && a.rstd) a.rstd[m] = rstd;
+    }
+    const bool bad = rq.scale != rq.scale;
+    uint8_t* q = static_cast<uint8_t*>(a.Q) + m * a.ldq;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = (i * threads + tid) * VEC;
+      if (n < N) {
+        Vec<uint8_t, VEC> o;
+        pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
+        *reinterpret_cast<Vec<uint8_t, VEC>*>(q + n) = o;
+      }
+    }
+  }
+  // no copy may be in flight when the CTA's shared memory goes away (only after a wait gave up)
+  if (tid == 0 && *ring.abort_flag)
+    for (int i = max(0, issued - stages); i < issued; ++i)
+      ptx::mbar_wait_drain(ring.bar(i), (uint32_t)(i / stages) & 1u, &g_rows_error, ERR_WAIT_ROW, limit_ns);
 }
 
 // The same for rows too long for a block's registers: two passes over the row, element by element.
@@ -276,18 +457,25 @@ __global__ void __launch_bounds__(kRowThreads)
     const int64_t m = b / bpr, n = ((b - m * bpr) * kRowThreads + threadIdx.x) * VEC;
     if (n >= N) continue;
     const float s = __ldg(scale + m);
-    const Vec<uint8_t, VEC> q = load_vec<uint8_t, VEC>(Q + m * ldq, n, N);
-    constexpr int OUT = VEC < 16 / (int)sizeof(T) ? VEC : 16 / (int)sizeof(T);  // values per store
+    auto value = [&](uint8_t c) {
+      const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c));
+      return clamp_to(v * s, top);
+    };
+    const uint8_t* q = Q + m * ldq + n;
+    T* x = X + m * ldx + n;
+    if (VEC > 1 && n + VEC <= N) {
+      const Vec<uint8_t, VEC> c = *reinterpret_cast<const Vec<uint8_t, VEC>*>(q);
+      constexpr int OUT = VEC < 16 / (int)sizeof(T) ? VEC : 16 / (int)sizeof(T);  // values per store
 #pragma unroll
-    for (int i = 0; i < VEC; i += OUT) {
-      Vec<T, OUT> o;
+      for (int i = 0; i < VEC; i += OUT) {
+        Vec<T, OUT> o;
 #pragma unroll
-      for (int j = 0; j < OUT; ++j) {
-        const uint8_t c = q.e[i + j];
-        const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c));
-        from_f(&o.e[j], clamp_to(v * s, top));
+        for (int j = 0; j < OUT; ++j) from_f(&o.e[j], value(c.e[i + j]));
+        *reinterpret_cast<Vec<T, OUT>*>(x + i) = o;
       }
-      if (n + i < N) store_vec<T, OUT>(X + m * ldx, n + i, N, o);
+    } else {
+      const int count = N - n < VEC ? (int)(N - n) : VEC;
+      for (int j = 0; j < count; ++j) from_f(x + j, value(q[j]));
     }
   }
 }
@@ -363,16 +551,56 @@ int launch_rows(const NormArgs& a, int threads, int sms, cudaStream_t s) {
   return launched("rows_to_q8_kernel");
 }
 
+// A launch of rows_ring_kernel, or false where its stages do not fit or a row owner would have too few
+// rows for the ring to matter.
+template <typename T, bool NORM, int V, bool WARP>
+bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
+  const int owners = WARP ? kRingThreads / 32 : 1;
+  const uint32_t row_bytes = (uint32_t)(a.N * (int64_t)sizeof(T));
+  const uint32_t stage = (a.R ? 2 : 1) * row_bytes;
+  constexpr uint32_t kBudget = 112 * 1024;  // two CTAs an SM
+  const int stages = (int)std::min<uint32_t>(4, (kBudget - 1024) / (owners * stage));
+  if (stages < 2) return false;
+  const int64_t blocks = std::min<int64_t>((a.M + owners - 1) / owners, (int64_t)sms * 2);
+  if (a.M < blocks * owners * 2) return false;
+  const uint32_t smem = (uint32_t)(owners * stages) * (stage + 8);
+  auto fn = rows_ring_kernel<T, NORM, V, WARP>;
+  static std::atomic<uint64_t> ready{0};  // devices whose limit was raised
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBudget);
+    if (e == cudaSuccess) ready |= 1ull << dev;
+  }
+  if (e != cudaSuccess) {
+    *rc = cuda_fail(e, "cudaFuncSetAttribute(smem)");
+    return true;
+  }
+  fn<<<(unsigned)blocks, kRingThreads, smem, s>>>(a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
+  *rc = launched("rows_ring_kernel");
+  return true;
+}
+
 // Vectors of 16 bytes where every address and pitch allows, else single elements; short rows one a
 // warp.  A thread holds as many vectors as keep the block at 256 threads, up to 4 of them.
 template <typename T, bool NORM>
 int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int es = (int)sizeof(T);
-  const bool vec = aligned(a.X, a.ldx * es, a.M, 16) && (!a.R || aligned(a.R, a.ldr * es, a.M, 16)) &&
+  const bool vec = a.N % VEC == 0 && aligned(a.X, a.ldx * es, a.M, 16) && (!a.R || aligned(a.R, a.ldr * es, a.M, 16)) &&
                    (!a.H || aligned(a.H, a.ldh * es, a.M, 16)) && aligned(a.Q, a.ldq, a.M, VEC);
   if (vec) {
-    const int64_t nv = (a.N + VEC - 1) / VEC;
+    const int64_t nv = a.N / VEC;
+    int rc = B2G_OK;
+    if (nv <= 32 ? launch_ring<T, NORM, 1, true>(a, sms, s, &rc)
+        : nv <= 64 ? launch_ring<T, NORM, 2, true>(a, sms, s, &rc)
+        : nv <= 128 ? launch_ring<T, NORM, 4, true>(a, sms, s, &rc)
+        : nv <= 256 ? launch_ring<T, NORM, 1, false>(a, sms, s, &rc)
+        : nv <= 512 ? launch_ring<T, NORM, 2, false>(a, sms, s, &rc)
+        : nv <= 1024 ? launch_ring<T, NORM, 4, false>(a, sms, s, &rc)
+        : nv <= 2048 ? launch_ring<T, NORM, 8, false>(a, sms, s, &rc)
+                     : false)
+      return rc;
     if (nv <= 32) return launch_rows<T, NORM, VEC, 1, true>(a, 128, sms, s);
     if (nv <= 64) return launch_rows<T, NORM, VEC, 2, true>(a, 128, sms, s);
     if (nv <= 128) return launch_rows<T, NORM, VEC, 4, true>(a, 128, sms, s);
@@ -381,8 +609,9 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
     if (nv <= 1024) return launch_rows<T, NORM, VEC, 4, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
     if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, false, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
   } else {
-    if (a.N <= 32 * 16) return launch_rows<T, NORM, 1, 16, true>(a, 128, sms, s);
-    if (a.N <= 256 * 16) return launch_rows<T, NORM, 1, 16, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
+    if (a.N <= 32 * 8) return launch_rows<T, NORM, 1, 8, true>(a, 128, sms, s);
+    if (a.N <= 256 * 8) return launch_rows<T, NORM, 1, 8, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
+    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, false, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
     if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, false, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
   }
   long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);

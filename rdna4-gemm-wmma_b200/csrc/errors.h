@@ -12,6 +12,7 @@ void count_launch();
 int shard_device_error(int clear, int* value);
 // The same for the kernels of the 8-bit linear layer (b2g_q8.cu).
 int q8_device_error(int clear, int* value);
+int rows_device_error(int clear, int* value);  // ... and of its row kernels (b2g_rows.cu)
 // Options of the multi-GPU entry points (b2g_set_option "comm_timeout_ms", "comm_nonblocking").
 int64_t comm_timeout_ms();
 bool comm_nonblocking();

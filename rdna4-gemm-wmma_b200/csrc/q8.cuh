@@ -40,6 +40,41 @@ __device__ __forceinline__ float clamp_to(float v, float top) {
   return v > top ? top : v < -top ? -top : v;
 }
 
+// Two fp32 values in one register pair: sm_100 multiplies, adds and fuses pairs in one instruction,
+// which matters where a row kernel's instructions, not its bytes, are the limit.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_get(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+// max(top, |v|), NaN if either is (so that a row's largest value tells of every NaN in it).
+__device__ __forceinline__ float max_abs(float top, float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(top), "f"(fabsf(v)));
+  return r;
+}
+
 // How the elements v of a row become 8-bit values t.  v is first scaled by a power of two that brings
 // the row's largest value near 1 (exact, and no later product overflows); then
 //   without pow2   t = v * qmax / amax, the quotient correctly rounded: for 16-bit v it often lies
@@ -109,29 +144,40 @@ __device__ __forceinline__ void pack_q8(const float (&v)[N], const RowQuant& r, 
                                         uint8_t (&o)[N]) {
   if constexpr (N % 4 == 0) {
     uint32_t* w = reinterpret_cast<uint32_t*>(o);
-    float t[N];
+    const F2 mul = f2(r.mul, r.mul), rcp = f2(r.rcp, r.rcp), nden = f2(-r.den, -r.den);
+    F2 t[N / 2];
     if (r.den == 0.0f) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) t[j] = v[j] * r.mul * r.rcp;
+      for (int j = 0; j < N / 2; ++j) t[j] = f2_mul(f2_mul(f2(v[2 * j], v[2 * j + 1]), mul), rcp);
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) t[j] = quotient(v[j], r);
+      for (int j = 0; j < N / 2; ++j) {  // quotient(), two at a time
+        const F2 a = f2_mul(f2(v[2 * j], v[2 * j + 1]), mul);
+        const F2 q = f2_mul(a, rcp);
+        t[j] = f2_fma(f2_fma(q, nden, a), rcp, q);
+      }
     }
     if (q_dtype == B2G_DTYPE_I8) {
       // 1.5 * 2^23 added: the sum's unit is 1, so the addition rounds t to an integer (to nearest
       // even) and leaves its two's complement in the low byte
+      const F2 magic = f2(12582912.0f, 12582912.0f);
 #pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        const uint32_t a = __float_as_uint(t[j] + 12582912.0f), b = __float_as_uint(t[j + 1] + 12582912.0f);
-        const uint32_t c = __float_as_uint(t[j + 2] + 12582912.0f), d = __float_as_uint(t[j + 3] + 12582912.0f);
-        w[j / 4] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+      for (int j = 0; j < N / 4; ++j) {
+        float a, b, c, d;
+        f2_get(f2_add(t[2 * j], magic), a, b);
+        f2_get(f2_add(t[2 * j + 1], magic), c, d);
+        w[j] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                           __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < N; j += 4) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[j], t[j + 1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[j + 2], t[j + 3]), __NV_SATFINITE, __NV_E4M3);
-        w[j / 4] = lo | hi << 16;
+      for (int j = 0; j < N / 4; ++j) {
+        float a, b, c, d;
+        f2_get(t[2 * j], a, b);
+        f2_get(t[2 * j + 1], c, d);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        w[j] = lo | hi << 16;
       }
     }
     if (bad) {

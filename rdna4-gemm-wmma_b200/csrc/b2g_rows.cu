@@ -155,47 +155,54 @@ __device__ __forceinline__ bool weights_vec(const void* W, int w_dtype) {
   return (reinterpret_cast<uintptr_t>(W) & (w_dtype == B2G_DTYPE_F32 ? 15 : 7)) == 0;
 }
 
-// (sum, integer maximum) over the threads of a row: a warp, or the block.  `buf` holds two words
-// per warp for each parity of the row count, so consecutive rows need one barrier each.
-template <bool WARP>
+// (sum, integer maximum) over the threads of a row: LANES consecutive lanes of a warp, or (LANES = 0)
+// the block.  `buf` holds two words per warp for each parity of the row count, so consecutive rows
+// need one barrier each.  SUM: whether the sum is wanted.
+template <int LANES, bool SUM>
 __device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, float* buf, int parity) {
+  constexpr int L = LANES ? LANES : 32;
+  if constexpr (SUM) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if constexpr (!WARP) {
+  if constexpr (L == 32) {
+    top = __reduce_max_sync(0xffffffffu, top);
+  } else {
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  if constexpr (LANES == 0) {
     float2* b = reinterpret_cast<float2*>(buf) + parity * 32;
     if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = make_float2(sum, __uint_as_float(top));
     __syncthreads();
     const int warps = (int)blockDim.x >> 5, lane = threadIdx.x & 31;
     const float2 x = lane < warps ? b[lane] : make_float2(0.0f, 0.0f);
-    sum = x.x;
-    top = __float_as_uint(x.y);
+    if constexpr (SUM) {
+      sum = x.x;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
+    top = __reduce_max_sync(0xffffffffu, __float_as_uint(x.y));
   }
 }
 
-// Rows into 8 bits, each row held in registers: one pass over the data.  A row belongs to a warp
-// (WARP: short rows) or to the block; a thread holds V vectors of VEC elements of it, `threads`
-// vectors apart.  Blocks stride over the rows; where registers allow (AHEAD: blocks of up to 256
-// threads) a row's loads are issued before the previous row is reduced, so that the reduction's
-// barrier is not waited out with the memory idle.
+// Rows into 8 bits, each row held in registers: one pass over the data.  A row belongs to LANES lanes of
+// a warp (short rows) or, LANES = 0, to the block; a thread holds V vectors of VEC elements of it,
+// `threads` vectors apart.  Blocks stride over the rows; where registers allow (AHEAD: blocks of up
+// to 256 threads) a row's loads are issued before the previous row is reduced, so that the
+// reduction is not waited out with the memory idle.
 //
 // Per row: sum of squares and largest |h * w| (|x| without the norm).  The largest |y| is rstd
 // times that, so one reduction serves both; rstd cancels from the 8-bit values (row_quant).
-template <typename T, bool NORM, int VEC, int V, bool WARP, bool AHEAD>
-__global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AHEAD ? 2 : 1)
+template <typename T, bool NORM, int VEC, int V, int LANES, bool AHEAD>
+__global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 5 : AHEAD ? 2 : 1)
     rows_to_q8_kernel(const NormArgs a) {
   __shared__ float buf[128];
-  const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-  const int threads = WARP ? 32 : (int)blockDim.x;
-  const int64_t first = WARP ? (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = WARP ? (int64_t)gridDim.x * (blockDim.x >> 5) : gridDim.x;
+  constexpr int PER = LANES ? 128 / LANES : 1;  // rows a block holds at once
+  const int tid = LANES ? (int)threadIdx.x % (LANES ? LANES : 1) : (int)threadIdx.x;
+  const int threads = LANES ? LANES : (int)blockDim.x;
+  const int64_t first = (int64_t)blockIdx.x * PER + (LANES ? (int)threadIdx.x / (LANES ? LANES : 1) : 0);
+  const int64_t step = (int64_t)gridDim.x * PER;
   const T* X = static_cast<const T*>(a.X);
   const T* R = static_cast<const T*>(a.R);
   const int N = (int)a.N;
@@ -210,8 +217,12 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
   };
   if (AHEAD && first < a.M) fetch(first);
   int parity = 0;
-  for (int64_t m = first; m < a.M; m += step, parity ^= 1) {
-    if (!AHEAD) fetch(m);
+  // (the lanes of a warp stay together: those whose rows have run out go on with the last row's
+  // values until the warp's first row is past the end, and store nothing)
+  const int64_t end = LANES ? a.M + (int64_t)(threadIdx.x % 32) / (LANES ? LANES : 1) : a.M;
+  for (int64_t m = first; m < end; m += step, parity ^= 1) {
+    const bool live = m < a.M;
+    if (!AHEAD && live) fetch(m);
     float v[V][VEC];
     float ss = 0.0f;
     uint32_t top = 0;
@@ -225,7 +236,7 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
 #pragma unroll
           for (int j = 0; j < VEC; ++j) v[i][j] += to_f(r[i].e[j]);
         }
-        if (a.H) {
+        if (a.H && live) {
           Vec<T, VEC> h;
 #pragma unroll
           for (int j = 0; j < VEC; ++j) from_f(&h.e[j], v[i][j]);
@@ -243,7 +254,8 @@ __global__ void __launch_bounds__(WARP ? 128 : AHEAD ? 256 : 1024, WARP ? 4 : AH
       for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
     }
     if (AHEAD && m + step < a.M) fetch(m + step);
-    row_reduce<WARP>(ss, top, buf, parity);
+    row_reduce<LANES, NORM>(ss, top, buf, parity);
+    if (!live) continue;
     const float rstd = NORM ? 1.0f / sqrtf(ss / (float)N + a.eps) : 1.0f;
     const RowQuant rq = row_quant(top, rstd, q_max(a.q_dtype), a.pow2);
     if (tid == 0) {
@@ -269,11 +281,11 @@ __device__ __forceinline__ void unpack(const uint8_t* p, float (&v)[VEC]) {
   for (int j = 0; j < VEC; ++j) v[j] = to_f(x.e[j]);
 }
 
-// A ring of row buffers in shared memory, filled by bulk copies: one ring a row owner (a warp, or the
-// block).  `full` barriers count the bytes of each buffer; the owner's leader refills a buffer once
-// every thread of the owner has read it.  Copies run ahead of the rows by up to `stages`, which
-// keeps the memory busy however long a row's reduction takes, and costs no registers.  A wait that
-// runs out marks the CTA, later waits return at once, and its rows come out as NaN.
+// A ring of row buffers in shared memory, filled by bulk copies.  `full` barriers count the bytes of each
+// buffer; thread 0 refills a buffer once every thread has read it.  Copies run ahead of the rows by
+// up to `stages`, which keeps the memory busy however long a row's reduction takes, and costs no
+// registers.  A wait that runs out marks the block, later waits return at once, and its rows come
+// out as NaN.
 struct Ring {
   uint32_t base, bars, stage_bytes;
   int stages;
@@ -284,45 +296,45 @@ struct Ring {
   __device__ __forceinline__ bool wait(int k) const {
     return ptx::mbar_wait(bar(k), (uint32_t)(k / stages) & 1u, abort_flag, &g_rows_error, ERR_WAIT_ROW, limit_ns);
   }
+  // After a wait gave up: no copy may be in flight when the shared memory goes away.
+  __device__ __forceinline__ void drain(int issued) const {
+    for (int i = max(0, issued - stages); i < issued; ++i)
+      ptx::mbar_wait_drain(bar(i), (uint32_t)(i / stages) & 1u, &g_rows_error, ERR_WAIT_ROW, limit_ns);
+  }
 };
 
-// Sets up `owners` rings of `stages` buffers in dynamic shared memory and returns this thread's.
-__device__ __forceinline__ Ring make_ring(uint8_t* smem, int owners, int owner, int stages,
-                                          uint32_t stage_bytes, uint64_t limit_ns, int* abort_flag) {
-  const uint32_t base = ptx::smem_u32(smem), bars = base + (uint32_t)(owners * stages) * stage_bytes;
+// A ring of `stages` buffers at the start of dynamic shared memory, its barriers behind them.
+__device__ __forceinline__ Ring make_ring(uint8_t* smem, int stages, uint32_t stage_bytes, uint64_t limit_ns,
+                                          int* abort_flag) {
+  const uint32_t base = ptx::smem_u32(smem), bars = base + (uint32_t)stages * stage_bytes;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < owners * stages; ++i) ptx::mbar_init(bars + 8u * i, 1);
+    for (int i = 0; i < stages; ++i) ptx::mbar_init(bars + 8u * i, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
   }
   __syncthreads();
-  return {base + (uint32_t)(owner * stages) * stage_bytes, bars + 8u * (uint32_t)(owner * stages), stage_bytes,
-          stages, abort_flag, limit_ns};
+  return {base, bars, stage_bytes, stages, abort_flag, limit_ns};
 }
 
-constexpr int kRingThreads = 256;
-
-// rows_to_q8_kernel with its rows in a ring (16-byte rows, at least a few rows an owner).  A thread
-// holds V vectors of a row; the norm's weights stay in its registers where V <= 4.
-template <typename T, bool NORM, int V, bool WARP>
-__global__ void __launch_bounds__(kRingThreads, 2)
+// rows_to_q8_kernel with its rows in a ring: rows of whole 16-byte vectors, one row at a time a block of
+// THREADS threads, which hold V vectors each.  The norm's weights stay in registers where V <= 4.
+// CTAS blocks share an SM, so that one's reduction overlaps the others' arithmetic.
+template <typename T, bool NORM, int V, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
     rows_ring_kernel(const NormArgs a, int stages, uint32_t row_bytes, uint64_t limit_ns) {
   constexpr int VEC = 16 / (int)sizeof(T);
   constexpr bool WREG = NORM && V <= 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float buf[128];
   __shared__ int abort_flag;
-  const int tid = WARP ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-  const int threads = WARP ? 32 : kRingThreads;
-  const int owners = WARP ? kRingThreads / 32 : 1, owner = WARP ? (int)(threadIdx.x >> 5) : 0;
-  const int64_t first = (int64_t)blockIdx.x * owners + owner, step = (int64_t)gridDim.x * owners;
+  const int tid = (int)threadIdx.x;
+  const int64_t first = blockIdx.x, step = gridDim.x;
   const T* X = static_cast<const T*>(a.X);
   const T* R = NORM ? static_cast<const T*>(a.R) : nullptr;
   const int N = (int)a.N;
   const uint32_t r_off = row_bytes;  // R's row follows X's in a stage
-  const Ring ring = make_ring(smem, owners, owner, stages, R ? 2 * row_bytes : row_bytes, limit_ns, &abort_flag);
-  const uint8_t* const ring_ptr = smem + (ring.base - ptx::smem_u32(smem));
+  const Ring ring = make_ring(smem, stages, R ? 2 * row_bytes : row_bytes, limit_ns, &abort_flag);
   auto fill = [&](int64_t m, int k) {
     const uint32_t bar = ring.bar(k), dst = ring.stage(k);
     ptx::mbar_arrive_expect_tx(bar, R ? 2 * row_bytes : row_bytes);
@@ -336,17 +348,17 @@ __global__ void __launch_bounds__(kRingThreads, 2)
   float wreg[WREG ? V : 1][VEC];
   if constexpr (WREG)
 #pragma unroll
-    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, wreg[i]);
+    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * THREADS + tid) * VEC, N, wreg[i]);
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
     const bool ok = ring.wait(k);
-    const uint8_t* st = ring_ptr + (uint32_t)(k % stages) * ring.stage_bytes;
+    const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     float v[V][VEC];
     F2 ss = f2(0.0f, 0.0f);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * threads + tid) * VEC;
+      const int n = (i * THREADS + tid) * VEC;
       if (n < N) {
         unpack<T, VEC>(st + n * (int)sizeof(T), v[i]);
         if constexpr (NORM) {
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     f2_get(ss, s0, s1);
     float sum = s0 + s1;
     uint32_t bits = ok ? __float_as_uint(top) : 0x7fffffffu;
-    row_reduce<WARP>(sum, bits, buf, k & 1);
+    row_reduce<0, NORM>(sum, bits, buf, k & 1);
     if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
       fill(m + step * stages, k + stages);  // every thread has read this row (row_reduce)
       ++issued;
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
     uint8_t* q = static_cast<uint8_t*>(a.Q) + m * a.ldq;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * threads + tid) * VEC;
+      const int n = (i * THREADS + tid) * VEC;
       if (n < N) {
         Vec<uint8_t, VEC> o;
         pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
@@ -404,10 +416,7 @@ __global__ void __launch_bounds__(kRingThreads, 2)
       }
     }
   }
-  // no copy may be in flight when the CTA's shared memory goes away (only after a wait gave up)
-  if (tid == 0 && *ring.abort_flag)
-    for (int i = max(0, issued - stages); i < issued; ++i)
-      ptx::mbar_wait_drain(ring.bar(i), (uint32_t)(i / stages) & 1u, &g_rows_error, ERR_WAIT_ROW, limit_ns);
+  if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
 // The same for rows too long for a block's registers: two passes over the row, element by element.
@@ -445,37 +454,60 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const Norm
   }
 }
 
-// Rows out of 8 bits: VEC values a thread and piece, pieces of a row `gridDim`-strided over the whole
-// matrix.  Memory-bound: 1 byte in, 2 or 4 out.
-template <typename T, int VEC>
+// Rows out of 8 bits.  Memory-bound: 1 byte in, 2 or 4 out.  A block does one piece of a row, PIECE
+// vectors of 16 values a thread (one value a thread where !VEC16), all loads before the first store.
+constexpr int kPiece = 2;
+
+template <typename T, bool VEC16>
 __global__ void __launch_bounds__(kRowThreads)
     dequantize_kernel(const uint8_t* Q, const float* scale, T* X, int64_t M, int64_t N, int64_t ldq,
                       int64_t ldx, int q_dtype, float top) {
-  const int64_t per_row = (N + VEC - 1) / VEC;
-  const int64_t bpr = (per_row + kRowThreads - 1) / kRowThreads;  // block pieces of a row
+  constexpr int VEC = VEC16 ? 16 : 1, OUT = 16 / (int)sizeof(T);
+  const int per_block = kRowThreads * kPiece * VEC;
+  const int64_t bpr = (N + per_block - 1) / per_block;  // pieces of a row
   for (int64_t b = blockIdx.x; b < M * bpr; b += gridDim.x) {
-    const int64_t m = b / bpr, n = ((b - m * bpr) * kRowThreads + threadIdx.x) * VEC;
-    if (n >= N) continue;
+    const int64_t m = b / bpr, n0 = (b - m * bpr) * per_block + (int64_t)threadIdx.x * VEC;
+    const uint8_t* q = Q + m * ldq;
+    T* x = X + m * ldx;
     const float s = __ldg(scale + m);
-    auto value = [&](uint8_t c) {
-      const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c));
-      return clamp_to(v * s, top);
+    auto one = [&](int64_t n) {
+      from_f(x + n, clamp_to(load_elem(q, n, q_dtype) * s, top));
     };
-    const uint8_t* q = Q + m * ldq + n;
-    T* x = X + m * ldx + n;
-    if (VEC > 1 && n + VEC <= N) {
-      const Vec<uint8_t, VEC> c = *reinterpret_cast<const Vec<uint8_t, VEC>*>(q);
-      constexpr int OUT = VEC < 16 / (int)sizeof(T) ? VEC : 16 / (int)sizeof(T);  // values per store
+    if constexpr (VEC16) {
+      uint4 c[kPiece];
 #pragma unroll
-      for (int i = 0; i < VEC; i += OUT) {
-        Vec<T, OUT> o;
+      for (int i = 0; i < kPiece; ++i) {
+        const int64_t n = n0 + (int64_t)i * kRowThreads * VEC;
+        if (n + VEC <= N) c[i] = __ldcs(reinterpret_cast<const uint4*>(q + n));
+      }
+      const bool big = !(fabsf(s) * 448.0f <= top);  // a value may pass the type's range (or s is NaN)
 #pragma unroll
-        for (int j = 0; j < OUT; ++j) from_f(&o.e[j], value(c.e[i + j]));
-        *reinterpret_cast<Vec<T, OUT>*>(x + i) = o;
+      for (int i = 0; i < kPiece; ++i) {
+        const int64_t n = n0 + (int64_t)i * kRowThreads * VEC;
+        if (n + VEC <= N && !big) {
+          const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+          Vec<T, OUT> o[16 / OUT];
+          T* d = o[0].e;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            F2 lo, hi;
+            unpack_q8x4(w[j], q_dtype, lo, hi);
+            float v[4];
+            f2_get(f2_mul(lo, f2(s, s)), v[0], v[1]);
+            f2_get(f2_mul(hi, f2(s, s)), v[2], v[3]);
+#pragma unroll
+            for (int l = 0; l < 4; ++l) from_f(d + 4 * j + l, v[l]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16 / OUT; ++j) *reinterpret_cast<Vec<T, OUT>*>(x + n + j * OUT) = o[j];
+        } else {
+          for (int64_t j = n; j < N && j < n + VEC; ++j) one(j);
+        }
       }
     } else {
-      const int count = N - n < VEC ? (int)(N - n) : VEC;
-      for (int j = 0; j < count; ++j) from_f(x + j, value(q[j]));
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i)
+        if (n0 + (int64_t)i * kRowThreads < N) one(n0 + (int64_t)i * kRowThreads);
     }
   }
 }
@@ -541,78 +573,95 @@ bool aligned(const void* p, int64_t pitch_bytes, int64_t rows, int to) {
   return ((uintptr_t)p % to) == 0 && (rows == 1 || pitch_bytes % to == 0);
 }
 
-// One launch of rows_to_q8_kernel: as many resident blocks as the GPU holds, at most one a row.
-template <typename T, bool NORM, int VEC, int V, bool WARP, bool AHEAD = true>
+// One launch of rows_to_q8_kernel: as many resident blocks as the GPU holds, at most one a row (set of rows).
+template <typename T, bool NORM, int VEC, int V, int LANES, bool AHEAD = true>
 int launch_rows(const NormArgs& a, int threads, int sms, cudaStream_t s) {
-  const int per_block = WARP ? threads / 32 : 1;
+  if (LANES) threads = 128;
+  const int per_block = LANES ? 128 / (LANES ? LANES : 1) : 1;
   const int64_t need = (a.M + per_block - 1) / per_block;
   const int64_t cap = (int64_t)sms * std::max(1, 1024 / threads);
-  rows_to_q8_kernel<T, NORM, VEC, V, WARP, AHEAD><<<(unsigned)std::min(need, cap), threads, 0, s>>>(a);
+  rows_to_q8_kernel<T, NORM, VEC, V, LANES, AHEAD><<<(unsigned)std::min(need, cap), threads, 0, s>>>(a);
   return launched("rows_to_q8_kernel");
 }
 
-// A launch of rows_ring_kernel, or false where its stages do not fit or a row owner would have too few
-// rows for the ring to matter.
-template <typename T, bool NORM, int V, bool WARP>
-bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
-  const int owners = WARP ? kRingThreads / 32 : 1;
-  const uint32_t row_bytes = (uint32_t)(a.N * (int64_t)sizeof(T));
-  const uint32_t stage = (a.R ? 2 : 1) * row_bytes;
-  constexpr uint32_t kBudget = 112 * 1024;  // two CTAs an SM
-  const int stages = (int)std::min<uint32_t>(4, (kBudget - 1024) / (owners * stage));
-  if (stages < 2) return false;
-  const int64_t blocks = std::min<int64_t>((a.M + owners - 1) / owners, (int64_t)sms * 2);
-  if (a.M < blocks * owners * 2) return false;
-  const uint32_t smem = (uint32_t)(owners * stages) * (stage + 8);
-  auto fn = rows_ring_kernel<T, NORM, V, WARP>;
-  static std::atomic<uint64_t> ready{0};  // devices whose limit was raised
+// Stages and blocks an SM of a ring kernel: as many blocks as `ctas` if three stages each fit, else
+// fewer.  False where not even two stages fit one block.
+bool ring_shape(uint32_t stage, int ctas, int* blocks, int* stages) {
+  constexpr uint32_t kSmem = 220 * 1024;
+  for (int want = 3; want >= 2; --want)
+    for (int n = ctas; n >= 1; --n) {
+      const uint32_t fit = (kSmem / n - 2048) / stage;
+      if (fit >= (uint32_t)want) {
+        *blocks = n;
+        *stages = (int)std::min<uint32_t>(4, fit);
+        return true;
+      }
+    }
+  return false;
+}
+
+// Raises a kernel's shared-memory limit once per device.
+template <typename F>
+int raise_smem(F fn, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(ready.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBudget);
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
     if (e == cudaSuccess) ready |= 1ull << dev;
   }
-  if (e != cudaSuccess) {
-    *rc = cuda_fail(e, "cudaFuncSetAttribute(smem)");
-    return true;
-  }
-  fn<<<(unsigned)blocks, kRingThreads, smem, s>>>(a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
+  return e == cudaSuccess ? (int)B2G_OK : cuda_fail(e, "cudaFuncSetAttribute(smem)");
+}
+
+// A launch of rows_ring_kernel, or false where its stages do not fit or a block would have too few
+// rows for the ring to matter.
+template <typename T, bool NORM, int V, int THREADS, int CTAS>
+bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
+  const uint32_t row_bytes = (uint32_t)(a.N * (int64_t)sizeof(T));
+  const uint32_t stage = (a.R ? 2 : 1) * row_bytes;
+  int ctas = 0, stages = 0;
+  if (!ring_shape(stage, CTAS, &ctas, &stages) || a.M < (int64_t)sms * ctas * 2) return false;
+  auto fn = rows_ring_kernel<T, NORM, V, THREADS, CTAS>;
+  static std::atomic<uint64_t> ready{0};
+  *rc = raise_smem(fn, ready);
+  if (*rc != B2G_OK) return true;
+  fn<<<(unsigned)(sms * ctas), THREADS, (uint32_t)stages * (stage + 8), s>>>(
+      a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
   *rc = launched("rows_ring_kernel");
   return true;
 }
 
-// Vectors of 16 bytes where every address and pitch allows, else single elements; short rows one a
-// warp.  A thread holds as many vectors as keep the block at 256 threads, up to 4 of them.
+// Vectors of 16 bytes where every address and pitch allows, else single elements.  Rows of up to 128
+// vectors: four vectors a lane, several rows a warp; longer ones: a ring, or with few rows (latency
+// counts then) one block a row with its loads in registers.
 template <typename T, bool NORM>
 int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int es = (int)sizeof(T);
-  const bool vec = a.N % VEC == 0 && aligned(a.X, a.ldx * es, a.M, 16) && (!a.R || aligned(a.R, a.ldr * es, a.M, 16)) &&
+  const bool vec = a.N % VEC == 0 && aligned(a.X, a.ldx * es, a.M, 16) &&
+                   (!a.R || aligned(a.R, a.ldr * es, a.M, 16)) &&
                    (!a.H || aligned(a.H, a.ldh * es, a.M, 16)) && aligned(a.Q, a.ldq, a.M, VEC);
   if (vec) {
     const int64_t nv = a.N / VEC;
+    if (nv <= 16) return launch_rows<T, NORM, VEC, 4, 4>(a, 0, sms, s);
+    if (nv <= 32) return launch_rows<T, NORM, VEC, 4, 8>(a, 0, sms, s);
+    if (nv <= 64) return launch_rows<T, NORM, VEC, 4, 16>(a, 0, sms, s);
+    if (nv <= 128) return launch_rows<T, NORM, VEC, 4, 32>(a, 0, sms, s);
     int rc = B2G_OK;
-    if (nv <= 32 ? launch_ring<T, NORM, 1, true>(a, sms, s, &rc)
-        : nv <= 64 ? launch_ring<T, NORM, 2, true>(a, sms, s, &rc)
-        : nv <= 128 ? launch_ring<T, NORM, 4, true>(a, sms, s, &rc)
-        : nv <= 256 ? launch_ring<T, NORM, 1, false>(a, sms, s, &rc)
-        : nv <= 512 ? launch_ring<T, NORM, 2, false>(a, sms, s, &rc)
-        : nv <= 1024 ? launch_ring<T, NORM, 4, false>(a, sms, s, &rc)
-        : nv <= 2048 ? launch_ring<T, NORM, 8, false>(a, sms, s, &rc)
+    if (nv <= 256 ? launch_ring<T, NORM, 2, 128, NORM ? 7 : 8>(a, sms, s, &rc)
+        : nv <= 512 ? launch_ring<T, NORM, 4, 128, NORM ? 4 : 7>(a, sms, s, &rc)
+        : nv <= 1024 ? launch_ring<T, NORM, 4, 256, NORM ? 2 : 4>(a, sms, s, &rc)
+        : nv <= 2048 ? launch_ring<T, NORM, 8, 256, 2>(a, sms, s, &rc)
                      : false)
       return rc;
-    if (nv <= 32) return launch_rows<T, NORM, VEC, 1, true>(a, 128, sms, s);
-    if (nv <= 64) return launch_rows<T, NORM, VEC, 2, true>(a, 128, sms, s);
-    if (nv <= 128) return launch_rows<T, NORM, VEC, 4, true>(a, 128, sms, s);
-    if (nv <= 256) return launch_rows<T, NORM, VEC, 1, false>(a, (int)(nv + 31) / 32 * 32, sms, s);
-    if (nv <= 512) return launch_rows<T, NORM, VEC, 2, false>(a, (int)(nv + 63) / 64 * 32, sms, s);
-    if (nv <= 1024) return launch_rows<T, NORM, VEC, 4, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
-    if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, false, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
+    if (nv <= 256) return launch_rows<T, NORM, VEC, 1, 0>(a, (int)(nv + 31) / 32 * 32, sms, s);
+    if (nv <= 512) return launch_rows<T, NORM, VEC, 2, 0>(a, (int)(nv + 63) / 64 * 32, sms, s);
+    if (nv <= 1024) return launch_rows<T, NORM, VEC, 4, 0>(a, (int)(nv + 127) / 128 * 32, sms, s);
+    if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, 0, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
   } else {
-    if (a.N <= 32 * 8) return launch_rows<T, NORM, 1, 8, true>(a, 128, sms, s);
-    if (a.N <= 256 * 8) return launch_rows<T, NORM, 1, 8, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
-    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, false, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
-    if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, false, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
+    if (a.N <= 32 * 8) return launch_rows<T, NORM, 1, 8, 32>(a, 0, sms, s);
+    if (a.N <= 256 * 8) return launch_rows<T, NORM, 1, 8, 0>(a, (int)(a.N + 255) / 256 * 32, sms, s);
+    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, 0, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
+    if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, 0, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
   }
   long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
   return launched("long_rows_to_q8_kernel");
@@ -637,12 +686,12 @@ int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N,
                   int q_dtype, float top, int sms, cudaStream_t s) {
   const uint8_t* q = static_cast<const uint8_t*>(Q);
   const bool vec = aligned(Q, ldq, M, 16) && aligned(X, ldx * (int64_t)sizeof(T), M, 16);
-  const int64_t per_row = (N + (vec ? 15 : 0)) / (vec ? 16 : 1);
-  const int64_t blocks = std::min<int64_t>(M * ((per_row + kRowThreads - 1) / kRowThreads), (int64_t)sms * 1024);
+  const int64_t per_block = kRowThreads * kPiece * (vec ? 16 : 1);
+  const int64_t blocks = std::min<int64_t>(M * ((N + per_block - 1) / per_block), (int64_t)sms * 1024);
   if (vec)
-    dequantize_kernel<T, 16><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
+    dequantize_kernel<T, true><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
   else
-    dequantize_kernel<T, 1><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
+    dequantize_kernel<T, false><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
   return launched("dequantize_kernel");
 }
 

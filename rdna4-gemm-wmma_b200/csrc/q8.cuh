@@ -75,6 +75,26 @@ __device__ __forceinline__ float max_abs(float top, float v) {
   return r;
 }
 
+// Four 8-bit values of a word as fp32 pairs.  int8: the byte with its sign bit flipped, placed in the low
+// byte of 2^23, is 2^23 + 128 + value (a conversion instruction runs at an eighth of this rate).
+__device__ __forceinline__ void unpack_q8x4(uint32_t w, int q_dtype, F2& lo, F2& hi) {
+  if (q_dtype == B2G_DTYPE_I8) {
+    w ^= 0x80808080u;
+    const F2 off = f2(-8388736.0f, -8388736.0f);
+    lo = f2_add(f2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)),
+                   __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441))), off);
+    hi = f2_add(f2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)),
+                   __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443))), off);
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    lo = f2(x.x, x.y);
+    hi = f2(y.x, y.y);
+  }
+}
+
 // How the elements v of a row become 8-bit values t.  v is first scaled by a power of two that brings
 // the row's largest value near 1 (exact, and no later product overflows); then
 //   without pow2   t = v * qmax / amax, the quotient correctly rounded: for 16-bit v it often lies

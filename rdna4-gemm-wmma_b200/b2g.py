@@ -449,63 +449,102 @@ def contract5d_batched(A, a_shape, a_stride, B, b_shape, b_stride, b_batch_strid
                                          float(alpha), float(beta), _stream(stream)))
 
 
-_TORCH_NAMES = {DTYPE_F16: ("torch.float16",), DTYPE_BF16: ("torch.bfloat16",),
-                DTYPE_F32: ("torch.float32",), DTYPE_I8: ("torch.int8",),
-                DTYPE_E4M3: ("torch.float8_e4m3fn", "torch.uint8")}
-_torch_types = None  # type code -> torch dtypes, filled in at the first tensor
+_torch = None
+_torch_types = {}  # type code -> the torch dtypes that hold it
 
 
-def _operand(x, dtype, what, rows=None, cols=None, ld=None):
-    """(pointer, leading dimension) of an operand of the 8-bit operators.  A raw pointer is taken
-    as it is (its leading dimension defaults to `cols`).  A torch tensor has to be of the type
-    that the call names, on the current device, and, with rows and cols, a row-major matrix of
-    that size at least, whose row stride is the default leading dimension."""
-    if x is None:
-        return None, (cols or 1) if ld is None else ld
-    if not hasattr(x, "stride"):
-        return _ptr(x), (cols or 1) if ld is None else ld
-    global _torch_types
-    import torch
-    if _torch_types is None:
-        _torch_types = {c: [getattr(torch, n.split(".")[1]) for n in names if hasattr(torch, n.split(".")[1])]
-                        for c, names in _TORCH_NAMES.items()}
-    if dtype in _torch_types and x.dtype not in _torch_types[dtype]:
-        raise B2GError(ERR_INVALID_ARG, "%s is %s, not of type code %r" % (what, x.dtype, dtype))
-    if not x.is_cuda:
-        raise B2GError(ERR_INVALID_ARG, "%s is not on a GPU" % what)
-    if x.get_device() != torch.cuda.current_device():
-        raise B2GError(ERR_INVALID_ARG, "%s is on another device than the current one" % what)
-    if rows is None:  # a vector
-        if cols and (x.numel() < cols or not x.is_contiguous()):
-            raise B2GError(ERR_INVALID_ARG, "%s has fewer than %d contiguous values" % (what, cols))
-        return x.data_ptr(), 1
-    if not rows or not cols:
-        return x.data_ptr(), (cols or 1) if ld is None else ld
-    if x.dim() == 2 and ld is None:
-        if x.shape[0] < rows or x.shape[1] < cols or (x.stride(1) != 1 and x.shape[1] > 1):
-            raise B2GError(ERR_INVALID_ARG, "%s is no row-major matrix of %d x %d" % (what, rows, cols))
-        return x.data_ptr(), x.stride(0) if rows > 1 else max(x.stride(0), cols)
-    return x.data_ptr(), cols if ld is None else ld
+def _device():
+    """The current device, which every tensor of a call has to be on (None without torch)."""
+    global _torch
+    if _torch is None:
+        try:
+            import torch
+        except ImportError:
+            return None
+        _torch = torch
+        for code, names in ((DTYPE_F16, ["float16"]), (DTYPE_BF16, ["bfloat16"]), (DTYPE_F32, ["float32"]),
+                            (DTYPE_I8, ["int8"]), (DTYPE_E4M3, ["float8_e4m3fn", "uint8"])):
+            _torch_types[code] = tuple(getattr(torch, n) for n in names if hasattr(torch, n))
+    return _torch.cuda.current_device() if _torch.cuda.is_initialized() else None
+
+
+def _refuse(msg, *args):
+    raise B2GError(ERR_INVALID_ARG, msg % args)
+
+
+def _check_tensor(x, dtype, what, dev):
+    if x.dtype not in _torch_types.get(dtype, (x.dtype,)):
+        _refuse("%s is %s, not of type code %r", what, x.dtype, dtype)
+    if x.get_device() != dev:
+        _refuse("%s is not on %s", what, "a GPU" if not x.is_cuda else "the current device")
+
+
+def _matrix(x, dtype, what, rows, cols, ld, dev):
+    """(pointer, leading dimension) of a rows x cols operand of the 8-bit operators.  A raw pointer is
+    taken as it is (leading dimension `cols` unless given).  A torch tensor has to be of the type
+    that the call names and on the current device, and a row-major matrix of that size at least,
+    whose row stride is the default leading dimension."""
+    if x is None or isinstance(x, int):
+        return x, (cols or 1) if ld is None else ld
+    if dev is None or not isinstance(x, _torch.Tensor):
+        p = _ptr(x)
+        if dev is None and _torch is not None and isinstance(x, _torch.Tensor):
+            _check_tensor(x, dtype, what, dev)
+        return p, (cols or 1) if ld is None else ld
+    _check_tensor(x, dtype, what, dev)
+    if ld is None:
+        ld = cols or 1
+        if rows and cols:
+            st, sh = x.stride(), x.shape
+            if len(st) != 2:
+                if not x.is_contiguous() or x.numel() < rows * cols:
+                    _refuse("%s is no row-major matrix of %d x %d", what, rows, cols)
+            elif sh[0] < rows or sh[1] < cols or (st[1] != 1 and cols > 1):
+                _refuse("%s is no row-major matrix of %d x %d", what, rows, cols)
+            elif rows > 1:
+                ld = st[0]
+    return x.data_ptr(), ld
+
+
+def _vector(x, dtype, what, n, dev):
+    """Pointer of a vector of n contiguous values (None: an optional one that is not given)."""
+    if x is None or isinstance(x, int):
+        return x
+    if dev is None or not isinstance(x, _torch.Tensor):
+        return _ptr(x)
+    _check_tensor(x, dtype, what, dev)
+    if x.numel() < n or not x.is_contiguous():
+        _refuse("%s has fewer than %d contiguous values", what, n)
+    return x.data_ptr()
+
+
+def _stream_of(stream, dev):
+    """_stream() without asking for a GPU again where the tensors' device is known."""
+    if stream is None and dev is not None:
+        return _torch.cuda.current_stream(dev).cuda_stream
+    return _stream(stream)
 
 
 def quantize_q8(X, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, pow2=False, ldx=None,
                 ldq=None, stream=None):
     """Q, scale = rows of X (M x N, type dtype) in 8 bits: scale = max|x| / qmax, with pow2
     rounded up to a power of two.  Leading dimensions default to the tensors' row strides."""
-    x, ldx = _operand(X, dtype, "X", M, N, ldx)
-    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
-    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
+    dev = _device()
+    x, ldx = _matrix(X, dtype, "X", M, N, ldx, dev)
+    q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
+    s = _vector(scale, DTYPE_F32, "scale", M, dev)
     _check(load().b2g_quantize_q8(x, q, s, M, N, ldx, ldq, dtype, q_dtype, 1 if pow2 else 0,
-                                  _stream(stream)))
+                                  _stream_of(stream, dev)))
 
 
 def dequantize_q8(Q, scale, X, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, ldq=None, ldx=None,
                   stream=None):
     """X (M x N, type dtype) = Q * scale (one scale per row)."""
-    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
-    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
-    x, ldx = _operand(X, dtype, "X", M, N, ldx)
-    _check(load().b2g_dequantize_q8(q, s, x, M, N, ldq, ldx, q_dtype, dtype, _stream(stream)))
+    dev = _device()
+    q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
+    s = _vector(scale, DTYPE_F32, "scale", M, dev)
+    x, ldx = _matrix(X, dtype, "X", M, N, ldx, dev)
+    _check(load().b2g_dequantize_q8(q, s, x, M, N, ldq, ldx, q_dtype, dtype, _stream_of(stream, dev)))
 
 
 def rmsnorm_q8(X, W, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, R=None, H=None, rstd=None,
@@ -513,59 +552,63 @@ def rmsnorm_q8(X, W, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, R=None, 
                stream=None):
     """h = X + R, Q, scale = (h / sqrt(mean(h^2) + eps) * W) in 8 bits.  Optional outputs: H = h
     in type dtype (may be X or R itself), rstd (M fp32 values, for rmsnorm_bwd_q8)."""
+    dev = _device()
     w_dtype = dtype if w_dtype is None else w_dtype
-    x, ldx = _operand(X, dtype, "X", M, N, ldx)
-    r, ldr = _operand(R, dtype, "R", M, N, ldr)
-    w, _ = _operand(W, w_dtype, "W", None, N)
-    h, ldh = _operand(H, dtype, "H", M, N, ldh)
-    q, ldq = _operand(Q, q_dtype, "Q", M, N, ldq)
-    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
-    rs, _ = _operand(rstd, DTYPE_F32, "rstd", None, M)
+    x, ldx = _matrix(X, dtype, "X", M, N, ldx, dev)
+    r, ldr = _matrix(R, dtype, "R", M, N, ldr, dev)
+    w = _vector(W, w_dtype, "W", N, dev)
+    h, ldh = _matrix(H, dtype, "H", M, N, ldh, dev)
+    q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
+    s = _vector(scale, DTYPE_F32, "scale", M, dev)
+    rs = _vector(rstd, DTYPE_F32, "rstd", M, dev)
     _check(load().b2g_rmsnorm_q8(x, r, w, h, q, s, rs, M, N, ldx, ldr, ldh, ldq, dtype, w_dtype,
-                                 q_dtype, float(eps), 1 if pow2 else 0, _stream(stream)))
+                                 q_dtype, float(eps), 1 if pow2 else 0, _stream_of(stream, dev)))
 
 
 def gemm_q8(A, B, C, M, N, K, dtype=DTYPE_I8, a_scale=None, b_scale=None, bias=None,
             c_dtype=DTYPE_F32, lda=None, ldb=None, ldc=None, stream=None):
     """C = (A . B^T) * a_scale[:, None] * b_scale + bias with A M x K and B N x K of 8-bit type
     dtype (int32 sums for DTYPE_I8) and C of type c_dtype."""
-    a, lda = _operand(A, dtype, "A", M, K, lda)
-    b, ldb = _operand(B, dtype, "B", N, K, ldb)
-    c, ldc = _operand(C, c_dtype, "C", M, N, ldc)
-    sa, _ = _operand(a_scale, DTYPE_F32, "a_scale", None, M)
-    sb, _ = _operand(b_scale, DTYPE_F32, "b_scale", None, N)
-    bi, _ = _operand(bias, DTYPE_F32, "bias", None, N)
+    dev = _device()
+    a, lda = _matrix(A, dtype, "A", M, K, lda, dev)
+    b, ldb = _matrix(B, dtype, "B", N, K, ldb, dev)
+    c, ldc = _matrix(C, c_dtype, "C", M, N, ldc, dev)
+    sa = _vector(a_scale, DTYPE_F32, "a_scale", M, dev)
+    sb = _vector(b_scale, DTYPE_F32, "b_scale", N, dev)
+    bi = _vector(bias, DTYPE_F32, "bias", N, dev)
     _check(load().b2g_gemm_q8(a, b, c, M, N, K, lda, ldb, ldc, dtype, sa, sb, bi, c_dtype,
-                              _stream(stream)))
+                              _stream_of(stream, dev)))
 
 
 def wgrad_q8(dY, Q, scale, dW, M, N, K, dtype=DTYPE_BF16, q_dtype=DTYPE_I8, accumulate=False,
              c_dtype=DTYPE_F32, ldy=None, ldq=None, ldw=None, stream=None):
     """dW (N x K) = dY^T . (Q * scale) from the 8-bit checkpoint Q (M x K) of a linear layer's
     input and the gradient dY (M x N) of its output; accumulate adds into an fp32 dW."""
-    y, ldy = _operand(dY, dtype, "dY", M, N, ldy)
-    q, ldq = _operand(Q, q_dtype, "Q", M, K, ldq)
-    s, _ = _operand(scale, DTYPE_F32, "scale", None, M)
-    w, ldw = _operand(dW, c_dtype, "dW", N, K, ldw)
+    dev = _device()
+    y, ldy = _matrix(dY, dtype, "dY", M, N, ldy, dev)
+    q, ldq = _matrix(Q, q_dtype, "Q", M, K, ldq, dev)
+    s = _vector(scale, DTYPE_F32, "scale", M, dev)
+    w, ldw = _matrix(dW, c_dtype, "dW", N, K, ldw, dev)
     _check(load().b2g_wgrad_q8(y, q, s, w, M, N, K, ldy, ldq, ldw, dtype, q_dtype,
-                               1 if accumulate else 0, c_dtype, _stream(stream)))
+                               1 if accumulate else 0, c_dtype, _stream_of(stream, dev)))
 
 
 def rmsnorm_bwd_q8(dY, X, x_scale, W, rstd, dX, dw, M, N, dtype=DTYPE_BF16, x_dtype=DTYPE_I8,
                    w_dtype=None, dres=None, ldy=None, ldx=None, ldr=None, lddx=None, stream=None):
     """Backward pass of rmsnorm_q8: dX = rstd * (dY*W - xh * mean(dY*W*xh)) (+ dres) and
     dw = sum over rows of dY * xh, xh = (the checkpoint X * x_scale of h) * rstd.  dw may be None."""
+    dev = _device()
     w_dtype = dtype if w_dtype is None else w_dtype
-    y, ldy = _operand(dY, dtype, "dY", M, N, ldy)
-    x, ldx = _operand(X, x_dtype, "X", M, N, ldx)
-    xs, _ = _operand(x_scale, DTYPE_F32, "x_scale", None, M)
-    w, _ = _operand(W, w_dtype, "W", None, N)
-    rs, _ = _operand(rstd, DTYPE_F32, "rstd", None, M)
-    r, ldr = _operand(dres, dtype, "dres", M, N, ldr)
-    d, lddx = _operand(dX, dtype, "dX", M, N, lddx)
-    g, _ = _operand(dw, DTYPE_F32, "dw", None, N)
+    y, ldy = _matrix(dY, dtype, "dY", M, N, ldy, dev)
+    x, ldx = _matrix(X, x_dtype, "X", M, N, ldx, dev)
+    xs = _vector(x_scale, DTYPE_F32, "x_scale", M, dev)
+    w = _vector(W, w_dtype, "W", N, dev)
+    rs = _vector(rstd, DTYPE_F32, "rstd", M, dev)
+    r, ldr = _matrix(dres, dtype, "dres", M, N, ldr, dev)
+    d, lddx = _matrix(dX, dtype, "dX", M, N, lddx, dev)
+    g = _vector(dw, DTYPE_F32, "dw", N, dev)
     _check(load().b2g_rmsnorm_bwd_q8(y, x, xs, w, rs, r, d, g, M, N, ldy, ldx, ldr, lddx, dtype,
-                                     x_dtype, w_dtype, _stream(stream)))
+                                     x_dtype, w_dtype, _stream_of(stream, dev)))
 
 
 def version():

@@ -547,16 +547,169 @@ __global__ void __launch_bounds__(kRowThreads) rmsnorm_bwd_kernel(const BwdArgs 
   }
 }
 
-// dw[n] = sum over the blocks' partial sums, in block order.
-__global__ void __launch_bounds__(kRowThreads)
-    dw_sum_kernel(const float* part, float* dw, int64_t N, int blocks) {
-  const int64_t n = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (n >= N) return;
-  float s = 0.0f;
-  for (int b = 0; b < blocks; ++b) s += part[(int64_t)b * N + n];
-  dw[n] = s;
+// VEC checkpoint values from shared memory: 8-bit, or of the gradient's type.
+template <typename T, bool X8>
+struct XVec {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  static constexpr int SIZE = X8 ? VEC : 16;  // bytes
+  alignas(16) uint32_t w[SIZE / 4];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (SIZE == 16)
+      *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else if constexpr (SIZE == 8)
+      *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+    else
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+  __device__ __forceinline__ void get(int x_dtype, F2 (&v)[VEC / 2]) const {
+    if constexpr (X8) {
+#pragma unroll
+      for (int j = 0; j < VEC / 4; ++j) unpack_q8x4(w[j], x_dtype, v[2 * j], v[2 * j + 1]);
+    } else {
+      const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) v[j] = f2(to_f(e[2 * j]), to_f(e[2 * j + 1]));
+    }
+  }
+};
+
+// rmsnorm_bwd_kernel over a ring of rows (dY, X and dR of whole 16-byte vectors).  A thread keeps its V
+// vectors of a row packed in registers between the reduction and the output, and its columns' share
+// of dw in fp32 over all of the block's rows: dw costs no traffic but one partial row a block.
+template <typename T, bool X8, int V, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS)
+    rmsnorm_bwd_ring_kernel(const BwdArgs a, int stages, uint32_t y_bytes, uint32_t x_bytes,
+                            uint64_t limit_ns) {
+  using XV = XVec<T, X8>;
+  constexpr int VEC = XV::VEC;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float buf[128];
+  __shared__ int abort_flag;
+  const int tid = (int)threadIdx.x;
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  const int N = (int)a.N;
+  const T* dY = static_cast<const T*>(a.dY);
+  const T* dR = static_cast<const T*>(a.dR);
+  const uint8_t* X = static_cast<const uint8_t*>(a.X);
+  const int64_t x_pitch = a.ldx * (X8 ? 1 : (int)sizeof(T));
+  const uint32_t stage_bytes = (dR ? 2 * y_bytes : y_bytes) + x_bytes, r_off = y_bytes + x_bytes;
+  const Ring ring = make_ring(smem, stages, stage_bytes, limit_ns, &abort_flag);
+  auto fill = [&](int64_t m, int k) {
+    const uint32_t bar = ring.bar(k), dst = ring.stage(k);
+    ptx::mbar_arrive_expect_tx(bar, stage_bytes);
+    ptx::bulk_load(dst, dY + m * a.ldy, y_bytes, bar);
+    ptx::bulk_load(dst + y_bytes, X + m * x_pitch, x_bytes, bar);
+    if (dR) ptx::bulk_load(dst + r_off, dR + m * a.ldr, y_bytes, bar);
+  };
+  int issued = 0;
+  if (tid == 0)
+    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+  const bool wvec = weights_vec(a.W, a.w_dtype);
+  F2 dw[V][VEC / 2];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) dw[i][j] = f2(0.0f, 0.0f);
+  int k = 0;
+  for (int64_t m = first; m < a.M; m += step, ++k) {
+    const float rstd = __ldg(a.rstd + m);
+    const float xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    const F2 xs2 = f2(xs, xs);
+    const bool ok = ring.wait(k);
+    const uint8_t* st = smem + (uint32_t)(k % stages) * stage_bytes;
+    Vec<T, VEC> y[V], r[V];
+    XV x[V];
+    F2 c2 = f2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = (i * THREADS + tid) * VEC;
+      if (n < N) {
+        y[i] = *reinterpret_cast<const Vec<T, VEC>*>(st + n * (int)sizeof(T));
+        x[i].load(st + y_bytes + n * (X8 ? 1 : (int)sizeof(T)));
+        if (dR) r[i] = *reinterpret_cast<const Vec<T, VEC>*>(st + r_off + n * (int)sizeof(T));
+        float w[VEC];
+        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
+        F2 xv[VEC / 2];
+        x[i].get(a.x_dtype, xv);
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const F2 dy = f2(to_f(y[i].e[2 * j]), to_f(y[i].e[2 * j + 1]));
+          c2 = f2_fma(f2_mul(dy, f2(w[2 * j], w[2 * j + 1])), f2_mul(xv[j], xs2), c2);
+        }
+      }
+    }
+    float c0, c1;
+    f2_get(c2, c0, c1);
+    float c = c0 + c1;
+    uint32_t late = ok ? 0u : 1u;
+    row_reduce<0, true>(c, late, buf, k & 1);
+    if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
+      fill(m + step * stages, k + stages);  // every thread holds its part of this row (row_reduce)
+      ++issued;
+    }
+    c = late ? __int_as_float(0x7fc00000) : c / (float)N;
+    const F2 nc = f2(-c * rstd, -c * rstd), rs2 = f2(rstd, rstd);
+    T* dX = static_cast<T*>(a.dX) + m * a.lddx;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = (i * THREADS + tid) * VEC;
+      if (n < N) {
+        float w[VEC];
+        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
+        F2 xv[VEC / 2];
+        x[i].get(a.x_dtype, xv);
+        Vec<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC / 2; ++j) {
+          const F2 dy = f2(to_f(y[i].e[2 * j]), to_f(y[i].e[2 * j + 1]));
+          const F2 xh = f2_mul(xv[j], xs2);
+          dw[i][j] = f2_fma(dy, xh, dw[i][j]);
+          F2 d = f2_fma(xh, nc, f2_mul(f2_mul(dy, f2(w[2 * j], w[2 * j + 1])), rs2));
+          if (dR) d = f2_add(d, f2(to_f(r[i].e[2 * j]), to_f(r[i].e[2 * j + 1])));
+          float d0, d1;
+          f2_get(d, d0, d1);
+          from_f(&o.e[2 * j], d0);
+          from_f(&o.e[2 * j + 1], d1);
+        }
+        *reinterpret_cast<Vec<T, VEC>*>(dX + n) = o;
+      }
+    }
+  }
+  if (a.part) {
+    float* p = a.part + (int64_t)blockIdx.x * a.N;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = (i * THREADS + tid) * VEC;
+      if (n < N)
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) {
+          float4 v;
+          f2_get(dw[i][j / 2], v.x, v.y);
+          f2_get(dw[i][j / 2 + 1], v.z, v.w);
+          *reinterpret_cast<float4*>(p + n + j) = v;
+        }
+    }
+  }
+  if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
+// dw[n] = the blocks' partial sums: a block sums 32 columns, its warp w the rows w, w + 8, ..., and the
+// warps' sums are added in order.
+__global__ void __launch_bounds__(kRowThreads) dw_sum_kernel(const float* part, float* dw, int64_t N, int rows) {
+  __shared__ float buf[kRowThreads / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (n < N)
+#pragma unroll 8
+    for (int b = warp; b < rows; b += kRowThreads / 32) s += __ldcs(part + (int64_t)b * N + n);
+  buf[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && n < N) {
+    for (int w = 1; w < kRowThreads / 32; ++w) s += buf[w][lane];
+    dw[n] = s;
+  }
+}
 
 unsigned row_blocks(int64_t M, int sms) { return (unsigned)std::min<int64_t>(M, (int64_t)sms * 8); }
 
@@ -695,6 +848,65 @@ int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N,
   return launched("dequantize_kernel");
 }
 
+// Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel: blocks an SM and
+// stages in *ctas and *stages.  V and THREADS as in launch_bwd_ring.
+template <typename T>
+bool bwd_ring_ok(const BwdArgs& a, bool x8, int most, int* ctas, int* stages) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int es = (int)sizeof(T), xe = x8 ? 1 : es;
+  if (a.N % VEC != 0 || a.N * xe % 16 != 0 || !aligned(a.dY, a.ldy * es, a.M, 16) ||
+      !aligned(a.X, a.ldx * xe, a.M, 16) || !aligned(a.dX, a.lddx * es, a.M, 16) ||
+      (a.dR && !aligned(a.dR, a.ldr * es, a.M, 16)) || a.N > 2048 * VEC)
+    return false;
+  return ring_shape((uint32_t)(a.N * ((a.dR ? 2 : 1) * es + xe)), most, ctas, stages);
+}
+
+template <typename T, bool X8, int V, int THREADS, int CTAS>
+int launch_bwd_ring(const BwdArgs& a, unsigned blocks, int stages, cudaStream_t s) {
+  const uint32_t yb = (uint32_t)(a.N * (int64_t)sizeof(T)), xb = X8 ? (uint32_t)a.N : yb;
+  auto fn = rmsnorm_bwd_ring_kernel<T, X8, V, THREADS, CTAS>;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = raise_smem(fn, ready);
+  if (rc != B2G_OK) return rc;
+  fn<<<blocks, THREADS, (uint32_t)stages * ((a.dR ? 2 : 1) * yb + xb + 8), s>>>(
+      a, stages, yb, xb, (uint64_t)launch_options().timeout_ns);
+  return launched("rmsnorm_bwd_ring_kernel");
+}
+
+template <typename T, bool X8>
+int bwd_ring(const BwdArgs& a, unsigned blocks, int stages, cudaStream_t s) {
+  const int64_t nv = a.N / (16 / (int)sizeof(T));
+  if (nv <= 128) return launch_bwd_ring<T, X8, 1, 128, 8>(a, blocks, stages, s);
+  if (nv <= 256) return launch_bwd_ring<T, X8, 2, 128, 6>(a, blocks, stages, s);
+  if (nv <= 512) return launch_bwd_ring<T, X8, 4, 128, 4>(a, blocks, stages, s);
+  if (nv <= 1024) return launch_bwd_ring<T, X8, 4, 256, 2>(a, blocks, stages, s);
+  return launch_bwd_ring<T, X8, 8, 256, 1>(a, blocks, stages, s);
+}
+
+template <typename T>
+int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
+  const int64_t nv = a.N / (16 / (int)sizeof(T));
+  int ctas = nv <= 128 ? 8 : nv <= 256 ? 6 : nv <= 512 ? 4 : nv <= 1024 ? 2 : 1, stages = 0;
+  const bool ring = (x8 || same) && bwd_ring_ok<T>(a, x8, ctas, &ctas, &stages);
+  const unsigned blocks = ring ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas) : row_blocks(a.M, sms);
+  Workspace ws(s);
+  int rc = B2G_OK;
+  if (dw) {
+    rc = ws.alloc((size_t)blocks * (size_t)a.N * sizeof(float), "cudaMallocFromPoolAsync(dw partial sums)");
+    if (rc != B2G_OK) return rc;
+    a.part = static_cast<float*>(ws.get());
+  }
+  if (ring) {
+    rc = x8 ? bwd_ring<T, true>(a, blocks, stages, s) : bwd_ring<T, false>(a, blocks, stages, s);
+  } else {
+    rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
+    rc = launched("rmsnorm_bwd_kernel");
+  }
+  if (rc != B2G_OK || !dw) return rc;
+  dw_sum_kernel<<<(unsigned)((a.N + 31) / 32), kRowThreads, 0, s>>>(a.part, dw, a.N, (int)blocks);
+  return launched("dw_sum_kernel");
+}
+
 }  // namespace
 
 int dequantize_rows(const void* Q, const float* scale, void* X, int64_t M, int64_t N, int64_t ldq,
@@ -813,17 +1025,10 @@ extern "C" int b2g_rmsnorm_bwd_q8(const void* dY, const void* X, const float* x_
   a.dX = dX;
   a.M = M; a.N = N; a.ldy = ldy; a.ldx = ldx; a.ldr = ldr; a.lddx = lddx;
   a.dtype = dtype; a.x_dtype = x_dtype; a.w_dtype = w_dtype;
-  const unsigned blocks = row_blocks(M, sms);
-  Workspace ws(s);
-  if (dw) {
-    rc = ws.alloc((size_t)blocks * (size_t)N * sizeof(float), "cudaMallocFromPoolAsync(dw partial sums)");
-    if (rc != B2G_OK) return rc;
-    a.part = static_cast<float*>(ws.get());
+  const bool x8 = is_q8(x_dtype), same = x_dtype == dtype;
+  switch (dtype) {
+    case B2G_DTYPE_F16: return bwd_of<__half>(a, x8, same, dw, sms, s);
+    case B2G_DTYPE_BF16: return bwd_of<__nv_bfloat16>(a, x8, same, dw, sms, s);
+    default: return bwd_of<float>(a, x8, same, dw, sms, s);
   }
-  rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
-  rc = launched("rmsnorm_bwd_kernel");
-  if (rc != B2G_OK || !dw) return rc;
-  dw_sum_kernel<<<(unsigned)((N + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(
-      a.part, dw, N, (int)blocks);
-  return launched("dw_sum_kernel");
 }

@@ -450,18 +450,20 @@ def contract5d_batched(A, a_shape, a_stride, B, b_shape, b_stride, b_batch_strid
 
 
 _torch = None
+_raw_stream = None  # device -> its current stream as an integer, where this torch has it
 _torch_types = {}  # type code -> the torch dtypes that hold it
 
 
 def _device():
     """The current device, which every tensor of a call has to be on (None without torch)."""
-    global _torch
+    global _torch, _raw_stream
     if _torch is None:
         try:
             import torch
         except ImportError:
             return None
         _torch = torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         for code, names in ((DTYPE_F16, ["float16"]), (DTYPE_BF16, ["bfloat16"]), (DTYPE_F32, ["float32"]),
                             (DTYPE_I8, ["int8"]), (DTYPE_E4M3, ["float8_e4m3fn", "uint8"])):
             _torch_types[code] = tuple(getattr(torch, n) for n in names if hasattr(torch, n))
@@ -472,11 +474,10 @@ def _refuse(msg, *args):
     raise B2GError(ERR_INVALID_ARG, msg % args)
 
 
-def _check_tensor(x, dtype, what, dev):
+def _wrong_tensor(x, dtype, what):
     if x.dtype not in _torch_types.get(dtype, (x.dtype,)):
         _refuse("%s is %s, not of type code %r", what, x.dtype, dtype)
-    if x.get_device() != dev:
-        _refuse("%s is not on %s", what, "a GPU" if not x.is_cuda else "the current device")
+    _refuse("%s is not on %s", what, "the current device" if x.is_cuda else "a GPU")
 
 
 def _matrix(x, dtype, what, rows, cols, ld, dev):
@@ -484,14 +485,10 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
     taken as it is (leading dimension `cols` unless given).  A torch tensor has to be of the type
     that the call names and on the current device, and a row-major matrix of that size at least,
     whose row stride is the default leading dimension."""
-    if x is None or isinstance(x, int):
-        return x, (cols or 1) if ld is None else ld
-    if dev is None or not isinstance(x, _torch.Tensor):
-        p = _ptr(x)
-        if dev is None and _torch is not None and isinstance(x, _torch.Tensor):
-            _check_tensor(x, dtype, what, dev)
-        return p, (cols or 1) if ld is None else ld
-    _check_tensor(x, dtype, what, dev)
+    if x is None or isinstance(x, int) or _torch is None or not isinstance(x, _torch.Tensor):
+        return _ptr(x), (cols or 1) if ld is None else ld
+    if x.get_device() != dev or x.dtype not in _torch_types.get(dtype, ()):
+        _wrong_tensor(x, dtype, what)
     if ld is None:
         ld = cols or 1
         if rows and cols:
@@ -508,20 +505,20 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
 
 def _vector(x, dtype, what, n, dev):
     """Pointer of a vector of n contiguous values (None: an optional one that is not given)."""
-    if x is None or isinstance(x, int):
-        return x
-    if dev is None or not isinstance(x, _torch.Tensor):
+    if x is None or isinstance(x, int) or _torch is None or not isinstance(x, _torch.Tensor):
         return _ptr(x)
-    _check_tensor(x, dtype, what, dev)
+    if x.get_device() != dev or x.dtype not in _torch_types.get(dtype, ()):
+        _wrong_tensor(x, dtype, what)
     if x.numel() < n or not x.is_contiguous():
         _refuse("%s has fewer than %d contiguous values", what, n)
     return x.data_ptr()
 
 
 def _stream_of(stream, dev):
-    """_stream() without asking for a GPU again where the tensors' device is known."""
-    if stream is None and dev is not None:
-        return _torch.cuda.current_stream(dev).cuda_stream
+    """_stream(), by the shorter way where the tensors' device is known (building a Stream object
+    costs as much as the launch)."""
+    if stream is None and dev is not None and _raw_stream is not None:
+        return _raw_stream(dev)
     return _stream(stream)
 
 

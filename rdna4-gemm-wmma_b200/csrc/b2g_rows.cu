@@ -318,7 +318,7 @@ __device__ __forceinline__ Ring make_ring(uint8_t* smem, int stages, uint32_t st
 }
 
 // rows_to_q8_kernel with its rows in a ring: rows of whole 16-byte vectors, one row at a time a block of
-// THREADS threads, which hold V vectors each.  The norm's weights stay in registers where V <= 4.
+// up to THREADS threads, which hold V vectors each.  The norm's weights stay in registers where V <= 4.
 // CTAS blocks share an SM, so that one's reduction overlaps the others' arithmetic.
 template <typename T, bool NORM, int V, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float buf[128];
   __shared__ int abort_flag;
-  const int tid = (int)threadIdx.x;
+  const int tid = (int)threadIdx.x, threads = (int)blockDim.x;
   const int64_t first = blockIdx.x, step = gridDim.x;
   const T* X = static_cast<const T*>(a.X);
   const T* R = NORM ? static_cast<const T*>(a.R) : nullptr;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   float wreg[WREG ? V : 1][VEC];
   if constexpr (WREG)
 #pragma unroll
-    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * THREADS + tid) * VEC, N, wreg[i]);
+    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, wreg[i]);
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
     const bool ok = ring.wait(k);
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * THREADS + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
       if (n < N) {
         unpack<T, VEC>(st + n * (int)sizeof(T), v[i]);
         if constexpr (NORM) {
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     uint8_t* q = static_cast<uint8_t*>(a.Q) + m * a.ldq;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * THREADS + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
       if (n < N) {
         Vec<uint8_t, VEC> o;
         pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
@@ -573,19 +573,21 @@ struct XVec {
   }
 };
 
-// rmsnorm_bwd_kernel over a ring of rows (dY, X and dR of whole 16-byte vectors).  A thread keeps its V
-// vectors of a row packed in registers between the reduction and the output, and its columns' share
-// of dw in fp32 over all of the block's rows: dw costs no traffic but one partial row a block.
-template <typename T, bool X8, int V, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS)
+// rmsnorm_bwd_kernel over a ring of rows (dY, X and dR of whole 16-byte vectors).  A thread holds V
+// vectors of a row, and its columns' share of dw in fp32 over all of the block's rows: dw costs no
+// traffic but one partial row a block.  HOLD (up to 16 elements a thread): the weights, and a row's
+// dy * w and xh, stay in fp32 registers; else a row stays packed between the reduction and the
+// output and is unpacked twice, with the weights read from L1.
+template <typename T, bool X8, int V, bool HOLD>
+__global__ void __launch_bounds__(512, 1)
     rmsnorm_bwd_ring_kernel(const BwdArgs a, int stages, uint32_t y_bytes, uint32_t x_bytes,
                             uint64_t limit_ns) {
   using XV = XVec<T, X8>;
-  constexpr int VEC = XV::VEC;
+  constexpr int VEC = XV::VEC, P = VEC / 2;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float buf[128];
   __shared__ int abort_flag;
-  const int tid = (int)threadIdx.x;
+  const int tid = (int)threadIdx.x, threads = (int)blockDim.x;
   const int64_t first = blockIdx.x, step = gridDim.x;
   const int N = (int)a.N;
   const T* dY = static_cast<const T*>(a.dY);
@@ -605,11 +607,21 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   if (tid == 0)
     for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
   const bool wvec = weights_vec(a.W, a.w_dtype);
-  F2 dw[V][VEC / 2];
+  auto weights = [&](int i, F2 (&w)[P]) {
+    float f[VEC];
+    load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, f);
+#pragma unroll
+    for (int j = 0; j < P; ++j) w[j] = f2(f[2 * j], f[2 * j + 1]);
+  };
+  F2 wreg[HOLD ? V : 1][P], g[HOLD ? V : 1][P], xh[HOLD ? V : 1][P];
+  if constexpr (HOLD)
+#pragma unroll
+    for (int i = 0; i < V; ++i) weights(i, wreg[i]);
+  F2 dw[V][P];
 #pragma unroll
   for (int i = 0; i < V; ++i)
 #pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) dw[i][j] = f2(0.0f, 0.0f);
+    for (int j = 0; j < P; ++j) dw[i][j] = f2(0.0f, 0.0f);
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
     const float rstd = __ldg(a.rstd + m);
@@ -622,19 +634,25 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     F2 c2 = f2(0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * THREADS + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
       if (n < N) {
         y[i] = *reinterpret_cast<const Vec<T, VEC>*>(st + n * (int)sizeof(T));
         x[i].load(st + y_bytes + n * (X8 ? 1 : (int)sizeof(T)));
         if (dR) r[i] = *reinterpret_cast<const Vec<T, VEC>*>(st + r_off + n * (int)sizeof(T));
-        float w[VEC];
-        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
-        F2 xv[VEC / 2];
+        F2 w[P], xv[P];
+        if constexpr (!HOLD) weights(i, w);
         x[i].get(a.x_dtype, xv);
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
+        for (int j = 0; j < P; ++j) {
           const F2 dy = f2(to_f(y[i].e[2 * j]), to_f(y[i].e[2 * j + 1]));
-          c2 = f2_fma(f2_mul(dy, f2(w[2 * j], w[2 * j + 1])), f2_mul(xv[j], xs2), c2);
+          xv[j] = f2_mul(xv[j], xs2);
+          const F2 gj = f2_mul(dy, HOLD ? wreg[HOLD ? i : 0][j] : w[j]);
+          c2 = f2_fma(gj, xv[j], c2);
+          if constexpr (HOLD) {
+            dw[i][j] = f2_fma(dy, xv[j], dw[i][j]);
+            g[i][j] = gj;
+            xh[i][j] = xv[j];
+          }
         }
       }
     }
@@ -652,19 +670,27 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     T* dX = static_cast<T*>(a.dX) + m * a.lddx;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * THREADS + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
       if (n < N) {
-        float w[VEC];
-        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
-        F2 xv[VEC / 2];
-        x[i].get(a.x_dtype, xv);
+        F2 w[P], xv[P];
+        if constexpr (!HOLD) {
+          weights(i, w);
+          x[i].get(a.x_dtype, xv);
+        }
         Vec<T, VEC> o;
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-          const F2 dy = f2(to_f(y[i].e[2 * j]), to_f(y[i].e[2 * j + 1]));
-          const F2 xh = f2_mul(xv[j], xs2);
-          dw[i][j] = f2_fma(dy, xh, dw[i][j]);
-          F2 d = f2_fma(xh, nc, f2_mul(f2_mul(dy, f2(w[2 * j], w[2 * j + 1])), rs2));
+        for (int j = 0; j < P; ++j) {
+          F2 gj, xj;
+          if constexpr (HOLD) {
+            gj = g[i][j];
+            xj = xh[i][j];
+          } else {
+            const F2 dy = f2(to_f(y[i].e[2 * j]), to_f(y[i].e[2 * j + 1]));
+            xj = f2_mul(xv[j], xs2);
+            dw[i][j] = f2_fma(dy, xj, dw[i][j]);
+            gj = f2_mul(dy, w[j]);
+          }
+          F2 d = f2_fma(xj, nc, f2_mul(gj, rs2));
           if (dR) d = f2_add(d, f2(to_f(r[i].e[2 * j]), to_f(r[i].e[2 * j + 1])));
           float d0, d1;
           f2_get(d, d0, d1);
@@ -679,7 +705,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     float* p = a.part + (int64_t)blockIdx.x * a.N;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = (i * THREADS + tid) * VEC;
+      const int n = (i * threads + tid) * VEC;
       if (n < N)
 #pragma unroll
         for (int j = 0; j < VEC; j += 4) {
@@ -693,22 +719,22 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
-// dw[n] = the blocks' partial sums: a block sums 32 columns, its warp w the rows w, w + 8, ..., and the
+// dw[n] = the blocks' partial sums: a block sums 32 columns, its warp w the rows w, w + 32, ..., and the
 // warps' sums are added in order.
-__global__ void __launch_bounds__(kRowThreads) dw_sum_kernel(const float* part, float* dw, int64_t N, int rows) {
-  __shared__ float buf[kRowThreads / 32][32];
+__global__ void __launch_bounds__(1024) dw_sum_kernel(const float* part, float* dw, int64_t N, int rows) {
+  __shared__ float buf[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
   if (n < N)
 #pragma unroll 8
-    for (int b = warp; b < rows; b += kRowThreads / 32) s += __ldcs(part + (int64_t)b * N + n);
+    for (int b = warp; b < rows; b += 32) s += __ldcs(part + (int64_t)b * N + n);
   buf[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && n < N) {
-    for (int w = 1; w < kRowThreads / 32; ++w) s += buf[w][lane];
-    dw[n] = s;
-  }
+  s = buf[lane][warp];  // column `warp` of the 32, one partial sum a lane
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t c = (int64_t)blockIdx.x * 32 + warp;
+  if (lane == 0 && c < N) dw[c] = s;
 }
 
 unsigned row_blocks(int64_t M, int sms) { return (unsigned)std::min<int64_t>(M, (int64_t)sms * 8); }
@@ -737,19 +763,19 @@ int launch_rows(const NormArgs& a, int threads, int sms, cudaStream_t s) {
   return launched("rows_to_q8_kernel");
 }
 
-// Stages and blocks an SM of a ring kernel: as many blocks as `ctas` if three stages each fit, else
-// fewer.  False where not even two stages fit one block.
-bool ring_shape(uint32_t stage, int ctas, int* blocks, int* stages) {
-  constexpr uint32_t kSmem = 220 * 1024;
-  for (int want = 3; want >= 2; --want)
-    for (int n = ctas; n >= 1; --n) {
-      const uint32_t fit = (kSmem / n - 2048) / stage;
-      if (fit >= (uint32_t)want) {
-        *blocks = n;
-        *stages = (int)std::min<uint32_t>(4, fit);
-        return true;
-      }
+// Stages and blocks an SM of a ring kernel: as many blocks as `most` if two stages of each fit (one
+// block's copies run while another's row is worked on), then up to four stages.  False where not
+// even two stages of one block fit.
+bool ring_shape(uint32_t stage, int most, int* blocks, int* stages) {
+  constexpr uint32_t kSmem = 224 * 1024;
+  for (int n = most; n >= 1; --n) {
+    const uint32_t fit = (kSmem / n - 2048) / stage;
+    if (fit >= 2) {
+      *blocks = n;
+      *stages = (int)std::min<uint32_t>(4, fit);
+      return true;
     }
+  }
   return false;
 }
 
@@ -759,7 +785,7 @@ int raise_smem(F fn, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(ready.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
     if (e == cudaSuccess) ready |= 1ull << dev;
   }
   return e == cudaSuccess ? (int)B2G_OK : cuda_fail(e, "cudaFuncSetAttribute(smem)");
@@ -777,7 +803,9 @@ bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   static std::atomic<uint64_t> ready{0};
   *rc = raise_smem(fn, ready);
   if (*rc != B2G_OK) return true;
-  fn<<<(unsigned)(sms * ctas), THREADS, (uint32_t)stages * (stage + 8), s>>>(
+  const int64_t nv = a.N * (int64_t)sizeof(T) / 16;
+  const int threads = (int)((nv + V * 32 - 1) / (V * 32)) * 32;
+  fn<<<(unsigned)(sms * ctas), threads, (uint32_t)stages * (stage + 8), s>>>(
       a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
   *rc = launched("rows_ring_kernel");
   return true;
@@ -848,46 +876,32 @@ int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N,
   return launched("dequantize_kernel");
 }
 
-// Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel: blocks an SM and
-// stages in *ctas and *stages.  V and THREADS as in launch_bwd_ring.
-template <typename T>
-bool bwd_ring_ok(const BwdArgs& a, bool x8, int most, int* ctas, int* stages) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int es = (int)sizeof(T), xe = x8 ? 1 : es;
-  if (a.N % VEC != 0 || a.N * xe % 16 != 0 || !aligned(a.dY, a.ldy * es, a.M, 16) ||
-      !aligned(a.X, a.ldx * xe, a.M, 16) || !aligned(a.dX, a.lddx * es, a.M, 16) ||
-      (a.dR && !aligned(a.dR, a.ldr * es, a.M, 16)) || a.N > 2048 * VEC)
-    return false;
-  return ring_shape((uint32_t)(a.N * ((a.dR ? 2 : 1) * es + xe)), most, ctas, stages);
-}
-
-template <typename T, bool X8, int V, int THREADS, int CTAS>
-int launch_bwd_ring(const BwdArgs& a, unsigned blocks, int stages, cudaStream_t s) {
+template <typename T, bool X8, int V, bool HOLD>
+int launch_bwd_ring(const BwdArgs& a, int threads, unsigned blocks, int stages, cudaStream_t s) {
   const uint32_t yb = (uint32_t)(a.N * (int64_t)sizeof(T)), xb = X8 ? (uint32_t)a.N : yb;
-  auto fn = rmsnorm_bwd_ring_kernel<T, X8, V, THREADS, CTAS>;
+  auto fn = rmsnorm_bwd_ring_kernel<T, X8, V, HOLD>;
   static std::atomic<uint64_t> ready{0};
   const int rc = raise_smem(fn, ready);
   if (rc != B2G_OK) return rc;
-  fn<<<blocks, THREADS, (uint32_t)stages * ((a.dR ? 2 : 1) * yb + xb + 8), s>>>(
+  fn<<<blocks, threads, (uint32_t)stages * ((a.dR ? 2 : 1) * yb + xb + 8), s>>>(
       a, stages, yb, xb, (uint64_t)launch_options().timeout_ns);
   return launched("rmsnorm_bwd_ring_kernel");
 }
 
-template <typename T, bool X8>
-int bwd_ring(const BwdArgs& a, unsigned blocks, int stages, cudaStream_t s) {
-  const int64_t nv = a.N / (16 / (int)sizeof(T));
-  if (nv <= 128) return launch_bwd_ring<T, X8, 1, 128, 8>(a, blocks, stages, s);
-  if (nv <= 256) return launch_bwd_ring<T, X8, 2, 128, 6>(a, blocks, stages, s);
-  if (nv <= 512) return launch_bwd_ring<T, X8, 4, 128, 4>(a, blocks, stages, s);
-  if (nv <= 1024) return launch_bwd_ring<T, X8, 4, 256, 2>(a, blocks, stages, s);
-  return launch_bwd_ring<T, X8, 8, 256, 1>(a, blocks, stages, s);
-}
-
+// Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel, others (and a
+// checkpoint of another 16- or 32-bit type than dY's) on the simple one.
 template <typename T>
 int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
-  const int64_t nv = a.N / (16 / (int)sizeof(T));
-  int ctas = nv <= 128 ? 8 : nv <= 256 ? 6 : nv <= 512 ? 4 : nv <= 1024 ? 2 : 1, stages = 0;
-  const bool ring = (x8 || same) && bwd_ring_ok<T>(a, x8, ctas, &ctas, &stages);
+  constexpr int VEC = 16 / (int)sizeof(T), V = 16 / VEC;  // 16 elements a thread
+  const int es = (int)sizeof(T), xe = x8 ? 1 : es;
+  const int64_t nv = a.N / VEC;
+  const bool hold = nv <= 512 * V;
+  const int threads = (int)((nv + (hold ? V : 2 * V) * 32 - 1) / ((hold ? V : 2 * V) * 32)) * 32;
+  int ctas = std::max(1, 512 / std::max(threads, 32)), stages = 0;
+  const bool ring = (x8 || same) && a.N % VEC == 0 && a.N * xe % 16 == 0 && nv <= 1024 * V &&
+                    aligned(a.dY, a.ldy * es, a.M, 16) && aligned(a.X, a.ldx * xe, a.M, 16) &&
+                    aligned(a.dX, a.lddx * es, a.M, 16) && (!a.dR || aligned(a.dR, a.ldr * es, a.M, 16)) &&
+                    ring_shape((uint32_t)(a.N * ((a.dR ? 2 : 1) * es + xe)), ctas, &ctas, &stages);
   const unsigned blocks = ring ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas) : row_blocks(a.M, sms);
   Workspace ws(s);
   int rc = B2G_OK;
@@ -896,14 +910,18 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
     if (rc != B2G_OK) return rc;
     a.part = static_cast<float*>(ws.get());
   }
-  if (ring) {
-    rc = x8 ? bwd_ring<T, true>(a, blocks, stages, s) : bwd_ring<T, false>(a, blocks, stages, s);
-  } else {
+  if (!ring) {
     rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
     rc = launched("rmsnorm_bwd_kernel");
+  } else if (hold) {
+    rc = x8 ? launch_bwd_ring<T, true, V, true>(a, threads, blocks, stages, s)
+            : launch_bwd_ring<T, false, V, true>(a, threads, blocks, stages, s);
+  } else {
+    rc = x8 ? launch_bwd_ring<T, true, 2 * V, false>(a, threads, blocks, stages, s)
+            : launch_bwd_ring<T, false, 2 * V, false>(a, threads, blocks, stages, s);
   }
   if (rc != B2G_OK || !dw) return rc;
-  dw_sum_kernel<<<(unsigned)((a.N + 31) / 32), kRowThreads, 0, s>>>(a.part, dw, a.N, (int)blocks);
+  dw_sum_kernel<<<(unsigned)((a.N + 31) / 32), 1024, 0, s>>>(a.part, dw, a.N, (int)blocks);
   return launched("dw_sum_kernel");
 }
 

@@ -60,6 +60,7 @@ enum {
   B2G_PATH_GENERIC = 3,   /* generic CUDA kernel (layouts outside TMA's rules) */
   B2G_PATH_ZERO = 4,      /* K == 0: C filled with zeros */
   B2G_PATH_EMPTY = 5,     /* M == 0 or N == 0: nothing to do */
+  B2G_PATH_FEW = 6,       /* b2g_gemm_q8 of a few tokens: weights straight into warp-level MMAs */
 };
 
 /*

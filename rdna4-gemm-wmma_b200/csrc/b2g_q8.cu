@@ -101,6 +101,156 @@ unsigned tile_blocks(int64_t rows, int64_t cols, int sms) {
   return (unsigned)std::min<int64_t>(t, (int64_t)sms * 32);
 }
 
+// ------------------------------------------------------------------ few tokens
+// D (16 x 8, 32-bit) += A (16 x 32 bytes) . B (32 bytes x 8): int8 into int32, or e4m3 into fp32.
+template <bool I8>
+__device__ __forceinline__ void mma_16x8x32(uint32_t (&d)[4], const uint32_t a0, const uint32_t a1,
+                                            const uint32_t a2, const uint32_t a3, const uint32_t b0,
+                                            const uint32_t b1) {
+  if constexpr (I8)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Products of a few tokens are bound by the weights' bytes: N * K of them, each used once a token.  So
+// the weights go from memory straight into the registers of warp-level MMAs, as their 16-row side
+// (the tokens are its 8 columns), with no shared memory, tile pipeline or split-K workspace between.
+// The order of K inside a product does not matter, so a lane's fragments are whole 16-byte pieces:
+// lane (g, t) of a warp takes bytes [16 t, 16 t + 16) of each 64-byte step of weight rows g and
+// g + 8 and of token g, and feeds two MMAs from them.
+//
+// A block has MT * 16 weight rows; its warps take K in turns of U steps and add their sums through
+// shared memory, in warp order.  The next turn's weights are loaded before this turn's products.
+template <bool I8, int MT, int NT, int U>
+__global__ void __launch_bounds__(512, 1)
+    gemm_q8_few_kernel(const int8_t* __restrict__ A, const int8_t* __restrict__ B, void* __restrict__ C,
+                       int M, int64_t N, int K, int64_t lda, int64_t ldb, int64_t ldc,
+                       const float* __restrict__ a_scale, const float* __restrict__ b_scale,
+                       const float* __restrict__ bias, int c_dtype) {
+  extern __shared__ uint32_t part[];  // [warps][MT * 16][NT * 8 + 1]
+  constexpr int COLS = NT * 8, PITCH = COLS + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t n0 = (int64_t)blockIdx.x * (MT * 16);
+  const int8_t* w[MT][2];  // rows past N read the last one; their sums are not stored
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[i][h] = B + min(n0 + i * 16 + h * 8 + g, N - 1) * ldb + t * 16;
+  const int8_t* x[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) x[j] = A + (int64_t)min(j * 8 + g, M - 1) * lda + t * 16;
+  uint32_t acc[MT][NT][4] = {};
+  uint4 cur[U][MT][2], nxt[U][MT][2];
+  const int step = warps * U * 64;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  auto fetch = [&](int k, uint4 (&d)[U][MT][2]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          d[u][i][h] = k + u * 64 + t * 16 < K ? __ldcs(reinterpret_cast<const uint4*>(w[i][h] + k + u * 64)) : zero;
+  };
+  int k = warp * U * 64;
+  if (k < K) fetch(k, cur);
+  for (; k < K; k += step) {
+    if (k + step < K) fetch(k + step, nxt);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = k + u * 64 + t * 16 < K;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint4 b = in ? __ldg(reinterpret_cast<const uint4*>(x[j] + k + u * 64)) : zero;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const uint4 p = cur[u][i][0], q = cur[u][i][1];
+          mma_16x8x32<I8>(acc[i][j], p.x, q.x, p.y, q.y, b.x, b.y);
+          mma_16x8x32<I8>(acc[i][j], p.z, q.z, p.w, q.w, b.z, b.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) cur[u][i][h] = nxt[u][i][h];
+  }
+  // row g (+ 8) of the weights, tokens 2 t and 2 t + 1
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      uint32_t* p = part + (warp * MT * 16 + i * 16 + g) * PITCH + j * 8 + 2 * t;
+      p[0] = acc[i][j][0];
+      p[1] = acc[i][j][1];
+      p[8 * PITCH] = acc[i][j][2];
+      p[8 * PITCH + 1] = acc[i][j][3];
+    }
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * 16 * M; o += blockDim.x) {
+    const int row = o % (MT * 16), m = o / (MT * 16);
+    const int64_t n = n0 + row;
+    if (n >= N) continue;
+    const uint32_t* p = part + row * PITCH + m;
+    float v;
+    if constexpr (I8) {
+      int s = 0;
+      for (int i = 0; i < warps; ++i) s += (int)p[i * MT * 16 * PITCH];
+      v = (float)s;
+    } else {
+      v = 0.0f;
+      for (int i = 0; i < warps; ++i) v += __uint_as_float(p[i * MT * 16 * PITCH]);
+    }
+    if (a_scale) v *= a_scale[m];
+    if (b_scale) v *= b_scale[n];
+    if (bias) v += bias[n];
+    store_elem(C, (int64_t)m * ldc + n, c_dtype, v);
+  }
+}
+
+struct FewArgs {
+  const void *A, *B;
+  void* C;
+  int64_t M, N, K, lda, ldb, ldc;
+  const float *a_scale, *b_scale, *bias;
+  int c_dtype;
+};
+
+// Up to this many tokens take the few-token kernel.  Measured at N = K = 8192, int8 (us a call): 1 token
+// 15.0 against the tensor-core tiles' 22.7, 8 tokens 15.3 against 22.6, 16 tokens 18.7 against 21.6,
+// 32 tokens 24.8 against 21.6; 28672 x 8192, 1 token: 43.5 against 62.8.
+constexpr int64_t kFewTokens = 16;
+
+// Warps of a block: as many (4 to 16) as give the GPU about 16 an SM, each with a whole turn of K.
+template <bool I8, int MT, int NT, int U>
+int launch_few(const FewArgs& a, int sms, cudaStream_t s) {
+  const int64_t blocks = (a.N + MT * 16 - 1) / (MT * 16);
+  int warps = 4;
+  while (warps < 16 && warps * 2 * MT * 16 * (NT * 8 + 1) * 4 <= 48 * 1024 && blocks * warps < (int64_t)sms * 16 && a.K >= (int64_t)warps * 2 * U * 64) warps *= 2;
+  const uint32_t smem = (uint32_t)(warps * MT * 16 * (NT * 8 + 1)) * 4;
+  gemm_q8_few_kernel<I8, MT, NT, U><<<(unsigned)blocks, warps * 32, smem, s>>>(
+      static_cast<const int8_t*>(a.A), static_cast<const int8_t*>(a.B), a.C, (int)a.M, a.N, (int)a.K, a.lda,
+      a.ldb, a.ldc, a.a_scale, a.b_scale, a.bias, a.c_dtype);
+  return launched("gemm_q8_few_kernel");
+}
+
+template <bool I8>
+int few_tokens(const FewArgs& a, int sms, cudaStream_t s) {
+  return a.M <= 8 ? launch_few<I8, 1, 1, 4>(a, sms, s) : launch_few<I8, 1, 2, 4>(a, sms, s);
+}
+
 // ------------------------------------------------------------------ aligned copies
 // Rows of `bytes` bytes from pitch `sp` to pitch `dp` (a multiple of 16), for operands whose base
 // or pitch TMA cannot address.  U: the widest power of two up to 4 that divides both.  One word of
@@ -423,6 +573,12 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
     rc = aligned_rows(&A, &lda, M, K, sms, wa, s);
     if (rc == B2G_OK) rc = aligned_rows(&B, &ldb, N, K, sms, wb, s);
     if (rc != B2G_OK) return rc;
+    if (M <= kFewTokens && K % 16 == 0 && (N + 15) / 16 <= INT32_MAX) {
+      const FewArgs f = {A, B, C, M, N, K, lda, ldb, ldc, a_scale, b_scale, bias, c_dtype};
+      rc = dtype == B2G_DTYPE_I8 ? few_tokens<true>(f, sms, s) : few_tokens<false>(f, sms, s);
+      if (rc == B2G_OK) set_path(B2G_PATH_FEW);
+      return rc;
+    }
     const Product g = {dtype == B2G_DTYPE_I8 ? Q_I8 : Q_FP8, A, B, C, M, N, K, lda, ldb, ldc, 0,
                        c_type_of(c_dtype), false, a_scale, b_scale, bias};
     return launch_product(g, dev, sms, s);

@@ -148,7 +148,14 @@ __device__ __forceinline__ void load_weights(const void* W, int w_dtype, bool ve
     }
   }
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) w[j] = n + j < N ? load_elem(W, n + j, w_dtype) : 0.0f;
+  for (int j = 0; j < VEC; ++j) {  // (no branch around the loads, which would then follow one another)
+    uint32_t bits = 0;
+    if (n + j < N && w_dtype == B2G_DTYPE_F32) bits = __ldg(static_cast<const uint32_t*>(W) + n + j);
+    if (n + j < N && w_dtype != B2G_DTYPE_F32) bits = __ldg(static_cast<const uint16_t*>(W) + n + j);
+    w[j] = w_dtype == B2G_DTYPE_F32    ? __uint_as_float(bits)
+           : w_dtype == B2G_DTYPE_BF16 ? __uint_as_float(bits << 16)
+                                       : __half2float(__ushort_as_half((unsigned short)bits));
+  }
 }
 
 __device__ __forceinline__ bool weights_vec(const void* W, int w_dtype) {
@@ -189,13 +196,13 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, float* buf
 // Rows into 8 bits, each row held in registers: one pass over the data.  A row belongs to LANES lanes of
 // a warp (short rows) or, LANES = 0, to the block; a thread holds V vectors of VEC elements of it,
 // `threads` vectors apart.  Blocks stride over the rows; where registers allow (AHEAD: blocks of up
-// to 256 threads) a row's loads are issued before the previous row is reduced, so that the
-// reduction is not waited out with the memory idle.
+// to 256 threads, and single elements) a row's loads are issued before the previous row is reduced,
+// so that the reduction is not waited out with the memory idle, and the weights stay in registers.
 //
 // Per row: sum of squares and largest |h * w| (|x| without the norm).  The largest |y| is rstd
 // times that, so one reduction serves both; rstd cancels from the 8-bit values (row_quant).
 template <typename T, bool NORM, int VEC, int V, int LANES, bool AHEAD>
-__global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 5 : AHEAD ? 2 : 1)
+__global__ void __launch_bounds__(LANES ? 128 : AHEAD && VEC > 1 ? 256 : 1024, LANES ? 4 : AHEAD && VEC > 1 ? 2 : 1)
     rows_to_q8_kernel(const NormArgs a) {
   __shared__ float buf[128];
   constexpr int PER = LANES ? 128 / LANES : 1;  // rows a block holds at once
@@ -216,6 +223,10 @@ __global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 5 : 
       for (int i = 0; i < V; ++i) r[i] = load_vec<T, VEC>(R + m * a.ldr, (i * threads + tid) * VEC, N);
   };
   if (AHEAD && first < a.M) fetch(first);
+  float wreg[NORM && AHEAD ? V : 1][VEC];
+  if constexpr (NORM && AHEAD)
+#pragma unroll
+    for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, wreg[i]);
   int parity = 0;
   // (the lanes of a warp stay together: those whose rows have run out go on with the last row's
   // values until the warp's first row is past the end, and store nothing)
@@ -224,8 +235,7 @@ __global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 5 : 
     const bool live = m < a.M;
     if (!AHEAD && live) fetch(m);
     float v[V][VEC];
-    float ss = 0.0f;
-    uint32_t top = 0;
+    float ss = 0.0f, ftop = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int n = (i * threads + tid) * VEC;
@@ -243,16 +253,17 @@ __global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 5 : 
           store_vec<T, VEC>(static_cast<T*>(a.H) + m * a.ldh, n, N, h);
         }
         float w[VEC];
-        load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
+        if constexpr (!AHEAD) load_weights<VEC>(a.W, a.w_dtype, wvec, n, N, w);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           ss = fmaf(v[i][j], v[i][j], ss);
-          v[i][j] *= w[j];
+          v[i][j] *= AHEAD ? wreg[NORM && AHEAD ? i : 0][j] : w[j];
         }
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7fffffffu);
+      for (int j = 0; j < VEC; ++j) ftop = max_abs(ftop, v[i][j]);
     }
+    uint32_t top = __float_as_uint(ftop);
     if (AHEAD && m + step < a.M) fetch(m + step);
     row_reduce<LANES, NORM>(ss, top, buf, parity);
     if (!live) continue;
@@ -455,15 +466,16 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const Norm
 }
 
 // Rows out of 8 bits.  Memory-bound: 1 byte in, 2 or 4 out.  A block does one piece of a row, PIECE
-// vectors of 16 values a thread (one value a thread where !VEC16), all loads before the first store.
-constexpr int kPiece = 2;
+// vectors of 16 values a thread (8 single values, a block's width apart, where !VEC16), all loads
+// before the first store.
+constexpr int kPiece = 2, kPieceElems = 8;
 
 template <typename T, bool VEC16>
 __global__ void __launch_bounds__(kRowThreads)
     dequantize_kernel(const uint8_t* Q, const float* scale, T* X, int64_t M, int64_t N, int64_t ldq,
                       int64_t ldx, int q_dtype, float top) {
   constexpr int VEC = VEC16 ? 16 : 1, OUT = 16 / (int)sizeof(T);
-  const int per_block = kRowThreads * kPiece * VEC;
+  const int per_block = kRowThreads * (VEC16 ? kPiece * VEC : kPieceElems);
   const int64_t bpr = (N + per_block - 1) / per_block;  // pieces of a row
   for (int64_t b = blockIdx.x; b < M * bpr; b += gridDim.x) {
     const int64_t m = b / bpr, n0 = (b - m * bpr) * per_block + (int64_t)threadIdx.x * VEC;
@@ -505,9 +517,16 @@ __global__ void __launch_bounds__(kRowThreads)
         }
       }
     } else {
+      uint8_t c[kPieceElems];
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i)
-        if (n0 + (int64_t)i * kRowThreads < N) one(n0 + (int64_t)i * kRowThreads);
+      for (int i = 0; i < kPieceElems; ++i) c[i] = n0 + i * kRowThreads < N ? q[n0 + i * kRowThreads] : 0;
+#pragma unroll
+      for (int i = 0; i < kPieceElems; ++i)
+        if (n0 + i * kRowThreads < N) {
+          const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c[i]
+                                                  : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c[i]));
+          from_f(x + n0 + i * kRowThreads, clamp_to(v * s, top));
+        }
     }
   }
 }
@@ -719,6 +738,74 @@ __global__ void __launch_bounds__(512, 1)
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
+// The same element by element, for rows without 16-byte alignment: a thread holds V elements of a row, a
+// block's width apart; the next row's loads are issued before this row is reduced.
+template <typename T, bool X8, int V>
+__global__ void __launch_bounds__(1024, 1) rmsnorm_bwd_elems_kernel(const BwdArgs a) {
+  using XT = typename std::conditional<X8, uint8_t, T>::type;
+  __shared__ float buf[128];
+  const int tid = (int)threadIdx.x, threads = (int)blockDim.x, N = (int)a.N;
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  const T* dY = static_cast<const T*>(a.dY);
+  const T* dR = static_cast<const T*>(a.dR);
+  const XT* X = static_cast<const XT*>(a.X);
+  Vec<T, 1> y[V], r[V];
+  Vec<XT, 1> x[V];
+  auto fetch = [&](int64_t m) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = load_vec<T, 1>(dY + m * a.ldy, i * threads + tid, N);
+#pragma unroll
+    for (int i = 0; i < V; ++i) x[i] = load_vec<XT, 1>(X + m * a.ldx, i * threads + tid, N);
+    if (dR)
+#pragma unroll
+      for (int i = 0; i < V; ++i) r[i] = load_vec<T, 1>(dR + m * a.ldr, i * threads + tid, N);
+  };
+  fetch(first);
+  float w[V], dw[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float f[1];
+    load_weights<1>(a.W, a.w_dtype, false, i * threads + tid, N, f);
+    w[i] = f[0];
+    dw[i] = 0.0f;
+  }
+  int parity = 0;
+  for (int64_t m = first; m < a.M; m += step, parity ^= 1) {
+    const float rstd = __ldg(a.rstd + m);
+    const float xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    float g[V], xh[V], dr[V];
+    float c = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float dy = to_f(y[i].e[0]);
+      if constexpr (X8) {
+        const uint8_t b = x[i].e[0];
+        xh[i] = (a.x_dtype == B2G_DTYPE_I8 ? (float)(int8_t)b : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&b))) * xs;
+      } else {
+        xh[i] = to_f(x[i].e[0]) * xs;
+      }
+      g[i] = dy * w[i];
+      dw[i] = fmaf(dy, xh[i], dw[i]);
+      dr[i] = dR ? to_f(r[i].e[0]) : 0.0f;
+      c = fmaf(g[i], xh[i], c);
+    }
+    if (m + step < a.M) fetch(m + step);
+    uint32_t unused = 0;
+    row_reduce<0, true>(c, unused, buf, parity);
+    c /= (float)N;
+    T* dX = static_cast<T*>(a.dX) + m * a.lddx;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = i * threads + tid;
+      if (n < N) from_f(dX + n, fmaf(xh[i], -c * rstd, g[i] * rstd) + dr[i]);
+    }
+  }
+  if (a.part)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * threads + tid < N) a.part[(int64_t)blockIdx.x * N + i * threads + tid] = dw[i];
+}
+
 // dw[n] = the blocks' partial sums: a block sums 32 columns, its warp w the rows w, w + 32, ..., and the
 // warps' sums are added in order.
 __global__ void __launch_bounds__(1024) dw_sum_kernel(const float* part, float* dw, int64_t N, int rows) {
@@ -840,8 +927,7 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
     if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, 0, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
   } else {
     if (a.N <= 32 * 8) return launch_rows<T, NORM, 1, 8, 32>(a, 0, sms, s);
-    if (a.N <= 256 * 8) return launch_rows<T, NORM, 1, 8, 0>(a, (int)(a.N + 255) / 256 * 32, sms, s);
-    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, 0, false>(a, (int)(a.N + 255) / 256 * 32, sms, s);
+    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, 0>(a, (int)(a.N + 255) / 256 * 32, sms, s);
     if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, 0, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
   }
   long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
@@ -867,7 +953,7 @@ int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N,
                   int q_dtype, float top, int sms, cudaStream_t s) {
   const uint8_t* q = static_cast<const uint8_t*>(Q);
   const bool vec = aligned(Q, ldq, M, 16) && aligned(X, ldx * (int64_t)sizeof(T), M, 16);
-  const int64_t per_block = kRowThreads * kPiece * (vec ? 16 : 1);
+  const int64_t per_block = kRowThreads * (vec ? kPiece * 16 : kPieceElems);
   const int64_t blocks = std::min<int64_t>(M * ((N + per_block - 1) / per_block), (int64_t)sms * 1024);
   if (vec)
     dequantize_kernel<T, true><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
@@ -888,8 +974,9 @@ int launch_bwd_ring(const BwdArgs& a, int threads, unsigned blocks, int stages, 
   return launched("rmsnorm_bwd_ring_kernel");
 }
 
-// Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel, others (and a
-// checkpoint of another 16- or 32-bit type than dY's) on the simple one.
+// Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel; others of up to 8192
+// elements element by element in registers; longer ones (and a checkpoint of another 16- or 32-bit
+// type than dY's) in two passes.
 template <typename T>
 int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T), V = 16 / VEC;  // 16 elements a thread
@@ -902,7 +989,11 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
                     aligned(a.dY, a.ldy * es, a.M, 16) && aligned(a.X, a.ldx * xe, a.M, 16) &&
                     aligned(a.dX, a.lddx * es, a.M, 16) && (!a.dR || aligned(a.dR, a.ldr * es, a.M, 16)) &&
                     ring_shape((uint32_t)(a.N * ((a.dR ? 2 : 1) * es + xe)), ctas, &ctas, &stages);
-  const unsigned blocks = ring ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas) : row_blocks(a.M, sms);
+  const bool elems = !ring && (x8 || same) && a.N <= 8192;
+  const int ethreads = (int)((a.N + 255) / 256 * 32);
+  if (elems) ctas = std::max(1, 1024 / ethreads);
+  const unsigned blocks = ring || elems ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas)
+                                        : row_blocks(a.M, sms);
   Workspace ws(s);
   int rc = B2G_OK;
   if (dw) {
@@ -910,7 +1001,13 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
     if (rc != B2G_OK) return rc;
     a.part = static_cast<float*>(ws.get());
   }
-  if (!ring) {
+  if (elems) {
+    if (x8)
+      rmsnorm_bwd_elems_kernel<T, true, 8><<<blocks, ethreads, 0, s>>>(a);
+    else
+      rmsnorm_bwd_elems_kernel<T, false, 8><<<blocks, ethreads, 0, s>>>(a);
+    rc = launched("rmsnorm_bwd_elems_kernel");
+  } else if (!ring) {
     rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
     rc = launched("rmsnorm_bwd_kernel");
   } else if (hold) {

@@ -344,8 +344,8 @@ int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t 
  *   - Any leading dimension >= the row length (in elements) and any alignment of the element type
  *     are accepted.  Row pitches and base addresses that are multiples of 16 bytes run fastest:
  *     elsewhere the row kernels load elements one by one and the products copy the operand into
- *     an aligned workspace first.  Elements between the row length and the pitch are neither
- *     read nor written.
+ *     an aligned workspace first.  Elements between the row length and the pitch are not written,
+ *     and their values are never used.
  *   - Pointers belong to the current device.  Every pointer the call needs has to be non-null
  *     unless it is said to be optional.  M == 0 is valid everywhere.
  *   - Outputs may not overlap inputs or each other, except where said.

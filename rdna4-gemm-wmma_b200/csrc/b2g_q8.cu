@@ -252,22 +252,45 @@ int few_tokens(const FewArgs& a, int sms, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------------ aligned copies
-// Rows of `bytes` bytes from pitch `sp` to pitch `dp` (a multiple of 16), for operands whose base
-// or pitch TMA cannot address.  U: the widest power of two up to 4 that divides both.  One word of
-// the copy per thread; bytes of the copy past the row are not written (TMA never reads them).
-template <typename U>
+// Rows of `bytes` bytes from pitch `sp` to pitch `dp` (a multiple of 16), for operands whose base or
+// pitch TMA cannot address.  A warp copies 512 bytes of a row: each lane loads whole 4-byte words from
+// the word that holds its piece's first byte on, takes the next word from its neighbour and shifts
+// the two together.  Words that reach out of the matrix (its very ends) are put together from
+// bytes.  Bytes of the copy past the row get whatever follows the row: TMA never reads them.
 __global__ void __launch_bounds__(256)
     repack_kernel(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t bytes, int64_t sp, int64_t dp) {
-  const int64_t words = (bytes + 3) / 4, total = rows * words;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / words, b = (i - r * words) * 4;
-    const uint8_t* s = src + r * sp + b;
-    uint32_t w = 0;
+  constexpr int U = 4;  // words a lane
+  const int lane = threadIdx.x & 31;
+  const int64_t pieces = (bytes + 128 * U - 1) / (128 * U), total = rows * pieces;
+  const uint8_t* const end = src + (rows - 1) * sp + bytes;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
+    const int64_t r = i / pieces, b = (i - r * pieces) * (128 * U);
+    const uint8_t* first = src + r * sp + b;
+    const uint32_t off = (uint32_t)(uintptr_t)first & 3u;
+    const uint8_t* base = first - off;
+    const int64_t left = bytes - b + off;  // bytes of the row from `base` on
+    auto word = [&](int64_t at) -> uint32_t {
+      const uint8_t* p = base + at;
+      if (at >= left) return 0;
+      if (p >= src && p + 4 <= end) return __ldcs(reinterpret_cast<const uint32_t*>(p));
+      uint32_t w = 0;
+      for (int k = 0; k < 4; ++k)
+        if (p + k >= src && p + k < end) w |= (uint32_t)p[k] << (8 * k);
+      return w;
+    };
+    uint32_t w[U], last = 0;
 #pragma unroll
-    for (int k = 0; k < 4; k += (int)sizeof(U))
-      if (b + k < bytes) w |= (uint32_t)*reinterpret_cast<const U*>(s + k) << (8 * k);
-    *reinterpret_cast<uint32_t*>(dst + r * dp + b) = w;
+    for (int u = 0; u < U; ++u) w[u] = word(u * 128 + lane * 4);
+    if (lane == 31) last = word(U * 128);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t next = __shfl_down_sync(0xffffffffu, w[u], 1);
+      const uint32_t wrap = u + 1 < U ? __shfl_sync(0xffffffffu, w[u + 1 < U ? u + 1 : u], 0) : last;
+      if (lane == 31) next = wrap;
+      const int64_t at = b + u * 128 + lane * 4;
+      if (at < bytes) *reinterpret_cast<uint32_t*>(dst + r * dp + at) = __funnelshift_r(w[u], next, off * 8);
+    }
   }
 }
 
@@ -279,17 +302,11 @@ int aligned_rows(const void** p, int64_t* pitch, int64_t rows, int64_t bytes, in
   const int64_t dp = (bytes + 15) / 16 * 16;
   int rc = ws.alloc((size_t)(rows * dp), "cudaMallocFromPoolAsync(aligned copy)");
   if (rc != B2G_OK) return rc;
-  const unsigned blocks = (unsigned)std::min<int64_t>((rows * ((bytes + 3) / 4) + 255) / 256, (int64_t)sms * 32);
-  const uint8_t* src = static_cast<const uint8_t*>(*p);
-  uint8_t* dst = static_cast<uint8_t*>(ws.get());
-  if ((low & 3) == 0 && bytes % 4 == 0)
-    repack_kernel<uint32_t><<<blocks, 256, 0, s>>>(src, dst, rows, bytes, *pitch, dp);
-  else if ((low & 1) == 0 && bytes % 2 == 0)
-    repack_kernel<uint16_t><<<blocks, 256, 0, s>>>(src, dst, rows, bytes, *pitch, dp);
-  else
-    repack_kernel<uint8_t><<<blocks, 256, 0, s>>>(src, dst, rows, bytes, *pitch, dp);
+  const unsigned blocks = (unsigned)std::min<int64_t>((rows * ((bytes + 511) / 512) + 7) / 8, (int64_t)sms * 32);
+  repack_kernel<<<blocks, 256, 0, s>>>(static_cast<const uint8_t*>(*p), static_cast<uint8_t*>(ws.get()), rows, bytes,
+                                       *pitch, dp);
   rc = launched("repack_kernel");
-  *p = dst;
+  *p = ws.get();
   *pitch = dp;
   return rc;
 }

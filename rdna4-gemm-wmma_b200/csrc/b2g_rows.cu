@@ -430,6 +430,117 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
+// Bulk copy of a row of `bytes` bytes without 16-byte alignment: the whole 16-byte pieces that hold it.
+// The pieces at its ends reach up to 15 bytes into the neighbouring rows, whose bytes are not used;
+// the matrix's first and last row, whose pieces could reach out of it, are never copied this way.
+__device__ __forceinline__ uint32_t span_bytes(const void* row, uint32_t bytes) {
+  return (((uint32_t)(uintptr_t)row & 15u) + bytes + 15u) & ~15u;
+}
+__device__ __forceinline__ void span_load(uint32_t dst, const void* row, uint32_t bytes, uint32_t bar) {
+  ptx::bulk_load(dst, reinterpret_cast<const void*>((uintptr_t)row & ~(uintptr_t)15), span_bytes(row, bytes), bar);
+}
+__device__ __forceinline__ uint32_t low4(const void* p) { return (uint32_t)(uintptr_t)p & 15u; }
+
+// rows_ring_kernel for rows of any alignment, element by element: element i * THREADS + tid of a row is a
+// thread's, so that shared and global accesses of a warp are consecutive.  Q, H and the first and
+// last row go through ordinary accesses.  Instructions are the limit here (one access an element and
+// operand), so THREADS is a constant: every address is one base with a constant offset.
+template <typename T, bool NORM, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
+    rows_ring_elems_kernel(const NormArgs a, int stages, uint32_t slot, uint64_t limit_ns) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float buf[128];
+  __shared__ int abort_flag;
+  const int tid = (int)threadIdx.x;
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  const T* X = static_cast<const T*>(a.X);
+  const T* R = NORM ? static_cast<const T*>(a.R) : nullptr;
+  const int N = (int)a.N;
+  const uint32_t row_bytes = (uint32_t)N * (uint32_t)sizeof(T);
+  const Ring ring = make_ring(smem, stages, R ? 2 * slot : slot, limit_ns, &abort_flag);
+  auto at_end = [&](int64_t m) { return m == 0 || m == a.M - 1; };
+  auto fill = [&](int64_t m, int k) {
+    const uint32_t bar = ring.bar(k), dst = ring.stage(k);
+    if (at_end(m)) {
+      ptx::mbar_arrive(bar);  // read from global memory when its turn comes
+      return;
+    }
+    const T* x = X + m * a.ldx;
+    const T* r = R ? R + m * a.ldr : nullptr;
+    ptx::mbar_arrive_expect_tx(bar, span_bytes(x, row_bytes) + (R ? span_bytes(r, row_bytes) : 0));
+    span_load(dst, x, row_bytes, bar);
+    if (R) span_load(dst + slot, r, row_bytes, bar);
+  };
+  int issued = 0;
+  if (tid == 0)
+    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+  float w[NORM ? V : 1];
+  if constexpr (NORM)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float f[1];
+      load_weights<1>(a.W, a.w_dtype, false, i * THREADS + tid, N, f);
+      w[i] = f[0];
+    }
+  int k = 0;
+  for (int64_t m = first; m < a.M; m += step, ++k) {
+    const bool ok = ring.wait(k), end = at_end(m);
+    const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
+    const T* gx = X + m * a.ldx;
+    const T* gr = R ? R + m * a.ldr : nullptr;
+    const T* sx = reinterpret_cast<const T*>(st + low4(gx));
+    const T* sr = reinterpret_cast<const T*>(st + slot + low4(gr));
+    float v[V];
+    float sum = 0.0f, top = 0.0f;
+    const int count = N - tid;  // element i is in the row if i * THREADS < count
+    auto take = [&](const T* x, const T* r) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = i * THREADS < count ? to_f(x[i * THREADS]) : 0.0f;
+      if (NORM && R)
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] += i * THREADS < count ? to_f(r[i * THREADS]) : 0.0f;
+    };
+    if (end)
+      take(gx + tid, gr + tid);
+    else
+      take(sx + tid, sr + tid);
+    if (NORM && a.H) {
+      T* h = static_cast<T*>(a.H) + m * a.ldh + tid;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i * THREADS < count) from_f(h + i * THREADS, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if constexpr (NORM) {
+        sum = fmaf(v[i], v[i], sum);
+        v[i] *= w[NORM ? i : 0];
+      }
+      top = max_abs(top, v[i]);
+    }
+    uint32_t bits = ok ? __float_as_uint(top) : 0x7fffffffu;
+    row_reduce<0, NORM>(sum, bits, buf, k & 1);
+    if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
+      fill(m + step * stages, k + stages);  // every thread has read this row (row_reduce)
+      ++issued;
+    }
+    const float rstd = NORM ? 1.0f / sqrtf(sum / (float)N + a.eps) : 1.0f;
+    const RowQuant rq = row_quant(bits, rstd, q_max(a.q_dtype), a.pow2);
+    if (tid == 0) {
+      a.scale[m] = rq.scale;
+      if (NORM && a.rstd) a.rstd[m] = rstd;
+    }
+    const bool bad = rq.scale != rq.scale;
+    uint8_t* q = static_cast<uint8_t*>(a.Q) + m * a.ldq + tid;
+    uint32_t o[V];
+    round_q8<V>(v, rq, a.q_dtype, bad, o);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * THREADS < count) q[i * THREADS] = (uint8_t)o[i];
+  }
+  if (tid == 0 && *ring.abort_flag) ring.drain(issued);
+}
+
 // The same for rows too long for a block's registers: two passes over the row, element by element.
 __global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const NormArgs a) {
   __shared__ float buf[kRowThreads / 32];
@@ -738,72 +849,116 @@ __global__ void __launch_bounds__(512, 1)
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
-// The same element by element, for rows without 16-byte alignment: a thread holds V elements of a row, a
-// block's width apart; the next row's loads are issued before this row is reduced.
-template <typename T, bool X8, int V>
-__global__ void __launch_bounds__(1024, 1) rmsnorm_bwd_elems_kernel(const BwdArgs a) {
+// The same for rows of any alignment, element by element (as rows_ring_elems_kernel).
+template <typename T, bool X8, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS)
+    rmsnorm_bwd_elems_kernel(const BwdArgs a, int stages, uint32_t y_slot, uint32_t x_slot, uint64_t limit_ns) {
   using XT = typename std::conditional<X8, uint8_t, T>::type;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float buf[128];
-  const int tid = (int)threadIdx.x, threads = (int)blockDim.x, N = (int)a.N;
+  __shared__ int abort_flag;
+  const int tid = (int)threadIdx.x, N = (int)a.N;
   const int64_t first = blockIdx.x, step = gridDim.x;
   const T* dY = static_cast<const T*>(a.dY);
   const T* dR = static_cast<const T*>(a.dR);
   const XT* X = static_cast<const XT*>(a.X);
-  Vec<T, 1> y[V], r[V];
-  Vec<XT, 1> x[V];
-  auto fetch = [&](int64_t m) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) y[i] = load_vec<T, 1>(dY + m * a.ldy, i * threads + tid, N);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = load_vec<XT, 1>(X + m * a.ldx, i * threads + tid, N);
-    if (dR)
-#pragma unroll
-      for (int i = 0; i < V; ++i) r[i] = load_vec<T, 1>(dR + m * a.ldr, i * threads + tid, N);
+  const uint32_t y_bytes = (uint32_t)N * (uint32_t)sizeof(T), x_bytes = (uint32_t)N * (uint32_t)sizeof(XT);
+  const Ring ring = make_ring(smem, stages, (dR ? 2 : 1) * y_slot + x_slot, limit_ns, &abort_flag);
+  auto at_end = [&](int64_t m) { return m == 0 || m == a.M - 1; };
+  auto fill = [&](int64_t m, int k) {
+    const uint32_t bar = ring.bar(k), dst = ring.stage(k);
+    if (at_end(m)) {
+      ptx::mbar_arrive(bar);  // read from global memory when its turn comes
+      return;
+    }
+    const T* y = dY + m * a.ldy;
+    const XT* x = X + m * a.ldx;
+    const T* r = dR ? dR + m * a.ldr : nullptr;
+    ptx::mbar_arrive_expect_tx(bar, span_bytes(y, y_bytes) + span_bytes(x, x_bytes) + (dR ? span_bytes(r, y_bytes) : 0));
+    span_load(dst, y, y_bytes, bar);
+    span_load(dst + y_slot, x, x_bytes, bar);
+    if (dR) span_load(dst + y_slot + x_slot, r, y_bytes, bar);
   };
-  fetch(first);
+  int issued = 0;
+  if (tid == 0)
+    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
   float w[V], dw[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float f[1];
-    load_weights<1>(a.W, a.w_dtype, false, i * threads + tid, N, f);
+    load_weights<1>(a.W, a.w_dtype, false, i * THREADS + tid, N, f);
     w[i] = f[0];
     dw[i] = 0.0f;
   }
-  int parity = 0;
-  for (int64_t m = first; m < a.M; m += step, parity ^= 1) {
+  int k = 0;
+  for (int64_t m = first; m < a.M; m += step, ++k) {
     const float rstd = __ldg(a.rstd + m);
     const float xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    const bool ok = ring.wait(k), end = at_end(m);
+    const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     float g[V], xh[V], dr[V];
     float c = 0.0f;
+    const int count = N - tid;  // element i is in the row if i * THREADS < count
+    auto take = [&](const T* y, const XT* x, const T* r) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float dy = to_f(y[i].e[0]);
-      if constexpr (X8) {
-        const uint8_t b = x[i].e[0];
-        xh[i] = (a.x_dtype == B2G_DTYPE_I8 ? (float)(int8_t)b : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&b))) * xs;
+      for (int i = 0; i < V; ++i) g[i] = i * THREADS < count ? to_f(y[i * THREADS]) : 0.0f;
+      if constexpr (!X8) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) xh[i] = i * THREADS < count ? to_f(x[i * THREADS]) : 0.0f;
+      } else if (a.x_dtype == B2G_DTYPE_I8) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)  // the byte, sign bit flipped, in the low byte of 2^23
+          xh[i] = __uint_as_float(0x4b000000u | ((i * THREADS < count ? x[i * THREADS] : 0u) ^ 0x80u)) - 8388736.0f;
       } else {
-        xh[i] = to_f(x[i].e[0]) * xs;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint8_t b = i * THREADS < count ? x[i * THREADS] : 0;
+          xh[i] = float(*reinterpret_cast<const __nv_fp8_e4m3*>(&b));
+        }
       }
-      g[i] = dy * w[i];
-      dw[i] = fmaf(dy, xh[i], dw[i]);
-      dr[i] = dR ? to_f(r[i].e[0]) : 0.0f;
+      if (dR)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dr[i] = i * THREADS < count ? to_f(r[i * THREADS]) : 0.0f;
+    };
+    const T* gy = dY + m * a.ldy;
+    const XT* gx = X + m * a.ldx;
+    const T* gr = dR ? dR + m * a.ldr : nullptr;
+    if (end)
+      take(gy + tid, gx + tid, gr + tid);
+    else
+      take(reinterpret_cast<const T*>(st + low4(gy)) + tid, reinterpret_cast<const XT*>(st + y_slot + low4(gx)) + tid,
+           reinterpret_cast<const T*>(st + y_slot + x_slot + low4(gr)) + tid);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {  // (a NaN scale must not reach elements past the row)
+      xh[i] *= xs;
+      if (i * THREADS >= count) xh[i] = 0.0f;
+      dw[i] = fmaf(g[i], xh[i], dw[i]);
+      g[i] *= w[i];
       c = fmaf(g[i], xh[i], c);
     }
-    if (m + step < a.M) fetch(m + step);
-    uint32_t unused = 0;
-    row_reduce<0, true>(c, unused, buf, parity);
-    c /= (float)N;
-    T* dX = static_cast<T*>(a.dX) + m * a.lddx;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int n = i * threads + tid;
-      if (n < N) from_f(dX + n, fmaf(xh[i], -c * rstd, g[i] * rstd) + dr[i]);
+    uint32_t late = ok ? 0u : 1u;
+    row_reduce<0, true>(c, late, buf, k & 1);
+    if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
+      fill(m + step * stages, k + stages);  // every thread holds its part of this row (row_reduce)
+      ++issued;
     }
+    c = late ? __int_as_float(0x7fc00000) : c / (float)N;
+    T* dX = static_cast<T*>(a.dX) + m * a.lddx + tid;
+    const float nc = -c * rstd;
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = fmaf(xh[i], nc, g[i] * rstd);
+    if (dR)
+#pragma unroll
+      for (int i = 0; i < V; ++i) g[i] += dr[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * THREADS < count) from_f(dX + i * THREADS, g[i]);
   }
   if (a.part)
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i * threads + tid < N) a.part[(int64_t)blockIdx.x * N + i * threads + tid] = dw[i];
+      if (i * THREADS + tid < N) a.part[(int64_t)blockIdx.x * N + i * THREADS + tid] = dw[i];
+  if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
 // dw[n] = the blocks' partial sums: a block sums 32 columns, its warp w the rows w, w + 32, ..., and the
@@ -898,6 +1053,22 @@ bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   return true;
 }
 
+// A launch of rows_ring_elems_kernel, or false where its stages do not fit.
+template <typename T, bool NORM, int THREADS, int V>
+bool launch_ring_elems(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
+  const uint32_t slot = ((uint32_t)(a.N * (int64_t)sizeof(T)) + 30u) & ~15u, stage = (a.R ? 2 : 1) * slot;
+  int ctas = V <= 16 ? 1024 / THREADS : 1, stages = 0;
+  if (!ring_shape(stage, ctas, &ctas, &stages)) return false;
+  auto fn = rows_ring_elems_kernel<T, NORM, THREADS, V>;
+  static std::atomic<uint64_t> ready{0};
+  *rc = raise_smem(fn, ready);
+  if (*rc != B2G_OK) return true;
+  fn<<<(unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas), THREADS, (uint32_t)stages * (stage + 8), s>>>(
+      a, stages, slot, (uint64_t)launch_options().timeout_ns);
+  *rc = launched("rows_ring_elems_kernel");
+  return true;
+}
+
 // Vectors of 16 bytes where every address and pitch allows, else single elements.  Rows of up to 128
 // vectors: four vectors a lane, several rows a warp; longer ones: a ring, or with few rows (latency
 // counts then) one block a row with its loads in registers.
@@ -927,8 +1098,14 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
     if (nv <= 4096) return launch_rows<T, NORM, VEC, 4, 0, false>(a, (int)(nv + 127) / 128 * 32, sms, s);
   } else {
     if (a.N <= 32 * 8) return launch_rows<T, NORM, 1, 8, 32>(a, 0, sms, s);
-    if (a.N <= 1024 * 8) return launch_rows<T, NORM, 1, 8, 0>(a, (int)(a.N + 255) / 256 * 32, sms, s);
-    if (a.N <= 1024 * 16) return launch_rows<T, NORM, 1, 16, 0, false>(a, (int)(a.N + 511) / 512 * 32, sms, s);
+    int rc = B2G_OK;
+    if (a.N <= 128 * 8 ? launch_ring_elems<T, NORM, 128, 8>(a, sms, s, &rc)
+        : a.N <= 128 * 16 ? launch_ring_elems<T, NORM, 128, 16>(a, sms, s, &rc)
+        : a.N <= 256 * 16 ? launch_ring_elems<T, NORM, 256, 16>(a, sms, s, &rc)
+        : a.N <= 512 * 16 ? launch_ring_elems<T, NORM, 512, 16>(a, sms, s, &rc)
+        : a.N <= 512 * 32 ? launch_ring_elems<T, NORM, 512, 32>(a, sms, s, &rc)
+                          : false)
+      return rc;
   }
   long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
   return launched("long_rows_to_q8_kernel");
@@ -974,6 +1151,27 @@ int launch_bwd_ring(const BwdArgs& a, int threads, unsigned blocks, int stages, 
   return launched("rmsnorm_bwd_ring_kernel");
 }
 
+template <typename T, bool X8, int THREADS, int V>
+int launch_bwd_elems(const BwdArgs& a, unsigned blocks, int stages, uint32_t y_slot, uint32_t x_slot,
+                     cudaStream_t s) {
+  auto fn = rmsnorm_bwd_elems_kernel<T, X8, THREADS, V>;
+  static std::atomic<uint64_t> ready{0};
+  const int rc = raise_smem(fn, ready);
+  if (rc != B2G_OK) return rc;
+  fn<<<blocks, THREADS, (uint32_t)stages * ((a.dR ? 2 : 1) * y_slot + x_slot + 8), s>>>(
+      a, stages, y_slot, x_slot, (uint64_t)launch_options().timeout_ns);
+  return launched("rmsnorm_bwd_elems_kernel");
+}
+
+template <typename T, bool X8>
+int bwd_elems(const BwdArgs& a, int threads, unsigned blocks, int stages, uint32_t y_slot, uint32_t x_slot,
+              cudaStream_t s) {
+  if (threads == 128 && a.N <= 1024) return launch_bwd_elems<T, X8, 128, 8>(a, blocks, stages, y_slot, x_slot, s);
+  if (threads == 128) return launch_bwd_elems<T, X8, 128, 16>(a, blocks, stages, y_slot, x_slot, s);
+  if (threads == 256) return launch_bwd_elems<T, X8, 256, 16>(a, blocks, stages, y_slot, x_slot, s);
+  return launch_bwd_elems<T, X8, 512, 16>(a, blocks, stages, y_slot, x_slot, s);
+}
+
 // Rows of whole 16-byte vectors whose stages fit shared memory run on the ring kernel; others of up to 8192
 // elements element by element in registers; longer ones (and a checkpoint of another 16- or 32-bit
 // type than dY's) in two passes.
@@ -989,10 +1187,12 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
                     aligned(a.dY, a.ldy * es, a.M, 16) && aligned(a.X, a.ldx * xe, a.M, 16) &&
                     aligned(a.dX, a.lddx * es, a.M, 16) && (!a.dR || aligned(a.dR, a.ldr * es, a.M, 16)) &&
                     ring_shape((uint32_t)(a.N * ((a.dR ? 2 : 1) * es + xe)), ctas, &ctas, &stages);
-  const bool elems = !ring && (x8 || same) && a.N <= 8192;
-  const int ethreads = (int)((a.N + 255) / 256 * 32);
-  if (elems) ctas = std::max(1, 1024 / ethreads);
-  const unsigned blocks = ring || elems ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas)
+  const uint32_t y_slot = ((uint32_t)(a.N * es) + 30u) & ~15u, x_slot = ((uint32_t)(a.N * xe) + 30u) & ~15u;
+  const int ethreads = a.N <= 2048 ? 128 : a.N <= 4096 ? 256 : 512;  // of the kernel for any alignment
+  int ectas = 512 / ethreads, estages = 0;
+  const bool elems = !ring && (x8 || same) && a.N >= 16 && a.N <= 8192 &&
+                     ring_shape((a.dR ? 2 : 1) * y_slot + x_slot, ectas, &ectas, &estages);
+  const unsigned blocks = ring || elems ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * (ring ? ctas : ectas))
                                         : row_blocks(a.M, sms);
   Workspace ws(s);
   int rc = B2G_OK;
@@ -1002,11 +1202,8 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
     a.part = static_cast<float*>(ws.get());
   }
   if (elems) {
-    if (x8)
-      rmsnorm_bwd_elems_kernel<T, true, 8><<<blocks, ethreads, 0, s>>>(a);
-    else
-      rmsnorm_bwd_elems_kernel<T, false, 8><<<blocks, ethreads, 0, s>>>(a);
-    rc = launched("rmsnorm_bwd_elems_kernel");
+    rc = x8 ? bwd_elems<T, true>(a, ethreads, blocks, estages, y_slot, x_slot, s)
+            : bwd_elems<T, false>(a, ethreads, blocks, estages, y_slot, x_slot, s);
   } else if (!ring) {
     rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
     rc = launched("rmsnorm_bwd_kernel");

@@ -158,52 +158,62 @@ __device__ __forceinline__ uint32_t to_q8(float t, int q_dtype) {
   return (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
 }
 
-// N values v of a row as 8-bit bytes (zeros for a bad row).
+// N values v of a row as 8-bit values, one in the low byte of each word (zeros for a bad row).
+template <int N>
+__device__ __forceinline__ void round_q8(const float (&v)[N], const RowQuant& r, int q_dtype, bool bad,
+                                         uint32_t (&o)[N]) {
+  static_assert(N % 2 == 0, "pairs");
+  const F2 mul = f2(r.mul, r.mul), rcp = f2(r.rcp, r.rcp), nden = f2(-r.den, -r.den);
+  F2 t[N / 2];
+  if (r.den == 0.0f) {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) t[j] = f2_mul(f2_mul(f2(v[2 * j], v[2 * j + 1]), mul), rcp);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {  // quotient(), two at a time
+      const F2 a = f2_mul(f2(v[2 * j], v[2 * j + 1]), mul);
+      const F2 q = f2_mul(a, rcp);
+      t[j] = f2_fma(f2_fma(q, nden, a), rcp, q);
+    }
+  }
+  if (q_dtype == B2G_DTYPE_I8) {
+    // 1.5 * 2^23 added: the sum's unit is 1, so the addition rounds t to an integer (to nearest
+    // even) and leaves its two's complement in the low byte
+    const F2 magic = f2(12582912.0f, 12582912.0f);
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      float a, b;
+      f2_get(f2_add(t[j], magic), a, b);
+      o[2 * j] = __float_as_uint(a);
+      o[2 * j + 1] = __float_as_uint(b);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      float a, b;
+      f2_get(t[j], a, b);
+      o[2 * j] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+      o[2 * j + 1] = o[2 * j] >> 8;
+    }
+  }
+  if (bad) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = 0;
+  }
+}
+
+// The same as packed bytes.
 template <int N>
 __device__ __forceinline__ void pack_q8(const float (&v)[N], const RowQuant& r, int q_dtype, bool bad,
                                         uint8_t (&o)[N]) {
   if constexpr (N % 4 == 0) {
+    uint32_t b[N];
+    round_q8<N>(v, r, q_dtype, bad, b);
     uint32_t* w = reinterpret_cast<uint32_t*>(o);
-    const F2 mul = f2(r.mul, r.mul), rcp = f2(r.rcp, r.rcp), nden = f2(-r.den, -r.den);
-    F2 t[N / 2];
-    if (r.den == 0.0f) {
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) t[j] = f2_mul(f2_mul(f2(v[2 * j], v[2 * j + 1]), mul), rcp);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N / 2; ++j) {  // quotient(), two at a time
-        const F2 a = f2_mul(f2(v[2 * j], v[2 * j + 1]), mul);
-        const F2 q = f2_mul(a, rcp);
-        t[j] = f2_fma(f2_fma(q, nden, a), rcp, q);
-      }
-    }
-    if (q_dtype == B2G_DTYPE_I8) {
-      // 1.5 * 2^23 added: the sum's unit is 1, so the addition rounds t to an integer (to nearest
-      // even) and leaves its two's complement in the low byte
-      const F2 magic = f2(12582912.0f, 12582912.0f);
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j) {
-        float a, b, c, d;
-        f2_get(f2_add(t[2 * j], magic), a, b);
-        f2_get(f2_add(t[2 * j + 1], magic), c, d);
-        w[j] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
-                           __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j) {
-        float a, b, c, d;
-        f2_get(t[2 * j], a, b);
-        f2_get(t[2 * j + 1], c, d);
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-        w[j] = lo | hi << 16;
-      }
-    }
-    if (bad) {
-#pragma unroll
-      for (int j = 0; j < N / 4; ++j) w[j] = 0;
-    }
+    for (int j = 0; j < N / 4; ++j)
+      w[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040),
+                         __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) o[j] = bad ? 0 : (uint8_t)to_q8(quotient(v[j], r), q_dtype);

@@ -202,7 +202,7 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, float* buf
 // Per row: sum of squares and largest |h * w| (|x| without the norm).  The largest |y| is rstd
 // times that, so one reduction serves both; rstd cancels from the 8-bit values (row_quant).
 template <typename T, bool NORM, int VEC, int V, int LANES, bool AHEAD>
-__global__ void __launch_bounds__(LANES ? 128 : AHEAD && VEC > 1 ? 256 : 1024, LANES ? 4 : AHEAD && VEC > 1 ? 2 : 1)
+__global__ void __launch_bounds__(LANES ? 128 : AHEAD ? 256 : 1024, LANES ? 7 : AHEAD ? 2 : 1)
     rows_to_q8_kernel(const NormArgs a) {
   __shared__ float buf[128];
   constexpr int PER = LANES ? 128 / LANES : 1;  // rows a block holds at once
@@ -1069,8 +1069,8 @@ bool launch_ring_elems(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   return true;
 }
 
-// Vectors of 16 bytes where every address and pitch allows, else single elements.  Rows of up to 128
-// vectors: four vectors a lane, several rows a warp; longer ones: a ring, or with few rows (latency
+// Vectors of 16 bytes where every address and pitch allows, else single elements.  Rows of up to 64
+// vectors: two vectors a lane, several rows a warp; longer ones: a ring, or with few rows (latency
 // counts then) one block a row with its loads in registers.
 template <typename T, bool NORM>
 int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
@@ -1081,12 +1081,13 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
                    (!a.H || aligned(a.H, a.ldh * es, a.M, 16)) && aligned(a.Q, a.ldq, a.M, VEC);
   if (vec) {
     const int64_t nv = a.N / VEC;
-    if (nv <= 16) return launch_rows<T, NORM, VEC, 4, 4>(a, 0, sms, s);
-    if (nv <= 32) return launch_rows<T, NORM, VEC, 4, 8>(a, 0, sms, s);
-    if (nv <= 64) return launch_rows<T, NORM, VEC, 4, 16>(a, 0, sms, s);
-    if (nv <= 128) return launch_rows<T, NORM, VEC, 4, 32>(a, 0, sms, s);
+    if (nv <= 8) return launch_rows<T, NORM, VEC, 2, 4>(a, 0, sms, s);
+    if (nv <= 16) return launch_rows<T, NORM, VEC, 2, 8>(a, 0, sms, s);
+    if (nv <= 32) return launch_rows<T, NORM, VEC, 2, 16>(a, 0, sms, s);
+    if (nv <= 64) return launch_rows<T, NORM, VEC, 2, 32>(a, 0, sms, s);
     int rc = B2G_OK;
-    if (nv <= 256 ? launch_ring<T, NORM, 2, 128, NORM ? 7 : 8>(a, sms, s, &rc)
+    if (nv <= 128 ? launch_ring<T, NORM, 2, 64, 14>(a, sms, s, &rc)
+        : nv <= 256 ? launch_ring<T, NORM, 2, 128, NORM ? 7 : 8>(a, sms, s, &rc)
         : nv <= 512 ? launch_ring<T, NORM, 4, 128, NORM ? 4 : 7>(a, sms, s, &rc)
         : nv <= 1024 ? launch_ring<T, NORM, 4, 256, NORM ? 2 : 4>(a, sms, s, &rc)
         : nv <= 2048 ? launch_ring<T, NORM, 8, 256, 2>(a, sms, s, &rc)

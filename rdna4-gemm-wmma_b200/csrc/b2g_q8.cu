@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 
 #include "../../include/b2g_gemm.h"
@@ -12,6 +13,7 @@
 #include "host.h"
 #include "plan.h"
 #include "q8.cuh"
+#include "skinny_sm100.cuh"
 
 namespace b2g {
 
@@ -102,6 +104,8 @@ unsigned tile_blocks(int64_t rows, int64_t cols, int sms) {
 }
 
 // ------------------------------------------------------------------ few tokens
+constexpr int kFewSteps = 4;  // 64-byte steps of K in a warp's turn
+
 // D (16 x 8, 32-bit) += A (16 x 32 bytes) . B (32 bytes x 8): int8 into int32, or e4m3 into fp32.
 template <bool I8>
 __device__ __forceinline__ void mma_16x8x32(uint32_t (&d)[4], const uint32_t a0, const uint32_t a1,
@@ -121,46 +125,43 @@ __device__ __forceinline__ void mma_16x8x32(uint32_t (&d)[4], const uint32_t a0,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Products of a few tokens are bound by the weights' bytes: N * K of them, each used once a token.  So
-// the weights go from memory straight into the registers of warp-level MMAs, as their 16-row side
-// (the tokens are its 8 columns), with no shared memory, tile pipeline or split-K workspace between.
-// The order of K inside a product does not matter, so a lane's fragments are whole 16-byte pieces:
-// lane (g, t) of a warp takes bytes [16 t, 16 t + 16) of each 64-byte step of weight rows g and
-// g + 8 and of token g, and feeds two MMAs from them.
+// Few tokens and few weights: latency counts, so the weights go from memory straight into the registers of
+// warp-level MMAs, as their 16-row side (the tokens are its 8 columns), with no pipeline to fill and
+// no tensor memory between.  The order of K inside a product does not matter, so a lane's fragments
+// are whole 16-byte pieces: lane (g, t) of a warp takes bytes [16 t, 16 t + 16) of each 64-byte step
+// of weight rows g and g + 8 and of token g, and feeds two MMAs from them.
 //
-// A block has MT * 16 weight rows; its warps take K in turns of U steps and add their sums through
-// shared memory, in warp order.  The next turn's weights are loaded before this turn's products.
-template <bool I8, int MT, int NT, int U>
+// A block has 16 weight rows; its warps take K in turns of U steps and add their sums through shared
+// memory, in warp order.  The next turn's weights are loaded before this turn's products.
+template <bool I8, int NT>
 __global__ void __launch_bounds__(512, 1)
     gemm_q8_few_kernel(const int8_t* __restrict__ A, const int8_t* __restrict__ B, void* __restrict__ C,
                        int M, int64_t N, int K, int64_t lda, int64_t ldb, int64_t ldc,
                        const float* __restrict__ a_scale, const float* __restrict__ b_scale,
                        const float* __restrict__ bias, int c_dtype) {
-  extern __shared__ uint32_t part[];  // [warps][MT * 16][NT * 8 + 1]
-  constexpr int COLS = NT * 8, PITCH = COLS + 1;
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  extern __shared__ uint32_t part[];  // [warps][16][NT * 8 + 1]
+  constexpr int U = kFewSteps, PITCH = NT * 8 + 1;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int64_t n0 = (int64_t)blockIdx.x * (MT * 16);
-  const int8_t* w[MT][2];  // rows past N read the last one; their sums are not stored
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int8_t* w[2];  // rows past N read the last one; their sums are not stored
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) w[i][h] = B + min(n0 + i * 16 + h * 8 + g, N - 1) * ldb + t * 16;
+  for (int h = 0; h < 2; ++h) w[h] = B + min(n0 + h * 8 + g, N - 1) * ldb + t * 16;
   const int8_t* x[NT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) x[j] = A + (int64_t)min(j * 8 + g, M - 1) * lda + t * 16;
-  uint32_t acc[MT][NT][4] = {};
-  uint4 cur[U][MT][2], nxt[U][MT][2];
+  uint32_t acc[NT][4] = {};
+  uint4 cur[U][2], nxt[U][2];
   const int step = warps * U * 64;
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  auto fetch = [&](int k, uint4 (&d)[U][MT][2]) {
+  auto fetch = [&](int k, uint4 (&d)[U][2]) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          d[u][i][h] = k + u * 64 + t * 16 < K ? __ldcs(reinterpret_cast<const uint4*>(w[i][h] + k + u * 64)) : zero;
+      for (int h = 0; h < 2; ++h)
+        d[u][h] = k + u * 64 + t * 16 < K ? __ldcs(reinterpret_cast<const uint4*>(w[h] + k + u * 64)) : zero;
   };
   int k = warp * U * 64;
   if (k < K) fetch(k, cur);
@@ -172,46 +173,39 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const uint4 b = in ? __ldg(reinterpret_cast<const uint4*>(x[j] + k + u * 64)) : zero;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint4 p = cur[u][i][0], q = cur[u][i][1];
-          mma_16x8x32<I8>(acc[i][j], p.x, q.x, p.y, q.y, b.x, b.y);
-          mma_16x8x32<I8>(acc[i][j], p.z, q.z, p.w, q.w, b.z, b.w);
-        }
+        const uint4 p = cur[u][0], q = cur[u][1];
+        mma_16x8x32<I8>(acc[j], p.x, q.x, p.y, q.y, b.x, b.y);
+        mma_16x8x32<I8>(acc[j], p.z, q.z, p.w, q.w, b.z, b.w);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) cur[u][i][h] = nxt[u][i][h];
+      for (int h = 0; h < 2; ++h) cur[u][h] = nxt[u][h];
   }
-  // row g (+ 8) of the weights, tokens 2 t and 2 t + 1
+  // rows g and g + 8 of the weights, tokens 2 t and 2 t + 1
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      uint32_t* p = part + (warp * MT * 16 + i * 16 + g) * PITCH + j * 8 + 2 * t;
-      p[0] = acc[i][j][0];
-      p[1] = acc[i][j][1];
-      p[8 * PITCH] = acc[i][j][2];
-      p[8 * PITCH + 1] = acc[i][j][3];
-    }
+  for (int j = 0; j < NT; ++j) {
+    uint32_t* p = part + (warp * 16 + g) * PITCH + j * 8 + 2 * t;
+    p[0] = acc[j][0];
+    p[1] = acc[j][1];
+    p[8 * PITCH] = acc[j][2];
+    p[8 * PITCH + 1] = acc[j][3];
+  }
   __syncthreads();
-  for (int o = threadIdx.x; o < MT * 16 * M; o += blockDim.x) {
-    const int row = o % (MT * 16), m = o / (MT * 16);
+  for (int o = threadIdx.x; o < 16 * M; o += blockDim.x) {
+    const int row = o % 16, m = o / 16;
     const int64_t n = n0 + row;
     if (n >= N) continue;
     const uint32_t* p = part + row * PITCH + m;
     float v;
     if constexpr (I8) {
       int s = 0;
-      for (int i = 0; i < warps; ++i) s += (int)p[i * MT * 16 * PITCH];
+      for (int i = 0; i < warps; ++i) s += (int)p[i * 16 * PITCH];
       v = (float)s;
     } else {
       v = 0.0f;
-      for (int i = 0; i < warps; ++i) v += __uint_as_float(p[i * MT * 16 * PITCH]);
+      for (int i = 0; i < warps; ++i) v += __uint_as_float(p[i * 16 * PITCH]);
     }
     if (a_scale) v *= a_scale[m];
     if (b_scale) v *= b_scale[n];
@@ -220,6 +214,7 @@ __global__ void __launch_bounds__(512, 1)
   }
 }
 
+// A product whose weights are read once for all tokens.
 struct FewArgs {
   const void *A, *B;
   void* C;
@@ -228,27 +223,42 @@ struct FewArgs {
   int c_dtype;
 };
 
-// Up to this many tokens take the few-token kernel.  Measured at N = K = 8192, int8 (us a call): 1 token
-// 15.0 against the tensor-core tiles' 22.7, 8 tokens 15.3 against 22.6, 16 tokens 18.7 against 21.6,
-// 32 tokens 24.8 against 21.6; 28672 x 8192, 1 token: 43.5 against 62.8.
-constexpr int64_t kFewTokens = 16;
+// gemm_q8_few_kernel takes up to 16 tokens where the weights are up to 12 Mi bytes (K a multiple of 16), as
+// measured against gemm_q8_skinny_kernel (us a call, back to back in a graph, int8): 1 token, N x K =
+// 1024 x 4096 2.7 against 5.2, 8192 x 1024 2.5 against 5.1, 4096 x 4096 6.0 against 6.2, 8192 x 8192
+// 15.5 against 13.8; 16 tokens, 2048 x 2048 3.3 against 6.7, 4096 x 4096 7.6 against 7.1.
+bool is_few(const FewArgs& a) { return a.M <= 16 && a.K % 16 == 0 && a.N * a.K <= (int64_t)12 << 20; }
 
 // Warps of a block: as many (4 to 16) as give the GPU about 16 an SM, each with a whole turn of K.
-template <bool I8, int MT, int NT, int U>
+template <bool I8, int NT>
 int launch_few(const FewArgs& a, int sms, cudaStream_t s) {
-  const int64_t blocks = (a.N + MT * 16 - 1) / (MT * 16);
+  const int64_t blocks = (a.N + 15) / 16;
   int warps = 4;
-  while (warps < 16 && warps * 2 * MT * 16 * (NT * 8 + 1) * 4 <= 48 * 1024 && blocks * warps < (int64_t)sms * 16 && a.K >= (int64_t)warps * 2 * U * 64) warps *= 2;
-  const uint32_t smem = (uint32_t)(warps * MT * 16 * (NT * 8 + 1)) * 4;
-  gemm_q8_few_kernel<I8, MT, NT, U><<<(unsigned)blocks, warps * 32, smem, s>>>(
-      static_cast<const int8_t*>(a.A), static_cast<const int8_t*>(a.B), a.C, (int)a.M, a.N, (int)a.K, a.lda,
-      a.ldb, a.ldc, a.a_scale, a.b_scale, a.bias, a.c_dtype);
-  return launched("gemm_q8_few_kernel");
+  while (warps < 16 && blocks * warps < (int64_t)sms * 16 && a.K >= (int64_t)warps * 2 * kFewSteps * 64) warps *= 2;
+  const uint32_t smem = (uint32_t)(warps * 16 * (NT * 8 + 1)) * 4;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+  cfg.blockDim = dim3((unsigned)warps * 32, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  if (launch_options().pdl) {
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, gemm_q8_few_kernel<I8, NT>, static_cast<const int8_t*>(a.A), static_cast<const int8_t*>(a.B), a.C,
+      (int)a.M, a.N, (int)a.K, a.lda, a.ldb, a.ldc, a.a_scale, a.b_scale, a.bias, a.c_dtype);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_q8_few_kernel launch");
+  count_launch();
+  return B2G_OK;
 }
 
 template <bool I8>
 int few_tokens(const FewArgs& a, int sms, cudaStream_t s) {
-  return a.M <= 8 ? launch_few<I8, 1, 1, 4>(a, sms, s) : launch_few<I8, 1, 2, 4>(a, sms, s);
+  return a.M <= 8 ? launch_few<I8, 1>(a, sms, s) : launch_few<I8, 2>(a, sms, s);
 }
 
 // ------------------------------------------------------------------ aligned copies
@@ -389,8 +399,8 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   const int esz = g.q == Q_WGRAD ? 2 : 1, kb = kRowBytes / esz;
   const int64_t nmt = (g.rows + kBM - 1) / kBM, kit = (g.k + kb - 1) / kb;
   const TileChoice tc = choose_tiles(nmt, g.cols, kit, sms, opt.cta_group, opt.tile_n, 128);
-  static const Variant variants[4] = {make_variant<1, 128, 4>(), make_variant<1, 256, 4>(),
-                                      make_variant<2, 256, 4>(), make_variant<2, 512, 8>()};
+  static const Variant variants[4] = {make_variant<1, 128, 8>(), make_variant<1, 256, 8>(),
+                                      make_variant<2, 256, 8>(), make_variant<2, 512, 8>()};
   const int v = tc.cg == 1 ? (tc.bn == 128 ? 0 : 1) : (tc.bn == 256 ? 2 : 3);
   const Variant& var = variants[v];
   const int cg = var.cg, bn = var.bn;
@@ -542,6 +552,87 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   return B2G_OK;
 }
 
+// ------------------------------------------------------------------ decoding batches
+// Up to this many tokens run on gemm_q8_skinny_kernel.  Measured against the tiles of larger batches (us a
+// call, back to back in a graph, int8, N = K = 8192): 1 token 13.8 against 24.0, 32 tokens 15.7
+// against 23.9, 64 tokens 17.7 against 23.9, 128 tokens 21.7 against 24.3; 10240 x 8192, 43 tokens
+// 19.7 against 27.3; 28672 x 8192, 128 tokens 48.7 against 53.0.
+constexpr int64_t kSkinnyTokens = 128;
+
+template <bool I8, int NT>
+int launch_skinny(const FewArgs& a, int sms, cudaStream_t s) {
+  using C = SkinnyCfg<NT>;
+  const LaunchOptions opt = launch_options();
+  auto fn = gemm_q8_skinny_kernel<I8, NT>;
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready.load() >> dev & 1)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM_BYTES);
+    if (e == cudaSuccess) ready |= 1ull << dev;
+  }
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(smem)");
+  CUtensorMap tmW, tmX;
+  auto encode = [&](CUtensorMap* m, const void* base, int64_t rows, int64_t ld, cuuint32_t box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)a.K, 1, (cuuint64_t)rows};
+    const cuuint64_t p = (cuuint64_t)(rows == 1 ? (ld + 15) / 16 * 16 : ld);
+    const cuuint64_t st[2] = {(cuuint64_t)((a.K + 15) / 16 * 16), p};
+    const cuuint32_t box[3] = {(cuuint32_t)kRowBytes, 1, box_rows};
+    return encode_cached(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, st, box,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+  };
+  CUresult r = encode(&tmW, a.B, a.N, a.ldb, 128);
+  if (r == CUDA_SUCCESS) r = encode(&tmX, a.A, a.M, a.lda, NT);
+  if (r != CUDA_SUCCESS) return fail(B2G_ERR_CUDA, "tensor map of a decoding batch: CUresult %d", (int)r);
+  SkinnyParams p{};
+  p.M = (int)a.M;
+  p.N = a.N;
+  p.k_iters = (int)((a.K + kRowBytes - 1) / kRowBytes);
+  const int tiles = (int)((a.N + 127) / 128);
+  // splits: up to two CTAs an SM, each split keeping 8 K blocks
+  int splits = opt.split_k > 0 ? std::min(opt.split_k, 8)
+                               : std::max(1, std::min({8, 2 * sms / tiles, p.k_iters / 8}));
+  splits = std::min(splits, p.k_iters);
+  p.k_per_split = (p.k_iters + splits - 1) / splits;
+  p.splits = (p.k_iters + p.k_per_split - 1) / p.k_per_split;  // no empty split
+  p.C = a.C;
+  p.ldc = a.ldc;
+  p.c_dtype = a.c_dtype;
+  p.a_scale = a.a_scale;
+  p.b_scale = a.b_scale;
+  p.bias = a.bias;
+  p.timeout_ns = (unsigned long long)opt.timeout_ns;
+  p.fault_flags = opt.fault_flags;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3((unsigned)(tiles * p.splits), 1, 1);
+  cfg.blockDim = dim3(C::THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.numAttrs = 1;
+  if (opt.pdl) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  e = cudaLaunchKernelEx(&cfg, fn, tmW, tmX, p);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_q8_skinny_kernel launch");
+  count_launch();
+  set_path(B2G_PATH_TC_1CTA);
+  return B2G_OK;
+}
+
+template <bool I8>
+int skinny(const FewArgs& a, int sms, cudaStream_t s) {
+  if (a.M <= 32) return launch_skinny<I8, 32>(a, sms, s);
+  if (a.M <= 64) return launch_skinny<I8, 64>(a, sms, s);
+  return launch_skinny<I8, 128>(a, sms, s);
+}
+
 // Whether a product can run on the tensor-core kernel: an sm_100 device, and extents that its
 // 32-bit coordinates hold.
 bool tensor_ok(int cc, int64_t rows, int64_t cols, int64_t k) {
@@ -590,12 +681,13 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
     rc = aligned_rows(&A, &lda, M, K, sms, wa, s);
     if (rc == B2G_OK) rc = aligned_rows(&B, &ldb, N, K, sms, wb, s);
     if (rc != B2G_OK) return rc;
-    if (M <= kFewTokens && K % 16 == 0 && (N + 15) / 16 <= INT32_MAX) {
-      const FewArgs f = {A, B, C, M, N, K, lda, ldb, ldc, a_scale, b_scale, bias, c_dtype};
+    const FewArgs f = {A, B, C, M, N, K, lda, ldb, ldc, a_scale, b_scale, bias, c_dtype};
+    if (is_few(f)) {
       rc = dtype == B2G_DTYPE_I8 ? few_tokens<true>(f, sms, s) : few_tokens<false>(f, sms, s);
       if (rc == B2G_OK) set_path(B2G_PATH_FEW);
       return rc;
     }
+    if (M <= kSkinnyTokens) return dtype == B2G_DTYPE_I8 ? skinny<true>(f, sms, s) : skinny<false>(f, sms, s);
     const Product g = {dtype == B2G_DTYPE_I8 ? Q_I8 : Q_FP8, A, B, C, M, N, K, lda, ldb, ldc, 0,
                        c_type_of(c_dtype), false, a_scale, b_scale, bias};
     return launch_product(g, dev, sms, s);

@@ -143,14 +143,15 @@ constexpr uint32_t kSmemLimit = 232448;  // max dynamic shared memory per CTA on
 // lanes 0-63 and columns [128, 256) in lanes 64-127 (the "2x2" data-path layout of M = 128
 // with cta_group::2).  It halves the partial tile a CTA holds when K is split, which is what
 // bounds the split-K reduction of skinny problems.
-// EW: epilogue warps, 4, or 8 for the 256 x 512 pair tile.  With one accumulator filling TMEM
+// EW: epilogue warps, 4, or 8 for the 256 x 512 pair tile and for every tile of the 8-bit layer's
+// instances (whose small problems have one tile a CTA, so that its epilogue is not overlapped).  With one accumulator filling TMEM
 // the MMA of the next tile waits for the epilogue to hand back each N-half.  Eight warps pull a
 // whole N-half into registers (each warp 32 rows x 128 columns) and hand it back before they
 // store it, instead of after storing 7/8 of it.
 template <int CG, int BN, int BMC = kBM, int EW = 4>
 struct Cfg {
   static_assert(CG == 1 || CG == 2, "CTA group");
-  static_assert(EW == 4 || (EW == 8 && CG == 2 && BN == 512 && BMC == kBM), "epilogue warps");
+  static_assert(EW == 4 || (EW == 8 && BMC == kBM), "epilogue warps");
   static_assert(BN == 256 || BN == 512 || (BN == 128 && CG == 1), "tile width");
   static_assert(BMC == kBM || (BMC == 64 && CG == 2 && BN == 256), "half-height pair tile");
   static constexpr int UN = BN < kUN ? BN : kUN;      // N of one UMMA instruction
@@ -519,8 +520,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
     const int q = warp & 3;  // TMEM lane quarter
     // EW = 8: warps 2-5 and 6-9 cover the four lane quarters twice; `part` picks the 128
     // columns of each N-half this warp handles.  EW = 4: one warp per quarter, every column.
-    const int part = (warp - 2) >> 2;
-    auto mine = [&](int ch) { return C::EPI_WARPS == 4 || ((ch >> 2) & 1) == part; };
+    const int part_id = (warp - 2) >> 2;
+    // (BN = 128: 64 of its columns)
+    constexpr int PART = C::CHUNKS < 8 ? C::CHUNKS / 2 : 4;  // consecutive chunks of one part
+    auto mine = [&](int ch) { return C::EPI_WARPS == 4 || ((ch / PART) & 1) == part_id; };
     const uint32_t cbuf = base + C::OFF_C + (uint32_t)(warp - 2) * (uint32_t)C::EPI_BUFS * kCBuf;
     // This warp's 32-row sub-box inside the CTA's BMC-row tile (flattened (a, b, i) order) and
     // its columns: BMC = 128, all BN columns of rows 32q..32q+31; BMC = 64 (folded
@@ -574,14 +577,21 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
           }
         }
       }
+      float row_scale = 1.0f;  // this lane's row
+      if constexpr (Q == Q_I8 || Q == Q_FP8) {
+        if (p.row_scale && rows_valid && ci + lane < p.i_size) row_scale = __ldg(p.row_scale + ci + lane);
+        // bring the tile's column scales and bias into L1 while its MMAs run (one 128-byte line a lane)
+        const int gc = tn * BN + 32 * lane;
+        if (lane < BN / 32 && gc < p.n_size) {
+          if (p.col_scale) ptx::prefetch_l1(p.col_scale + gc);
+          if (p.bias) ptx::prefetch_l1(p.bias + gc);
+        }
+      }
       const bool got = ptx::mbar_wait(tfull_bar(acc), aph, abort_flag, err, ERR_WAIT_TFULL, lim);
       if (!__all_sync(0xffffffffu, got)) break;
       ptx::tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)acc * C::ACC_COLS;
       const int n0 = tn * BN + col_off;
-      float row_scale = 1.0f;  // this lane's row
-      if constexpr (Q == Q_I8 || Q == Q_FP8)
-        if (p.row_scale && rows_valid && ci + lane < p.i_size) row_scale = __ldg(p.row_scale + ci + lane);
 
       // Stage chunk `ch` (32 columns of this warp's 32 rows) and TMA-store it.
       auto store_chunk = [&](const uint32_t (&v)[32], int ch) {
@@ -673,20 +683,23 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
               ptx::st_shared_b32(buf + 4u * (uint32_t)(lane * 32 + (j ^ lane)), w[j]);
             __syncwarp();
             const int nrows = min(32, p.i_size - ci), col = gcol + lane;
-            for (int r = 0; r < nrows; ++r) {
-              const float x = __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r))));
-              if (col < p.n_size) {
-                const long long at = (long long)(ci + r) * p.ldc + col;
-                if (p.c_type == 0) {
-                  float* c = static_cast<float*>(p.c_direct) + at;
-                  *c = p.accumulate ? *c + x : x;
-                } else if (p.c_type == 1) {
-                  static_cast<__half*>(p.c_direct)[at] = __float2half_rn(x);
-                } else {
-                  static_cast<__nv_bfloat16*>(p.c_direct)[at] = __float2bfloat16_rn(x);
-                }
-              }
-            }
+            auto rows_out = [&](auto* c, auto store) {
+              c += (long long)ci * p.ldc + col;
+#pragma unroll 8
+              for (int r = 0; r < 32; ++r)
+                if (r < nrows && col < p.n_size)
+                  store(c + (long long)r * p.ldc,
+                        __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r)))));
+            };
+            if (p.c_type == 1)
+              rows_out(static_cast<__half*>(p.c_direct), [](__half* c, float x) { *c = __float2half_rn(x); });
+            else if (p.c_type == 2)
+              rows_out(static_cast<__nv_bfloat16*>(p.c_direct),
+                       [](__nv_bfloat16* c, float x) { *c = __float2bfloat16_rn(x); });
+            else if (p.accumulate)
+              rows_out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c += x; });
+            else
+              rows_out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c = x; });
             __syncwarp();
             return;
           }
@@ -789,16 +802,20 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         };
         const uint32_t part = base + (uint32_t)(q * 8 * 32 + lane) * 16u;
         ptx::fence_proxy_async_smem();
-        // four chunks of TMEM loads in flight per wait (the wait is the cost here)
+        // four chunks of TMEM loads in flight per wait (the wait is the cost here); with eight
+        // epilogue warps, this warp's part of the tile
         static_assert(C::CHUNKS % 4 == 0, "fix-up copies four chunks per TMEM wait");
+        constexpr int FLY = C::EPI_WARPS == 4 ? 4 : PART;
+        const int ch_lo = C::EPI_WARPS == 4 ? 0 : part_id * PART;
+        const int ch_hi = C::EPI_WARPS == 4 ? C::CHUNKS : ch_lo + PART;
 #pragma unroll 1
-        for (int ch0 = 0; ch0 < C::CHUNKS; ch0 += 4) {
-          uint32_t w4[4][32];
+        for (int ch0 = ch_lo; ch0 < ch_hi; ch0 += FLY) {
+          uint32_t w4[FLY][32];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(tbase + 32u * (ch0 + c), w4[c]);
+          for (int c = 0; c < FLY; ++c) ptx::tmem_ld_32x32b_x32(tbase + 32u * (ch0 + c), w4[c]);
           ptx::tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < FLY; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               ptx::st_shared_v4(part + (uint32_t)(((ch0 + c) * 4 * 8 + j) * 32) * 16u,
@@ -819,23 +836,26 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         if (*ready_flag) {
 #pragma unroll 1
           for (int ch = sp; ch < C::CHUNKS; ch += ns) {
+            if (C::EPI_WARPS == 8 && (((ch - sp) / ns) & 1) != part_id) continue;  // alternate chunks
             float a[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) a[j] = 0.0f;
-            // Splits in order (deterministic sums), four splits' loads in flight at a time.
+            // Splits in order (deterministic sums), four splits' loads in flight at a time (two with
+            // eight epilogue warps, which have fewer registers each).
+            constexpr int SFLY = C::EPI_WARPS == 8 ? 2 : 4;
             const uint32_t off = part + (uint32_t)(ch * 4 * 8 * 32) * 16u;
 #pragma unroll 1
-            for (int r0 = 0; r0 < ns; r0 += 4) {
-              float4 x[4][8];
+            for (int r0 = 0; r0 < ns; r0 += SFLY) {
+              float4 x[SFLY][8];
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
+              for (int c = 0; c < SFLY; ++c) {
                 if (r0 + c >= ns) break;
                 const uint32_t src = ptx::mapa(off, split_cta(r0 + c));
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[c][j] = ptx::ld_shared_cluster_v4(src + (uint32_t)(j * 32) * 16u);
               }
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
+              for (int c = 0; c < SFLY; ++c) {
                 if (r0 + c >= ns) break;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -999,12 +1019,23 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         continue;
       }
 
+      if constexpr (C::EPI_WARPS == 8 && C::NH == 1) {
+        // this warp's part of the tile into registers, hand the accumulator back, then store
+        uint32_t v[PART][32];
+#pragma unroll
+        for (int c = 0; c < PART; ++c) ptx::tmem_ld_32x32b_x32(tbase + 32u * (part_id * PART + c), v[c]);
+        ptx::tmem_ld_wait();
+        release(acc);
+#pragma unroll
+        for (int c = 0; c < PART; ++c) store_chunk(v[c], part_id * PART + c);
+        continue;
+      }
       if constexpr (C::EPI_WARPS == 8) {
         // N-half h: this warp's four chunks (h*8 + part*4 + c) into registers, hand the half
         // back to the MMA warp as soon as all eight warps have loaded theirs, then store them.
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
-          const int ch0 = h * 8 + part * 4;
+          const int ch0 = h * 8 + part_id * 4;
           uint32_t v[4][32];
 #pragma unroll
           for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(tbase + 32u * (ch0 + c), v[c]);

@@ -135,6 +135,12 @@ __device__ __forceinline__ float4 ld_shared_cluster_v4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t ld_shared_cluster_b32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // Teardown variant: ignores the abort flag (the copies or MMAs being waited for finish
 // on their own) and is bounded by time only.
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err, int code,
@@ -321,6 +327,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 // into L2.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
+// A hint: the 128-byte line at `p` into L1 (a load whose value is not used: nothing waits for it).
+__device__ __forceinline__ void prefetch_l1(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
 }
 
 __device__ __forceinline__ void bulk_wait_all() {

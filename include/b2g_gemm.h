@@ -395,7 +395,7 @@ int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int64_t N, int
  * dY is M x N (dtype F16 or BF16), Q M x K (q_dtype) with its row scales, dW N x K of type
  * c_dtype: F32, or (accumulate == 0 only) F16 or BF16.  Q * scale is rounded to dY's type
  * (saturating): with power-of-two scales it is exact in BF16, and in F16 while it lies in
- * F16's range.  Products are exact in fp32 and summed in fp32; an fp32 dW sums at most 4096
+ * F16's range.  Products are exact in fp32 and summed in fp32; an fp32 dW sums at most 768
  * tokens in one tensor-core accumulator, and such partial sums in fp32.
  */
 int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, void* dW, int64_t M, int64_t N,

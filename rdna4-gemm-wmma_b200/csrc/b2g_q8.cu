@@ -335,6 +335,7 @@ struct Product {
   int c_type;             // 0 = fp32, 1 = fp16, 2 = bf16
   bool accumulate;
   const float *row_scale, *col_scale, *bias;
+  int part_blocks;        // Q_WGRAD: K blocks that one accumulator may sum (0: any number)
 };
 
 using KernFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GemmParams);
@@ -342,23 +343,34 @@ using KernFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap,
 struct Variant {
   int cg, bn, threads;
   uint32_t smem;
-  KernFn fn[3];  // Q_I8, Q_FP8, Q_WGRAD
+  KernFn fn[4];  // Q_I8, Q_FP8, Q_WGRAD, Q_WGRAD_SUM (null for the 512-column tile)
 };
 
 template <int CG, int BN, int EW>
 Variant make_variant() {
   using C = Cfg<CG, BN, kBM, EW>;
+  KernFn sum = nullptr;
+  if constexpr (BN <= 256) sum = gemm_tc_kernel<CG, BN, false, false, 2, kBM, EW, false, Q_WGRAD_SUM>;
   return {CG, BN, C::THREADS, C::SMEM_BYTES,
           {gemm_tc_kernel<CG, BN, true, false, 1, kBM, EW, false, Q_I8>,
            gemm_tc_kernel<CG, BN, true, false, 1, kBM, EW, false, Q_FP8>,
-           gemm_tc_kernel<CG, BN, false, false, 2, kBM, EW, false, Q_WGRAD>}};
+           gemm_tc_kernel<CG, BN, false, false, 2, kBM, EW, false, Q_WGRAD>, sum}};
+}
+
+const Variant* variants() {
+  static const Variant v[4] = {make_variant<1, 128, 8>(), make_variant<1, 256, 8>(), make_variant<2, 256, 8>(),
+                               make_variant<2, 512, 8>()};
+  return v;
+}
+int variant_of(const TileChoice& tc) {
+  return tc.cg == 1 ? (tc.bn == 128 ? 0 : 1) : (tc.bn == 256 ? 2 : 3);
 }
 
 // Clusters of `size` CTAs of a kernel resident at once on the current device, asked once per
 // (device, variant, Q, size); also raises the kernel's shared-memory limit the first time.
 int resident_clusters(int dev, int v, const Variant& var, int q, int size, int sms, int* out) {
   static std::mutex mu;
-  static int known[64][4][3][9] = {};
+  static int known[64][4][4][9] = {};
   if (dev < 0 || dev >= 64) return fail(B2G_ERR_UNSUPPORTED, "device ordinal %d out of range", dev);
   std::lock_guard<std::mutex> lk(mu);
   int& n = known[dev][v][q - 1][size];
@@ -394,15 +406,32 @@ int resident_clusters(int dev, int v, const Variant& var, int q, int size, int s
 
 bool al16(uintptr_t x) { return (x & 15) == 0; }
 
+// The plain product's tiles; where K goes in parts, at most 256 columns (two accumulators in TMEM).
+TileChoice tiles_of(int64_t nmt, int64_t cols, int64_t kit, int sms, const LaunchOptions& opt, int part_blocks) {
+  const TileChoice tc = choose_tiles(nmt, cols, kit, sms, opt.cta_group, opt.tile_n, 128);
+  if (part_blocks > 0 && kit > part_blocks && tc.bn == 512) return {tc.cg, 256, false};
+  return tc;
+}
+
+// K splits of every tile that launch_product plans for a product in parts (1: none).
+int product_splits(int64_t rows, int64_t cols, int64_t k, int q, int part_blocks, int dev, int sms, int* rc) {
+  const LaunchOptions opt = launch_options();
+  const int64_t kb = q == Q_WGRAD ? 64 : 128, nmt = (rows + kBM - 1) / kBM, kit = (k + kb - 1) / kb;
+  const TileChoice tc = tiles_of(nmt, cols, kit, sms, opt, part_blocks);
+  int cap = 0;
+  *rc = resident_clusters(dev, variant_of(tc), variants()[variant_of(tc)], q, tc.cg, sms, &cap);
+  if (*rc != B2G_OK) return 1;
+  const int tiles = (int)((nmt + tc.cg - 1) / tc.cg * ((cols + tc.bn - 1) / tc.bn));
+  return choose_splits(tiles, (int)kit, cap, tc.cg, opt.split_k, false).k_splits;
+}
+
 int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   const LaunchOptions opt = launch_options();
   const int esz = g.q == Q_WGRAD ? 2 : 1, kb = kRowBytes / esz;
   const int64_t nmt = (g.rows + kBM - 1) / kBM, kit = (g.k + kb - 1) / kb;
-  const TileChoice tc = choose_tiles(nmt, g.cols, kit, sms, opt.cta_group, opt.tile_n, 128);
-  static const Variant variants[4] = {make_variant<1, 128, 8>(), make_variant<1, 256, 8>(),
-                                      make_variant<2, 256, 8>(), make_variant<2, 512, 8>()};
-  const int v = tc.cg == 1 ? (tc.bn == 128 ? 0 : 1) : (tc.bn == 256 ? 2 : 3);
-  const Variant& var = variants[v];
+  const TileChoice tc = tiles_of(nmt, g.cols, kit, sms, opt, g.part_blocks);
+  const int v = variant_of(tc);
+  const Variant& var = variants()[v];
   const int cg = var.cg, bn = var.bn;
 
   // ---- tensor maps (dimensions of extent 1 get a stride that is never used)
@@ -495,12 +524,23 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   int group_cap = 0;
   int rc = resident_clusters(dev, v, var, g.q, cg, sms, &group_cap);
   if (rc != B2G_OK) return rc;
-  const SplitChoice sc = choose_splits(p.num_tiles, p.k_iters, group_cap, cg, opt.split_k, opt.tail_split);
+  // (a tail wave is split only where no tile is cut into parts)
+  const bool parts = g.part_blocks > 0 && p.k_iters > g.part_blocks;
+  const SplitChoice sc =
+      choose_splits(p.num_tiles, p.k_iters, group_cap, cg, opt.split_k, opt.tail_split && !parts);
   p.k_per_split = sc.k_per_split;
   p.k_splits = sc.k_splits;
   p.num_full = sc.num_full;
+  p.k_parts = 1;
+  const bool sum = g.part_blocks > 0 && p.k_splits == 1 && p.k_iters > g.part_blocks;
+  const int q = sum ? (int)Q_WGRAD_SUM : g.q;
+  if (sum) {
+    p.k_parts = (p.k_iters + g.part_blocks - 1) / g.part_blocks;
+    p.k_per_part = (p.k_iters + p.k_parts - 1) / p.k_parts;
+    p.k_parts = (p.k_iters + p.k_per_part - 1) / p.k_per_part;
+  }
   const int split_tiles = p.num_tiles - p.num_full;
-  p.num_units = p.num_full + split_tiles * p.k_splits;
+  p.num_units = sum ? p.num_tiles * p.k_parts : p.num_full + split_tiles * p.k_splits;
   if (cg == 1 && p.k_splits > 1 && p.k_splits <= 8 && p.num_full == 0 && opt.cluster_fixup &&
       !opt.serial_fixup) {
     int nclu = 0;
@@ -523,14 +563,15 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   }
   // parallel fix-up only when each CTA group holds at most one split unit (all of them then run
   // at the same time, so their mutual waits always end)
-  const int groups = p.cluster_fixup ? p.num_units : std::max(1, std::min(group_cap, p.num_units));
+  const int groups = p.cluster_fixup ? p.num_units
+                                     : std::max(1, std::min(group_cap, p.num_units / p.k_parts));
   p.fixup_parallel = p.k_splits > 1 && p.num_full % groups == 0 && p.num_units - p.num_full <= groups &&
                      !opt.serial_fixup;
 
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3((unsigned)(groups * cg), 1, 1);
-  cfg.blockDim = dim3((unsigned)var.threads, 1, 1);
+  cfg.blockDim = dim3((unsigned)(var.threads + 32 * (lead_warps(q) - 2)), 1, 1);
   cfg.dynamicSmemBytes = var.smem;
   cfg.stream = stream;
   cfg.attrs = attr;
@@ -545,7 +586,12 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, var.fn[g.q - 1], tmA, tmB, tmC, p);
+  if (sum) {  // raises the instance's shared-memory limit (its occupancy is the plain instance's)
+    int n = 0;
+    rc = resident_clusters(dev, v, var, q, cg, sms, &n);
+    if (rc != B2G_OK) return rc;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, var.fn[q - 1], tmA, tmB, tmC, p);
   if (e != cudaSuccess) return cuda_fail(e, "8-bit layer tcgen05 kernel launch");
   count_launch();
   set_path(cg == 1 ? B2G_PATH_TC_1CTA : B2G_PATH_TC_2CTA);
@@ -644,9 +690,11 @@ bool tensor_ok(int cc, int64_t rows, int64_t cols, int64_t k) {
 int c_type_of(int c_dtype) { return c_dtype == B2G_DTYPE_F32 ? 0 : c_dtype == B2G_DTYPE_F16 ? 1 : 2; }
 
 // Tokens that one tensor-core accumulator sums for an fp32 weight gradient.  The accumulator
-// truncates, so its error grows with the number of terms: against 64 bits, normal bf16 operands
-// gave 4.7e-7 (2-norm) at 2048 terms, 1.0e-6 at 8192 and 3.8e-6 at 28672.
-constexpr int64_t kMaxTokens = 4096;
+// truncates, so its error grows with the number of terms.  Against 64 bits (2-norm, int8 rows of
+// scales from 2^-6 to 2^1, fp32 library product 1.3e-7 to 5.8e-7): bf16 3.5e-7 over 512 tokens,
+// 9.1e-7 over 1024, 1.8e-6 over 2048; fp16 6.2e-7, 1.2e-6, 2.4e-6.  Parts cost speed where they
+// forbid the 512-column tile, whose operands need a quarter fewer L2 bytes.
+constexpr int64_t kMaxTokens = 768;
 
 }  // namespace
 }  // namespace b2g
@@ -689,7 +737,7 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
     }
     if (M <= kSkinnyTokens) return dtype == B2G_DTYPE_I8 ? skinny<true>(f, sms, s) : skinny<false>(f, sms, s);
     const Product g = {dtype == B2G_DTYPE_I8 ? Q_I8 : Q_FP8, A, B, C, M, N, K, lda, ldb, ldc, 0,
-                       c_type_of(c_dtype), false, a_scale, b_scale, bias};
+                       c_type_of(c_dtype), false, a_scale, b_scale, bias, 0};
     return launch_product(g, dev, sms, s);
   }
   const unsigned blocks = tile_blocks(M, N, sms);
@@ -736,14 +784,21 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
     int64_t pitch = ldy * 2;
     if (rc == B2G_OK) rc = aligned_rows(&dY, &pitch, M, N * 2, sms, wy, s);
     if (rc != B2G_OK) return rc;
-    // fp32: the tokens in equal parts of whole K blocks, each added to the last
-    const int64_t parts = c_dtype == B2G_DTYPE_F32 ? (M + kMaxTokens - 1) / kMaxTokens : 1;
-    const int64_t per = ((M + parts - 1) / parts + 63) / 64 * 64;
+    // fp32: whole tiles take their tokens in parts of kMaxTokens (launch_product); where K is split
+    // over CTAs, a launch has at most kMaxTokens a split, and the next one adds to it
+    const int part_blocks = c_dtype == B2G_DTYPE_F32 ? (int)(kMaxTokens / 64) : 0;
+    int64_t per = M;
+    if (part_blocks) {
+      const int splits = product_splits(N, K, M, Q_WGRAD, part_blocks, dev, sms, &rc);
+      if (rc != B2G_OK) return rc;
+      if (splits > 1) per = std::min(M, splits * kMaxTokens);
+    }
     for (int64_t m0 = 0; m0 < M && rc == B2G_OK; m0 += per) {
       const Product g = {Q_WGRAD, static_cast<const char*>(dY) + m0 * pitch,
                          static_cast<const char*>(wx.get()) + m0 * ldx * 2, dW, N, K,
                          std::min(per, M - m0), pitch / 2, ldx, ldw, dtype == B2G_DTYPE_F16 ? 0 : 1,
-                         c_type_of(c_dtype), accumulate != 0 || m0 > 0, nullptr, nullptr, nullptr};
+                         c_type_of(c_dtype), accumulate != 0 || m0 > 0, nullptr, nullptr, nullptr,
+                         part_blocks};
       rc = launch_product(g, dev, sms, s);
     }
     return rc;

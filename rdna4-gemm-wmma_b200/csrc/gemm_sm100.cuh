@@ -113,6 +113,10 @@ struct GemmParams {
   void* c_direct;          // non-null: C (row pitch ldc elements) is stored with ordinary stores,
   long long ldc;           // all of it (direct_all: a base or pitch that TMA does not take) or
   int direct_all;          // only chunks that pass the last column (N not whole 16-byte pieces)
+  // Q_WGRAD_SUM (no tile is split): K in k_parts parts of k_per_part blocks, each a unit of its own,
+  // one after the other on the same CTA group.
+  int k_parts;
+  int k_per_part;
 };
 
 // What an instance of the kernel computes beside the plain product.
@@ -121,6 +125,11 @@ enum : int {
   Q_I8 = 1,     // int8 operands, int32 accumulators, row and column scales
   Q_FP8 = 2,    // fp8 operands, row and column scales
   Q_WGRAD = 3,  // 16-bit operands, A stored with its rows contiguous ([k][m], as B is [k][n])
+  // The same with K in parts, whose accumulators the epilogue warps add up in fp32 registers while the
+  // next part's MMAs run, storing after the last: the tensor core's accumulator truncates, so sums
+  // of few terms each are more exact.  BN <= 256 (two accumulators in TMEM), eight epilogue warps,
+  // which form two warpgroups of their own and take over registers from the first one.
+  Q_WGRAD_SUM = 4,
 };
 
 constexpr int kBM = 128;  // rows per CTA (UMMA M per CTA)
@@ -237,6 +246,10 @@ __device__ __forceinline__ void load_cols(const float* p, int col, int n, float 
   }
 }
 
+// Warps before the epilogue's: TMA and MMA, and for Q_WGRAD_SUM two idle ones, so that the epilogue
+// starts at a warpgroup.
+__host__ __device__ constexpr int lead_warps(int q) { return q == Q_WGRAD_SUM ? 4 : 2; }
+
 // Unit u -> (tile, split index, number of splits of that tile, K-block range).
 __device__ __forceinline__ void unit_info(const GemmParams& p, int u, int& t, int& sp, int& ns,
                                           int& kb_lo, int& kb_hi) {
@@ -272,13 +285,15 @@ __device__ __forceinline__ void m_tile_origin(const GemmParams& p, int mt, int& 
 // A K block is 128 bytes of K (64 or 128 elements), consumed by 4 UMMAs of 32 bytes of K each.
 template <int CG, int BN, bool B_KMAJOR, bool C_MCONTIG, int ESZ, int BMC = kBM, int EW = 4,
           bool ADD = false, int Q = Q_NONE>
-__global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
+__global__ void __launch_bounds__(32 * (lead_warps(Q) + EW), 1)
     gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmC, const GemmParams p) {
   using C = Cfg<CG, BN, BMC, EW>;
   static_assert(Q == Q_NONE || (!C_MCONTIG && !ADD && BMC == kBM), "8-bit layer instances");
   static_assert((Q != Q_I8 && Q != Q_FP8) || (ESZ == 1 && B_KMAJOR), "8-bit operands are K-major");
-  static_assert(Q != Q_WGRAD || (ESZ == 2 && !B_KMAJOR), "weight gradient: both operands MN-major");
+  static_assert(Q < Q_WGRAD || (ESZ == 2 && !B_KMAJOR), "weight gradient: both operands MN-major");
+  static_assert(Q != Q_WGRAD_SUM || (EW == 8 && BN <= 256), "two accumulators, eight epilogue warps");
+  constexpr bool A_MN = Q == Q_WGRAD || Q == Q_WGRAD_SUM;  // rows of A contiguous
   constexpr bool I8 = Q == Q_I8;
   constexpr int KB = kRowBytes / ESZ;                 // K elements per stage
   constexpr int ATOM = kRowBytes / ESZ;               // MN-major swizzle atom width (elements)
@@ -351,6 +366,25 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
 
   const int group_id = blockIdx.x / CG;
   const int num_groups = gridDim.x / CG;
+  // i-th unit of this CTA group (with k_parts, unit u is part u % k_parts of tile u / k_parts, and a
+  // tile's parts follow one another)
+  const int parts = Q == Q_WGRAD_SUM ? p.k_parts : 1;
+  auto unit_at = [&](int i) {
+    if constexpr (Q != Q_WGRAD_SUM) return group_id + i * num_groups;
+    const int r = i / parts;
+    return (group_id + r * num_groups) * parts + (i - r * parts);
+  };
+  auto unit_of = [&](int u, int& t, int& sp, int& ns, int& kb_lo, int& kb_hi) {
+    if constexpr (Q == Q_WGRAD_SUM) {
+      t = u / parts;
+      sp = 0;
+      ns = 1;
+      kb_lo = (u - t * parts) * p.k_per_part;
+      kb_hi = min(p.k_iters, kb_lo + p.k_per_part);
+    } else {
+      unit_info(p, u, t, sp, ns, kb_lo, kb_hi);
+    }
+  };
 
   // B columns of N-half h held by this CTA start at n0 + h*UN + cta_rank*BPH.
   auto issue_b = [&](uint32_t sb, uint32_t fb, int n0, int kc, int jj, int lb) {
@@ -374,14 +408,17 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
     }
   };
 
+  if (warp < lead_warps(Q)) {
+  // launched with 168 registers for each of 384 threads; 128 * 56 + 256 * 216 is less than that
+  if constexpr (Q == Q_WGRAD_SUM) ptx::regs_dec<56>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int u = group_id; u < p.num_units && ok; u += num_groups) {
+      for (int i = 0, u = unit_at(0); u < p.num_units && ok; u = unit_at(++i)) {
         int t, sp, ns, kb_lo, kb_hi;
-        unit_info(p, u, t, sp, ns, kb_lo, kb_hi);
+        unit_of(u, t, sp, ns, kb_lo, kb_hi);
         int pm, tn;
         b2g_sched_tile(t, p.num_pm_tiles, p.num_n_tiles, p.raster_group, &pm, &tn);
         const int mt = pm * CG + (int)cta_rank;
@@ -400,7 +437,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
           if (p.fault_flags & 1) continue;
           const int jj = kb / p.k_blocks_per_j;
           const int kc = (kb - jj * p.k_blocks_per_j) * KB;
-          if constexpr (Q == Q_WGRAD) {
+          if constexpr (A_MN) {
 #pragma unroll
             for (int c = 0; c < BMC / ATOM; ++c)
               ptx::tma_load_3d<CG>(base + s * C::A_BYTES + (uint32_t)c * ATOM_BYTES, &tmA, fb,
@@ -425,12 +462,13 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
       }
       if (!ok || *abort_flag) ptx::spin_ns(200000ull);  // abnormal exit: grace period for copies
     }
-  } else if (warp == 1) {
+  }
+  if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (leader && lane == 0) {
       const uint32_t idesc = I8 ? make_idesc_i8(BMC * CG, C::UN)
                                 : make_idesc(BMC * CG, C::UN, !B_KMAJOR, (uint32_t)p.ab_format) |
-                                      (Q == Q_WGRAD ? 1u << 15 : 0u);  // bit 15: A is MN-major
+                                      (A_MN ? 1u << 15 : 0u);  // bit 15: A is MN-major
       int it = 0, tc = 0;
       bool ok = true;
       // Issue the MMAs of K block kb from stage s into N-halves [h_lo, h_hi).
@@ -439,7 +477,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         const uint32_t sb = base + C::OFF_B + s * C::B_BYTES;
 #pragma unroll
         for (int k16 = 0; k16 < 4; ++k16) {  // 4 UMMAs of 32 bytes of K
-          const uint64_t ad = Q == Q_WGRAD ? ptx::smem_desc_sw128(sa + MN_STEP * k16, ATOM_BYTES, 1024u)
+          const uint64_t ad = A_MN ? ptx::smem_desc_sw128(sa + MN_STEP * k16, ATOM_BYTES, 1024u)
                                            : ptx::smem_desc_sw128(sa + 32u * k16, 16u, 1024u);
 #pragma unroll
           for (int h = 0; h < C::NH; ++h) {
@@ -454,9 +492,9 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
           }
         }
       };
-      for (int u = group_id; u < p.num_units && ok; u += num_groups, ++tc) {
+      for (int u = unit_at(0); u < p.num_units && ok; u = unit_at(++tc)) {
         int t, sp, ns, kb_lo, kb_hi;
-        unit_info(p, u, t, sp, ns, kb_lo, kb_hi);
+        unit_of(u, t, sp, ns, kb_lo, kb_hi);
         const int nkb = kb_hi - kb_lo;
         // BN <= 256: two accumulators, tempty[acc] guards accumulator acc.
         // BN = 512: one accumulator, tempty[h] guards its N-half h (the epilogue frees the
@@ -515,16 +553,18 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
       ptx::umma_commit<CG>(mma_done_bar, (uint16_t)(0x1u << pair0));
       ptx::mbar_wait_drain(mma_done_bar, 0u, err, ERR_WAIT_DRAIN, lim);
     }
+  }
   } else {
     // ------------------------------------------------------------ epilogue
+    if constexpr (Q == Q_WGRAD_SUM) ptx::regs_inc<216>();
     const int q = warp & 3;  // TMEM lane quarter
     // EW = 8: warps 2-5 and 6-9 cover the four lane quarters twice; `part` picks the 128
     // columns of each N-half this warp handles.  EW = 4: one warp per quarter, every column.
-    const int part_id = (warp - 2) >> 2;
+    const int part_id = (warp - lead_warps(Q)) >> 2;
     // (BN = 128: 64 of its columns)
     constexpr int PART = C::CHUNKS < 8 ? C::CHUNKS / 2 : 4;  // consecutive chunks of one part
     auto mine = [&](int ch) { return C::EPI_WARPS == 4 || ((ch / PART) & 1) == part_id; };
-    const uint32_t cbuf = base + C::OFF_C + (uint32_t)(warp - 2) * (uint32_t)C::EPI_BUFS * kCBuf;
+    const uint32_t cbuf = base + C::OFF_C + (uint32_t)(warp - lead_warps(Q)) * (uint32_t)C::EPI_BUFS * kCBuf;
     // This warp's 32-row sub-box inside the CTA's BMC-row tile (flattened (a, b, i) order) and
     // its columns: BMC = 128, all BN columns of rows 32q..32q+31; BMC = 64 (folded
     // accumulator), columns [(q/2)*BN/2, (q/2+1)*BN/2) of rows 32(q%2)..32(q%2)+31.
@@ -544,9 +584,10 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
     const int b_l = (r0 / p.bi) % p.bb;
     const int i_l = r0 % p.bi;
     int tc = 0, nstore = 0;
-    for (int u = group_id; u < p.num_units; u += num_groups, ++tc) {
+    uint32_t sums[Q == Q_WGRAD_SUM ? PART : 1][32] = {};  // running sums of a tile's K parts
+    for (int u = unit_at(0); u < p.num_units; u = unit_at(++tc)) {
       int t, sp, ns, kb_lo, kb_hi;
-      unit_info(p, u, t, sp, ns, kb_lo, kb_hi);
+      unit_of(u, t, sp, ns, kb_lo, kb_hi);
       int pm, tn;
       b2g_sched_tile(t, p.num_pm_tiles, p.num_n_tiles, p.raster_group, &pm, &tn);
       const int mt = pm * CG + (int)cta_rank;
@@ -592,6 +633,29 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
       ptx::tc_fence_after();
       const uint32_t tbase = tmem_base + ((uint32_t)(32 * q) << 16) + (uint32_t)acc * C::ACC_COLS;
       const int n0 = tn * BN + col_off;
+
+      // The 32 x 32 chunk in `buf` (word j of row r at r * 32 + (j ^ r): no bank is hit twice when it
+      // is written by rows and read by columns) to C at column gcol, row by row.
+      auto rows_out = [&](uint32_t buf, int gcol) {
+        const int nrows = min(32, p.i_size - ci), col = gcol + lane;
+        auto out = [&](auto* c, auto store) {
+          c += (long long)ci * p.ldc + col;
+#pragma unroll 8
+          for (int r = 0; r < 32; ++r)
+            if (r < nrows && col < p.n_size)
+              store(c + (long long)r * p.ldc,
+                    __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r)))));
+        };
+        if (p.c_type == 1)
+          out(static_cast<__half*>(p.c_direct), [](__half* c, float x) { *c = __float2half_rn(x); });
+        else if (p.c_type == 2)
+          out(static_cast<__nv_bfloat16*>(p.c_direct),
+              [](__nv_bfloat16* c, float x) { *c = __float2bfloat16_rn(x); });
+        else if (p.accumulate)
+          out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c += x; });
+        else
+          out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c = x; });
+      };
 
       // Stage chunk `ch` (32 columns of this warp's 32 rows) and TMA-store it.
       auto store_chunk = [&](const uint32_t (&v)[32], int ch) {
@@ -676,30 +740,11 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         }
         if constexpr (Q != Q_NONE) {
           if (p.c_direct && (p.direct_all || gcol + 32 > p.n_size)) {
-            // turn the 32 x 32 chunk in shared memory (word j of row r at r * 32 + (j ^ r): no bank
-            // is hit twice either way) and store it row by row, 32 columns at a time
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               ptx::st_shared_b32(buf + 4u * (uint32_t)(lane * 32 + (j ^ lane)), w[j]);
             __syncwarp();
-            const int nrows = min(32, p.i_size - ci), col = gcol + lane;
-            auto rows_out = [&](auto* c, auto store) {
-              c += (long long)ci * p.ldc + col;
-#pragma unroll 8
-              for (int r = 0; r < 32; ++r)
-                if (r < nrows && col < p.n_size)
-                  store(c + (long long)r * p.ldc,
-                        __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r)))));
-            };
-            if (p.c_type == 1)
-              rows_out(static_cast<__half*>(p.c_direct), [](__half* c, float x) { *c = __float2half_rn(x); });
-            else if (p.c_type == 2)
-              rows_out(static_cast<__nv_bfloat16*>(p.c_direct),
-                       [](__nv_bfloat16* c, float x) { *c = __float2bfloat16_rn(x); });
-            else if (p.accumulate)
-              rows_out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c += x; });
-            else
-              rows_out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c = x; });
+            rows_out(buf, gcol);
             __syncwarp();
             return;
           }
@@ -790,6 +835,56 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         }
       };
 
+      if constexpr (Q == Q_WGRAD_SUM) {
+#pragma unroll
+        for (int c = 0; c < 2 * PART; ++c) {
+          uint32_t x[16];
+          ptx::tmem_ld_32x32b_x16(tbase + 32u * (part_id * PART) + 16u * c, x);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            uint32_t& s = sums[c / 2][16 * (c & 1) + j];
+            s = __float_as_uint(__uint_as_float(s) + __uint_as_float(x[j]));
+          }
+        }
+        release(acc);
+        if (kb_hi == p.k_iters) {
+#pragma unroll
+          for (int c = 0; c < PART; ++c) {  // fp32, straight from the sums: store_chunk's copies would spill them
+            const int gcol = n0 + 32 * (part_id * PART + c);
+            if (!rows_valid || gcol >= p.n_size) continue;
+            if (lane == 0) ptx::bulk_wait_read<0>();
+            __syncwarp();
+            if (p.c_direct && (p.direct_all || gcol + 32 > p.n_size)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                ptx::st_shared_b32(cbuf + 4u * (uint32_t)(lane * 32 + (j ^ lane)), sums[c][j]);
+              __syncwarp();
+              rows_out(cbuf, gcol);
+              __syncwarp();
+              continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              ptx::st_shared_v4(cbuf + (uint32_t)lane * 128u + (uint32_t)((j ^ (lane & 7)) << 4), sums[c][4 * j],
+                                sums[c][4 * j + 1], sums[c][4 * j + 2], sums[c][4 * j + 3]);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (p.accumulate)
+                ptx::tma_reduce_add_4d(&tmC, cbuf, gcol, ci, cb, ca);
+              else
+                ptx::tma_store_4d(&tmC, cbuf, gcol, ci, cb, ca);
+              ptx::bulk_commit();
+            }
+          }
+          // (a first part that overwrites instead would cost a second set of registers)
+#pragma unroll
+          for (int c = 0; c < PART; ++c)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sums[c][j] = 0u;
+        }
+      } else {
       if ((CG == 1 || BMC != kBM) && ns > 1 && p.cluster_fixup) {
         // ---- cluster fix-up: partial tile -> this CTA's shared memory (the operand stages,
         // idle after its only unit's main loop) as float4 [chunk][warp][j][lane]; then split sp
@@ -1063,6 +1158,7 @@ __global__ void __launch_bounds__(Cfg<CG, BN, BMC, EW>::THREADS, 1)
         if (ch + 2 < C::CHUNKS) ptx::tmem_ld_32x32b_x32(tbase + 32u * (ch + 2), v0);
         store_chunk(v1, ch + 1);
       }
+      }  // Q != Q_WGRAD_SUM
     }
     if (lane == 0) ptx::bulk_wait_all();
     __syncwarp();

@@ -257,6 +257,54 @@ def test_gemm(b2g, cuda, M, N, K, q):
         check_gemm(cuda, b2g, M, N, K, q, c, pad)
 
 
+# (CTAs per tile, tile width) of the tiles for larger batches
+TILES = [(1, 128), (1, 256), (2, 256), (2, 512)]
+SPLITS = [dict(split_k=1), dict(split_k=3), dict(split_k=4, cluster_fixup=0), dict(split_k=3, serial_fixup=1)]
+
+
+@pytest.mark.parametrize("split", SPLITS, ids=["whole", "cluster", "parallel", "serial"])
+@pytest.mark.parametrize("cg,tn", TILES)
+@pytest.mark.parametrize("q", [I8, E4M3], ids=NAMES.get)
+def test_gemm_tiles_and_splits(b2g, cuda, q, cg, tn, split):
+    """Every tile, whole and with K split each way, with whole and ragged edges and an unaligned C."""
+    with options(b2g, cta_group=cg, tile_n=tn, tail_split=0, **split):
+        for M, N, K, c, pad in ((300, 1040, 1600, F32, 0), (385, 777, 2064, BF16, 16), (200, 600, 520, F16, 5)):
+            check_gemm(cuda, b2g, M, N, K, q, c, pad)
+            assert b2g.last_path() == (b2g.PATH_TC_1CTA if cg == 1 else b2g.PATH_TC_2CTA)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("M", [17, 32, 33, 64, 65, 128])
+@pytest.mark.parametrize("q", [I8, E4M3], ids=NAMES.get)
+def test_gemm_decoding_batches(b2g, cuda, q, M, splits):
+    with options(b2g, split_k=splits):
+        check_gemm(cuda, b2g, M, 520, 1184, q, F32, 0)
+        check_gemm(cuda, b2g, M, 129, 1040, q, BF16, 3)
+        assert b2g.last_path() == b2g.PATH_TC_1CTA
+
+
+def test_gemm_few_tokens_path(b2g, cuda):
+    for M, N, K in ((1, 512, 2048), (8, 100, 64), (9, 33, 16), (16, 515, 4112)):
+        check_gemm(cuda, b2g, M, N, K, I8, F32)
+        assert b2g.last_path() == b2g.PATH_FEW
+        check_gemm(cuda, b2g, M, N, K, E4M3, F16, 16)
+        assert b2g.last_path() == b2g.PATH_FEW
+
+
+@pytest.mark.parametrize("M", [40, 300])
+def test_gemm_wait_that_runs_out_is_reported(b2g, cuda, M):
+    """With its loads left out (test option), the product's bounded wait gives up: an error word, no
+    hang, and the next call is sound."""
+    torch = cuda
+    _, A = q8_matrix(torch, M, 1024, I8, 1)
+    _, B = q8_matrix(torch, 512, 1024, I8, 2)
+    C = torch.zeros(M, 512, device="cuda")
+    with options(b2g, fault_flags=1, timeout_ns=2000000):
+        b2g.gemm_q8(A, B, C, M, 512, 1024)
+        assert b2g.device_status() != 0
+    check_gemm(torch, b2g, M, 512, 1024, I8, F32)
+
+
 def test_gemm_optional_vectors_and_offsets(b2g, cuda):
     """No scales, no bias, and scale vectors that are not 16-byte aligned."""
     for M in (1, 20, 150):
@@ -319,6 +367,34 @@ def check_wgrad(torch, b2g, M, N, K, dt, q, c, pad=0, acc=False):
 def test_wgrad(b2g, cuda, M, N, K, dt, q):
     for c, pad, acc in ((F32, 0, False), (F32, 8, True), (dt, 3, False), (F32, 5, True), (dt, 16, False)):
         check_wgrad(cuda, b2g, M, N, K, dt, q, c, pad, acc)
+
+
+@pytest.mark.parametrize("split", SPLITS, ids=["whole", "cluster", "parallel", "serial"])
+@pytest.mark.parametrize("cg,tn", TILES)
+def test_wgrad_tiles_and_splits(b2g, cuda, cg, tn, split):
+    """Every tile, whole (long sums in parts) and with the tokens split each way."""
+    with options(b2g, cta_group=cg, tile_n=tn, tail_split=0, **split):
+        check_wgrad(cuda, b2g, 1700, 300, 1040, BF16, I8, F32, 0)
+        check_wgrad(cuda, b2g, 1601, 520, 777, F16, E4M3, F32, 3, True)
+        check_wgrad(cuda, b2g, 900, 264, 600, BF16, E4M3, BF16, 8)
+
+
+def test_wgrad_long_sums_keep_fp32(b2g, cuda):
+    """Relative error (2-norm) against 64 bits at most 1e-6, or 1.5 times that of the fp32 product where
+    that is more, however many tokens are summed: the tensor core's accumulator alone is 2.4e-6 off
+    at 2048."""
+    torch = cuda
+    for M, N, K, dt in ((2048, 1024, 1024, F16), (5000, 768, 1032, BF16), (16384, 512, 512, F16), (16384, 2048, 2048, BF16)):
+        g = torch.Generator(device="cuda").manual_seed(M)
+        dY = torch.randn(M, N, generator=g, device="cuda").to(tt(torch, dt))
+        Q = torch.randn(M, K, generator=g, device="cuda").mul_(30).clamp_(-127, 127).round_().to(torch.int8)
+        s = scales(torch, M, 5, pow2=True)
+        dW = torch.zeros(N, K, device="cuda")
+        b2g.wgrad_q8(dY, Q, s, dW, M, N, K, dtype=dt)
+        x = Q.float() * s[:, None]
+        ref = dY.double().t() @ x.double()
+        rel = lambda v: float((v.double() - ref).norm() / ref.norm())
+        assert rel(dW) <= max(1e-6, 1.5 * rel(dY.float().t() @ x))
 
 
 @pytest.mark.parametrize("M", [96, 4096, 9000])

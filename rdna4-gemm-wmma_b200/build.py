@@ -17,7 +17,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb2g_gemm.so")
 SOURCES = ["b2g_api.cu", "b2g_shard.cu", "b2g_rows.cu", "b2g_q8.cu"]
-HEADERS = ["ptx.cuh", "gemm_sm100.cuh", "sched.h", "errors.h", "plan.h", "host.h", "q8.cuh"]
+HEADERS = ["ptx.cuh", "gemm_sm100.cuh", "sched.h", "errors.h", "plan.h", "host.h", "q8.cuh",
+           "skinny_sm100.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

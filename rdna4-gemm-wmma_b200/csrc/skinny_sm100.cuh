@@ -9,7 +9,12 @@
 //
 // K is split over the CTAs of a cluster.  Each leaves its accumulator in its (idle) stages, and CTA r of
 // S sums columns r, r + S, ... of all of them through distributed shared memory in rank order.
+//
+// Nothing overlaps the epilogue, and a warp alone on its scheduler issues an instruction every few
+// cycles: so eight warps share it, and loads from several CTAs are in flight together.
 #pragma once
+#include <type_traits>
+
 #include "gemm_sm100.cuh"
 #include "q8.cuh"
 
@@ -40,7 +45,8 @@ struct SkinnyCfg {
   static constexpr uint32_t OFF_SCALE = OFF_MISC + 16;
   static constexpr uint32_t SMEM_BYTES = OFF_SCALE + NT * 4 + 1024;
   static constexpr uint32_t TMEM_COLS = NT;
-  static constexpr int THREADS = 192;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
 };
 static_assert(SkinnyCfg<32>::OFF_BAR >= 128 * 32 * 4 && SkinnyCfg<64>::OFF_BAR >= 128 * 64 * 4 &&
                   SkinnyCfg<128>::OFF_BAR >= 128 * 128 * 4,
@@ -138,8 +144,8 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 2)
     }
   }
 
-  // ------------------------------------------------------------ epilogue: warps 2..5
-  const int q = warp & 3;
+  // ------------------------------------------------------------ epilogue: warps 2..9
+  const int q = warp & 3, half = (warp - 2) >> 2;  // TMEM lane quarter; which of its two warps
   const int row = 32 * q + lane;
   const bool mine = warp >= 2 && n0 + row < p.N;
   float ws = 1.0f, bias = 0.0f;
@@ -147,13 +153,33 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 2)
     // the row's (output channel's) scale and bias, and the tokens' scales, while the MMAs run
     if (mine && p.b_scale) ws = __ldg(p.b_scale + n0 + row);
     if (mine && p.bias) bias = __ldg(p.bias + n0 + row);
-    for (int j = (int)threadIdx.x - 64; j < NT; j += 128) scale[j] = p.a_scale && j < p.M ? __ldg(p.a_scale + j) : 1.0f;
-    ptx::named_barrier_sync(1, 128);
+    for (int j = (int)threadIdx.x - 64; j < NT; j += 32 * C::EPI_WARPS) scale[j] = p.a_scale && j < p.M ? __ldg(p.a_scale + j) : 1.0f;
+    ptx::named_barrier_sync(1, 32 * C::EPI_WARPS);
   }
-  auto store = [&](int m, uint32_t acc) {
-    float v = (I8 ? (float)(int)acc : __uint_as_float(acc)) * scale[m];
-    v = v * ws + bias;
-    q8::store_elem(p.C, (int64_t)m * p.ldc + n0 + row, p.c_dtype, v);
+  // COUNT results, of tokens m, m + step, ...: everything is computed before the first store (a store
+  // could alias the scales as far as the compiler knows, and would wait for each of them in turn)
+  auto store = [&](auto count, int m, int step, const uint32_t* acc) {
+    constexpr int COUNT = decltype(count)::value;
+    float v[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int at = m + j * step;
+      const float x = I8 ? (float)(int)acc[j] : __uint_as_float(acc[j]);
+      v[j] = x * (at < NT ? scale[at] : 0.0f) * ws + bias;
+    }
+    const int64_t first = (int64_t)m * p.ldc + n0 + row, pitch = (int64_t)step * p.ldc;
+    auto out = [&](auto* c, auto put) {
+      c += first;
+#pragma unroll
+      for (int j = 0; j < COUNT; ++j)
+        if (mine && m + j * step < p.M) put(c + j * pitch, v[j]);
+    };
+    if (p.c_dtype == B2G_DTYPE_BF16)
+      out(static_cast<__nv_bfloat16*>(p.C), [](__nv_bfloat16* c, float x) { *c = __float2bfloat16_rn(x); });
+    else if (p.c_dtype == B2G_DTYPE_F16)
+      out(static_cast<__half*>(p.C), [](__half* c, float x) { *c = __float2half_rn(x); });
+    else
+      out(static_cast<float*>(p.C), [](float* c, float x) { *c = x; });
   };
   if (warp >= 2) {
     const bool got = ptx::mbar_wait(tfull_bar, 0u, abort_flag, err, ERR_WAIT_TFULL, lim);
@@ -161,18 +187,16 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 2)
       ptx::tc_fence_after();
       const uint32_t t = tmem + ((uint32_t)(32 * q) << 16);
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 32) {
+      for (int c = 16 * half; c < NT; c += 32) {
         if (c >= p.M) break;
-        uint32_t v[32];
-        ptx::tmem_ld_32x32b_x32(t + c, v);
+        uint32_t v[16];
+        ptx::tmem_ld_32x32b_x16(t + c, v);
         ptx::tmem_ld_wait();
         if (p.splits == 1) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (mine && c + j < p.M) store(c + j, v[j]);
+          store(std::integral_constant<int, 16>(), c, 1, v);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) ptx::st_shared_b32(base + 4u * (uint32_t)((c + j) * 128 + row), v[j]);
+          for (int j = 0; j < 16; ++j) ptx::st_shared_b32(base + 4u * (uint32_t)((c + j) * 128 + row), v[j]);
         }
       }
     }
@@ -181,18 +205,28 @@ __global__ void __launch_bounds__(SkinnyCfg<NT>::THREADS, 2)
     __syncwarp();
     ptx::cluster_sync();  // every CTA's accumulator is in its shared memory
     if (warp >= 2) {
-#pragma unroll 2
-      for (int m = split; m < p.M; m += p.splits) {
+      // eight tokens of a CTA's share, four of each half, and up to four CTAs' loads at a time
+#pragma unroll 1
+      for (int m = split + 4 * half * p.splits; m < p.M; m += 8 * p.splits) {
         const uint32_t at = base + 4u * (uint32_t)(m * 128 + row);
-        uint32_t x[8];
+        uint32_t s[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 1
+        for (int r0 = 0; r0 < p.splits; r0 += 4) {
+          uint32_t x[4][4];
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          x[r] = r < p.splits ? ptx::ld_shared_cluster_b32(ptx::mapa(at, (uint32_t)r)) : 0u;
-        float s = __uint_as_float(x[0]);
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int r = 1; r < 8; ++r)
-          if (r < p.splits) s = acc_add<I8>(s, __uint_as_float(x[r]));
-        if (mine) store(m, __float_as_uint(s));
+            for (int j = 0; j < 4; ++j)
+              if (r0 + r < p.splits && m + j * p.splits < p.M)
+                x[r][j] = ptx::ld_shared_cluster_b32(ptx::mapa(at, (uint32_t)(r0 + r)) + 512u * (uint32_t)(j * p.splits));
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (r0 + r < p.splits && m + j * p.splits < p.M)
+                s[j] = __float_as_uint(acc_add<I8>(__uint_as_float(s[j]), __uint_as_float(x[r][j])));
+        }
+        store(std::integral_constant<int, 4>(), m, p.splits, s);
       }
     }
     __syncwarp();

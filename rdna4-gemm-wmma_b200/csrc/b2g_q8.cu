@@ -263,68 +263,105 @@ int few_tokens(const FewArgs& a, int sms, cudaStream_t s) {
 
 // ------------------------------------------------------------------ aligned copies
 // Rows of `bytes` bytes from pitch `sp` to pitch `dp` (a multiple of 16), for operands whose base or
-// pitch TMA cannot address.  A warp copies 512 bytes of a row: each lane loads whole 4-byte words from
-// the word that holds its piece's first byte on, takes the next word from its neighbour and shifts
-// the two together.  Words that reach out of the matrix (its very ends) are put together from
-// bytes.  Bytes of the copy past the row get whatever follows the row: TMA never reads them.
-__global__ void __launch_bounds__(256)
-    repack_kernel(const uint8_t* src, uint8_t* dst, int64_t rows, int64_t bytes, int64_t sp, int64_t dp) {
-  constexpr int U = 4;  // words a lane
+// pitch TMA cannot address: up to two matrices a launch.
+struct RepackJob {
+  const uint8_t* src;
+  uint8_t* dst;
+  int64_t rows, bytes, sp, dp;
+  uint32_t pieces;  // of a row
+  int64_t items;    // rows * pieces (0: no matrix)
+};
+
+// A warp copies a piece of a row: each lane loads whole 4-byte words from the word that holds its first
+// byte on, takes the next word from its neighbour and shifts the two together.  A row's piece may
+// begin up to 3 bytes before the row and end as far behind it, inside the matrix; in its first and last
+// row words are put together from bytes where they would reach out of it.  Memory-bound: all of a
+// piece's loads are issued before the first is used.
+constexpr int kRepackWords = 8;  // words a lane
+
+__global__ void __launch_bounds__(256) repack_kernel(const RepackJob a, const RepackJob b) {
+  constexpr int U = kRepackWords;
   const int lane = threadIdx.x & 31;
-  const int64_t pieces = (bytes + 128 * U - 1) / (128 * U), total = rows * pieces;
-  const uint8_t* const end = src + (rows - 1) * sp + bytes;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < total; i += warps) {
-    const int64_t r = i / pieces, b = (i - r * pieces) * (128 * U);
-    const uint8_t* first = src + r * sp + b;
-    const uint32_t off = (uint32_t)(uintptr_t)first & 3u;
-    const uint8_t* base = first - off;
-    const int64_t left = bytes - b + off;  // bytes of the row from `base` on
-    auto word = [&](int64_t at) -> uint32_t {
-      const uint8_t* p = base + at;
-      if (at >= left) return 0;
-      if (p >= src && p + 4 <= end) return __ldcs(reinterpret_cast<const uint32_t*>(p));
-      uint32_t w = 0;
-      for (int k = 0; k < 4; ++k)
-        if (p + k >= src && p + k < end) w |= (uint32_t)p[k] << (8 * k);
-      return w;
-    };
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); i < a.items + b.items; i += warps) {
+    const RepackJob& g = i < a.items ? a : b;
+    const uint64_t item = (uint64_t)(i < a.items ? i : i - a.items);
+    const int64_t r = item >> 32 ? (int64_t)(item / g.pieces) : (int64_t)((uint32_t)item / g.pieces);
+    const int64_t at0 = (int64_t)(item - (uint64_t)r * g.pieces) * (128 * U) + lane * 4;
+    const uint8_t* row = g.src + r * g.sp;
+    const uint32_t off = (uint32_t)(uintptr_t)row & 3u;  // (a piece is whole words: the same for all)
+    const uint8_t* p = row - off + at0;
+    const int64_t left = g.bytes + off - at0;  // bytes of the row from p on
     uint32_t w[U], last = 0;
+    if (r > 0 && r < g.rows - 1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = word(u * 128 + lane * 4);
-    if (lane == 31) last = word(U * 128);
+      for (int u = 0; u < U; ++u)
+        w[u] = u * 128 < left ? __ldcs(reinterpret_cast<const uint32_t*>(p + u * 128)) : 0u;
+      if (lane == 31 && (U - 1) * 128 + 4 < left) last = __ldcs(reinterpret_cast<const uint32_t*>(p + (U - 1) * 128 + 4));
+    } else {
+      const uint8_t* const end = g.src + (g.rows - 1) * g.sp + g.bytes;
+      auto word = [&](const uint8_t* q, int64_t here) -> uint32_t {
+        if (here <= 0) return 0;
+        if (q >= g.src && q + 4 <= end) return *reinterpret_cast<const uint32_t*>(q);
+        uint32_t v = 0;
+        for (int k = 0; k < 4; ++k)
+          if (q + k >= g.src && q + k < end) v |= (uint32_t)q[k] << (8 * k);
+        return v;
+      };
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = word(p + u * 128, left - u * 128);
+      if (lane == 31) last = word(p + (U - 1) * 128 + 4, left - (U - 1) * 128 - 4);
+    }
+    uint8_t* d = g.dst + r * g.dp + at0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint32_t next = __shfl_down_sync(0xffffffffu, w[u], 1);
       const uint32_t wrap = u + 1 < U ? __shfl_sync(0xffffffffu, w[u + 1 < U ? u + 1 : u], 0) : last;
       if (lane == 31) next = wrap;
-      const int64_t at = b + u * 128 + lane * 4;
-      if (at < bytes) *reinterpret_cast<uint32_t*>(dst + r * dp + at) = __funnelshift_r(w[u], next, off * 8);
+      if (at0 + u * 128 < g.bytes) *reinterpret_cast<uint32_t*>(d + u * 128) = __funnelshift_r(w[u], next, off * 8);
     }
   }
 }
 
-// *p and *pitch (bytes) become a 16-byte aligned form of the matrix: as they are, or a copy in `ws`.
-int aligned_rows(const void** p, int64_t* pitch, int64_t rows, int64_t bytes, int sms, Workspace& ws,
-                 cudaStream_t s) {
-  const uintptr_t low = (uintptr_t)*p | (uintptr_t)(rows > 1 ? *pitch : 0);
-  if ((low & 15) == 0) return B2G_OK;
-  const int64_t dp = (bytes + 15) / 16 * 16;
-  int rc = ws.alloc((size_t)(rows * dp), "cudaMallocFromPoolAsync(aligned copy)");
-  if (rc != B2G_OK) return rc;
-  const unsigned blocks = (unsigned)std::min<int64_t>((rows * ((bytes + 511) / 512) + 7) / 8, (int64_t)sms * 32);
-  repack_kernel<<<blocks, 256, 0, s>>>(static_cast<const uint8_t*>(*p), static_cast<uint8_t*>(ws.get()), rows, bytes,
-                                       *pitch, dp);
-  rc = launched("repack_kernel");
-  *p = ws.get();
-  *pitch = dp;
-  return rc;
+// An operand by its rows of bytes; `copy` where it needs a 16-byte aligned form.
+struct Rows {
+  const void* p;
+  int64_t pitch, rows, bytes;
+  bool copy() const { return (((uintptr_t)p | (uintptr_t)(rows > 1 ? pitch : 0)) & 15) != 0; }
+  int64_t aligned_pitch() const { return (bytes + 15) / 16 * 16; }
+  size_t copy_bytes() const { return copy() ? (size_t)(rows * aligned_pitch() + 255) / 256 * 256 : 0; }
+};
+
+// Turns the operands that need it into aligned copies in `mem` (the sum of their copy_bytes()).
+int align_rows(Rows* a, Rows* b, void* mem, int sms, cudaStream_t s) {
+  RepackJob jobs[2] = {};
+  uint8_t* at = static_cast<uint8_t*>(mem);
+  int n = 0;
+  for (Rows* x : {a, b}) {
+    if (!x || !x->copy()) continue;
+    RepackJob& j = jobs[n++];
+    j.src = static_cast<const uint8_t*>(x->p);
+    j.dst = at;
+    j.rows = x->rows;
+    j.bytes = x->bytes;
+    j.sp = x->pitch;
+    j.dp = x->aligned_pitch();
+    j.pieces = (uint32_t)((x->bytes + 128 * kRepackWords - 1) / (128 * kRepackWords));
+    j.items = j.rows * j.pieces;
+    at += x->copy_bytes();
+    x->p = j.dst;
+    x->pitch = j.dp;
+  }
+  if (n == 0) return B2G_OK;
+  const int64_t blocks = std::min<int64_t>((jobs[0].items + jobs[1].items + 7) / 8, (int64_t)sms * 64);
+  repack_kernel<<<(unsigned)blocks, 256, 0, s>>>(jobs[0], jobs[1]);
+  return launched("repack_kernel");
 }
 
 // ------------------------------------------------------------------ tensor-core launch
 // C (rows x cols, row-major) from a 128-byte-K-block product of gemm_tc_kernel.  Q_I8 / Q_FP8: A is
 // rows x k, B cols x k, 8-bit, K contiguous.  Q_WGRAD: A is k x rows, B k x cols, 16-bit, rows and
-// columns contiguous.  Bases and pitches of A and B are 16-byte aligned (aligned_rows).
+// columns contiguous.  Bases and pitches of A and B are 16-byte aligned (align_rows).
 struct Product {
   int q;
   const void *A, *B;
@@ -725,10 +762,15 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
   if (rc != B2G_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (tensor_ok(cc, M, N, K)) {
-    Workspace wa(s), wb(s);
-    rc = aligned_rows(&A, &lda, M, K, sms, wa, s);
-    if (rc == B2G_OK) rc = aligned_rows(&B, &ldb, N, K, sms, wb, s);
-    if (rc != B2G_OK) return rc;
+    Workspace ws(s);
+    Rows ra = {A, lda, M, K}, rb = {B, ldb, N, K};
+    if (ra.copy() || rb.copy()) {
+      rc = ws.alloc(ra.copy_bytes() + rb.copy_bytes(), "cudaMallocFromPoolAsync(aligned operands)");
+      if (rc == B2G_OK) rc = align_rows(&ra, &rb, ws.get(), sms, s);
+      if (rc != B2G_OK) return rc;
+      A = ra.p; lda = ra.pitch;
+      B = rb.p; ldb = rb.pitch;
+    }
     const FewArgs f = {A, B, C, M, N, K, lda, ldb, ldc, a_scale, b_scale, bias, c_dtype};
     if (is_few(f)) {
       rc = dtype == B2G_DTYPE_I8 ? few_tokens<true>(f, sms, s) : few_tokens<false>(f, sms, s);
@@ -777,13 +819,15 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
   if (rc != B2G_OK) return rc;
   if (tensor_ok(cc, N, K, M)) {
     // the checkpoint's rows in dY's type, then the product of two token-major matrices
-    Workspace wx(s), wy(s);
+    Workspace ws(s);
     const int64_t ldx = (K + 7) / 8 * 8;
-    rc = wx.alloc((size_t)(M * ldx) * 2, "cudaMallocFromPoolAsync(dequantized checkpoint)");
-    if (rc == B2G_OK) rc = dequantize_rows(Q, scale, wx.get(), M, K, ldq, ldx, q_dtype, dtype, s);
-    int64_t pitch = ldy * 2;
-    if (rc == B2G_OK) rc = aligned_rows(&dY, &pitch, M, N * 2, sms, wy, s);
+    const size_t x_bytes = ((size_t)(M * ldx) * 2 + 255) / 256 * 256;
+    Rows ry = {dY, ldy * 2, M, N * 2};
+    rc = ws.alloc(x_bytes + ry.copy_bytes(), "cudaMallocFromPoolAsync(dequantized checkpoint)");
+    if (rc == B2G_OK) rc = dequantize_rows(Q, scale, ws.get(), M, K, ldq, ldx, q_dtype, dtype, s);
+    if (rc == B2G_OK) rc = align_rows(&ry, nullptr, static_cast<char*>(ws.get()) + x_bytes, sms, s);
     if (rc != B2G_OK) return rc;
+    const int64_t pitch = ry.pitch;
     // fp32: whole tiles take their tokens in parts of kMaxTokens (launch_product); where K is split
     // over CTAs, a launch has at most kMaxTokens a split, and the next one adds to it
     const int part_blocks = c_dtype == B2G_DTYPE_F32 ? (int)(kMaxTokens / 64) : 0;
@@ -794,8 +838,8 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
       if (splits > 1) per = std::min(M, splits * kMaxTokens);
     }
     for (int64_t m0 = 0; m0 < M && rc == B2G_OK; m0 += per) {
-      const Product g = {Q_WGRAD, static_cast<const char*>(dY) + m0 * pitch,
-                         static_cast<const char*>(wx.get()) + m0 * ldx * 2, dW, N, K,
+      const Product g = {Q_WGRAD, static_cast<const char*>(ry.p) + m0 * pitch,
+                         static_cast<const char*>(ws.get()) + m0 * ldx * 2, dW, N, K,
                          std::min(per, M - m0), pitch / 2, ldx, ldw, dtype == B2G_DTYPE_F16 ? 0 : 1,
                          c_type_of(c_dtype), accumulate != 0 || m0 > 0, nullptr, nullptr, nullptr,
                          part_blocks};

@@ -576,39 +576,42 @@ __global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const Norm
   }
 }
 
-// Rows out of 8 bits.  Memory-bound: 1 byte in, 2 or 4 out.  A block does one piece of a row, PIECE
-// vectors of 16 values a thread (8 single values, a block's width apart, where !VEC16), all loads
-// before the first store.
+// Rows out of 8 bits.  Memory-bound: 1 byte in, 2 or 4 out.  VEC16: 16 values a vector, two vectors a
+// thread, vectors numbered over the whole matrix (so that short rows fill a block); else single
+// values, eight a thread, a block's width apart in one row.  All loads go before the first store.
 constexpr int kPiece = 2, kPieceElems = 8;
 
 template <typename T, bool VEC16>
 __global__ void __launch_bounds__(kRowThreads)
     dequantize_kernel(const uint8_t* Q, const float* scale, T* X, int64_t M, int64_t N, int64_t ldq,
                       int64_t ldx, int q_dtype, float top) {
-  constexpr int VEC = VEC16 ? 16 : 1, OUT = 16 / (int)sizeof(T);
-  const int per_block = kRowThreads * (VEC16 ? kPiece * VEC : kPieceElems);
-  const int64_t bpr = (N + per_block - 1) / per_block;  // pieces of a row
-  for (int64_t b = blockIdx.x; b < M * bpr; b += gridDim.x) {
-    const int64_t m = b / bpr, n0 = (b - m * bpr) * per_block + (int64_t)threadIdx.x * VEC;
-    const uint8_t* q = Q + m * ldq;
-    T* x = X + m * ldx;
-    const float s = __ldg(scale + m);
-    auto one = [&](int64_t n) {
-      from_f(x + n, clamp_to(load_elem(q, n, q_dtype) * s, top));
-    };
-    if constexpr (VEC16) {
+  if constexpr (VEC16) {
+    constexpr int OUT = 16 / (int)sizeof(T);
+    const uint32_t per_row = (uint32_t)((N + 15) / 16);
+    const int64_t total = M * per_row, span = (int64_t)gridDim.x * kRowThreads * kPiece;
+    for (int64_t i0 = (int64_t)blockIdx.x * kRowThreads * kPiece + threadIdx.x; i0 < total; i0 += span) {
       uint4 c[kPiece];
+      float s[kPiece];
+      int64_t m[kPiece], n[kPiece];
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i) {
-        const int64_t n = n0 + (int64_t)i * kRowThreads * VEC;
-        if (n + VEC <= N) c[i] = __ldcs(reinterpret_cast<const uint4*>(q + n));
+      for (int k = 0; k < kPiece; ++k) {
+        const int64_t i = i0 + k * kRowThreads;
+        m[k] = i >> 32 ? i / per_row : (int64_t)((uint32_t)i / per_row);
+        n[k] = (i - m[k] * per_row) * 16;
+        s[k] = 0.0f;
+        if (i < total) {
+          s[k] = __ldg(scale + m[k]);
+          if (n[k] + 16 <= N) c[k] = __ldcs(reinterpret_cast<const uint4*>(Q + m[k] * ldq + n[k]));
+        }
       }
-      const bool big = !(fabsf(s) * 448.0f <= top);  // a value may pass the type's range (or s is NaN)
 #pragma unroll
-      for (int i = 0; i < kPiece; ++i) {
-        const int64_t n = n0 + (int64_t)i * kRowThreads * VEC;
-        if (n + VEC <= N && !big) {
-          const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+      for (int k = 0; k < kPiece; ++k) {
+        if (i0 + k * kRowThreads >= total) break;
+        T* x = X + m[k] * ldx + n[k];
+        const float f = s[k];
+        // (a value that may pass the type's range, or a NaN scale, goes the slower way)
+        if (n[k] + 16 <= N && fabsf(f) * 448.0f <= top) {
+          const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
           Vec<T, OUT> o[16 / OUT];
           T* d = o[0].e;
 #pragma unroll
@@ -616,27 +619,37 @@ __global__ void __launch_bounds__(kRowThreads)
             F2 lo, hi;
             unpack_q8x4(w[j], q_dtype, lo, hi);
             float v[4];
-            f2_get(f2_mul(lo, f2(s, s)), v[0], v[1]);
-            f2_get(f2_mul(hi, f2(s, s)), v[2], v[3]);
+            f2_get(f2_mul(lo, f2(f, f)), v[0], v[1]);
+            f2_get(f2_mul(hi, f2(f, f)), v[2], v[3]);
 #pragma unroll
             for (int l = 0; l < 4; ++l) from_f(d + 4 * j + l, v[l]);
           }
 #pragma unroll
-          for (int j = 0; j < 16 / OUT; ++j) *reinterpret_cast<Vec<T, OUT>*>(x + n + j * OUT) = o[j];
+          for (int j = 0; j < 16 / OUT; ++j) *reinterpret_cast<Vec<T, OUT>*>(x + j * OUT) = o[j];
         } else {
-          for (int64_t j = n; j < N && j < n + VEC; ++j) one(j);
+          const int count = N - n[k] < 16 ? (int)(N - n[k]) : 16;
+          for (int j = 0; j < count; ++j) from_f(x + j, clamp_to(load_elem(Q + m[k] * ldq + n[k], j, q_dtype) * f, top));
         }
       }
-    } else {
+    }
+  } else {
+    constexpr int per_block = kRowThreads * kPieceElems;
+    const int64_t bpr = (N + per_block - 1) / per_block;  // pieces of a row
+    for (int64_t b = blockIdx.x; b < M * bpr; b += gridDim.x) {
+      const int64_t m = b / bpr, n0 = (b - m * bpr) * per_block + threadIdx.x;
+      const uint8_t* q = Q + m * ldq + n0;
+      T* x = X + m * ldx + n0;
+      const float s = __ldg(scale + m);
+      const int64_t left = N - n0;
       uint8_t c[kPieceElems];
 #pragma unroll
-      for (int i = 0; i < kPieceElems; ++i) c[i] = n0 + i * kRowThreads < N ? q[n0 + i * kRowThreads] : 0;
+      for (int i = 0; i < kPieceElems; ++i) c[i] = i * kRowThreads < left ? q[i * kRowThreads] : 0;
 #pragma unroll
       for (int i = 0; i < kPieceElems; ++i)
-        if (n0 + i * kRowThreads < N) {
+        if (i * kRowThreads < left) {
           const float v = q_dtype == B2G_DTYPE_I8 ? (float)(int8_t)c[i]
                                                   : float(*reinterpret_cast<const __nv_fp8_e4m3*>(&c[i]));
-          from_f(x + n0 + i * kRowThreads, clamp_to(v * s, top));
+          from_f(x + i * kRowThreads, clamp_to(v * s, top));
         }
     }
   }
@@ -1039,14 +1052,14 @@ template <typename T, bool NORM, int V, int THREADS, int CTAS>
 bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   const uint32_t row_bytes = (uint32_t)(a.N * (int64_t)sizeof(T));
   const uint32_t stage = (a.R ? 2 : 1) * row_bytes;
-  int ctas = 0, stages = 0;
-  if (!ring_shape(stage, CTAS, &ctas, &stages) || a.M < (int64_t)sms * ctas * 2) return false;
+  const int64_t nv = a.N * (int64_t)sizeof(T) / 16;
+  const int threads = (int)((nv + V * 32 - 1) / (V * 32)) * 32;
+  int ctas = 0, stages = 0;  // (blocks of fewer threads than THREADS leave registers for more of them)
+  if (!ring_shape(stage, THREADS * CTAS / threads, &ctas, &stages) || a.M < (int64_t)sms * ctas * 2) return false;
   auto fn = rows_ring_kernel<T, NORM, V, THREADS, CTAS>;
   static std::atomic<uint64_t> ready{0};
   *rc = raise_smem(fn, ready);
   if (*rc != B2G_OK) return true;
-  const int64_t nv = a.N * (int64_t)sizeof(T) / 16;
-  const int threads = (int)((nv + V * 32 - 1) / (V * 32)) * 32;
   fn<<<(unsigned)(sms * ctas), threads, (uint32_t)stages * (stage + 8), s>>>(
       a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
   *rc = launched("rows_ring_kernel");
@@ -1090,7 +1103,8 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
         : nv <= 256 ? launch_ring<T, NORM, 2, 128, NORM ? 7 : 8>(a, sms, s, &rc)
         : nv <= 512 ? launch_ring<T, NORM, 4, 128, NORM ? 4 : 7>(a, sms, s, &rc)
         : nv <= 1024 ? launch_ring<T, NORM, 4, 256, NORM ? 2 : 4>(a, sms, s, &rc)
-        : nv <= 2048 ? launch_ring<T, NORM, 8, 256, 2>(a, sms, s, &rc)
+        : nv <= 2048 ? launch_ring<T, NORM, 4, 512, NORM ? 1 : 2>(a, sms, s, &rc)
+        : nv <= 4096 ? launch_ring<T, NORM, 8, 512, 1>(a, sms, s, &rc)
                      : false)
       return rc;
     if (nv <= 256) return launch_rows<T, NORM, VEC, 1, 0>(a, (int)(nv + 31) / 32 * 32, sms, s);
@@ -1131,8 +1145,9 @@ int dequantize_to(const void* Q, const float* scale, T* X, int64_t M, int64_t N,
                   int q_dtype, float top, int sms, cudaStream_t s) {
   const uint8_t* q = static_cast<const uint8_t*>(Q);
   const bool vec = aligned(Q, ldq, M, 16) && aligned(X, ldx * (int64_t)sizeof(T), M, 16);
-  const int64_t per_block = kRowThreads * (vec ? kPiece * 16 : kPieceElems);
-  const int64_t blocks = std::min<int64_t>(M * ((N + per_block - 1) / per_block), (int64_t)sms * 1024);
+  const int64_t per_block = kRowThreads * (vec ? kPiece : kPieceElems);
+  const int64_t need = vec ? (M * ((N + 15) / 16) + per_block - 1) / per_block : M * ((N + per_block - 1) / per_block);
+  const int64_t blocks = std::min<int64_t>(need, (int64_t)sms * 1024);
   if (vec)
     dequantize_kernel<T, true><<<(unsigned)blocks, kRowThreads, 0, s>>>(q, scale, X, M, N, ldq, ldx, q_dtype, top);
   else

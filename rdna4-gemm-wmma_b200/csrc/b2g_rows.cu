@@ -765,10 +765,15 @@ __global__ void __launch_bounds__(512, 1)
   for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int j = 0; j < P; ++j) dw[i][j] = f2(0.0f, 0.0f);
+  // a row's two factors, loaded a row ahead
+  float next_rstd = __ldg(a.rstd + first), next_scale = a.x_scale ? __ldg(a.x_scale + first) : 1.0f;
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
-    const float rstd = __ldg(a.rstd + m);
-    const float xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    const float rstd = next_rstd, xs = next_scale * rstd;
+    if (m + step < a.M) {
+      next_rstd = __ldg(a.rstd + m + step);
+      if (a.x_scale) next_scale = __ldg(a.x_scale + m + step);
+    }
     const F2 xs2 = f2(xs, xs);
     const bool ok = ring.wait(k);
     const uint8_t* st = smem + (uint32_t)(k % stages) * stage_bytes;
@@ -903,10 +908,15 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS)
     w[i] = f[0];
     dw[i] = 0.0f;
   }
+  // a row's two factors, loaded a row ahead
+  float next_rstd = __ldg(a.rstd + first), next_scale = a.x_scale ? __ldg(a.x_scale + first) : 1.0f;
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
-    const float rstd = __ldg(a.rstd + m);
-    const float xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    const float rstd = next_rstd, xs = next_scale * rstd;
+    if (m + step < a.M) {
+      next_rstd = __ldg(a.rstd + m + step);
+      if (a.x_scale) next_scale = __ldg(a.x_scale + m + step);
+    }
     const bool ok = ring.wait(k), end = at_end(m);
     const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     float g[V], xh[V], dr[V];

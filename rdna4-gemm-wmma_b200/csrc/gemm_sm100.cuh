@@ -635,26 +635,25 @@ __global__ void __launch_bounds__(32 * (lead_warps(Q) + EW), 1)
       const int n0 = tn * BN + col_off;
 
       // The 32 x 32 chunk in `buf` (word j of row r at r * 32 + (j ^ r): no bank is hit twice when it
-      // is written by rows and read by columns) to C at column gcol, row by row.
+      // is written by rows and read by columns; a 16-bit C's values in the low halves) to C at
+      // column gcol, row by row.
       auto rows_out = [&](uint32_t buf, int gcol) {
         const int nrows = min(32, p.i_size - ci), col = gcol + lane;
-        auto out = [&](auto* c, auto store) {
-          c += (long long)ci * p.ldc + col;
+        if (col >= p.n_size) return;
+        const int esz = p.c_type == 0 ? 4 : 2;
+        char* c = static_cast<char*>(p.c_direct) + ((long long)ci * p.ldc + col) * esz;
+        const long long pitch = p.ldc * esz;
+        auto word = [&](int r) { return ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r))); };
+        if (p.c_type != 0) {
 #pragma unroll 8
-          for (int r = 0; r < 32; ++r)
-            if (r < nrows && col < p.n_size)
-              store(c + (long long)r * p.ldc,
-                    __uint_as_float(ptx::ld_shared_b32(buf + 4u * (uint32_t)(r * 32 + (lane ^ r)))));
-        };
-        if (p.c_type == 1)
-          out(static_cast<__half*>(p.c_direct), [](__half* c, float x) { *c = __float2half_rn(x); });
-        else if (p.c_type == 2)
-          out(static_cast<__nv_bfloat16*>(p.c_direct),
-              [](__nv_bfloat16* c, float x) { *c = __float2bfloat16_rn(x); });
-        else if (p.accumulate)
-          out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c += x; });
-        else
-          out(static_cast<float*>(p.c_direct), [](float* c, float x) { *c = x; });
+          for (int r = 0; r < nrows; ++r, c += pitch) *reinterpret_cast<uint16_t*>(c) = (uint16_t)word(r);
+        } else if (!p.accumulate) {
+#pragma unroll 8
+          for (int r = 0; r < nrows; ++r, c += pitch) *reinterpret_cast<uint32_t*>(c) = word(r);
+        } else {
+#pragma unroll 8
+          for (int r = 0; r < nrows; ++r, c += pitch) *reinterpret_cast<float*>(c) += __uint_as_float(word(r));
+        }
       };
 
       // Stage chunk `ch` (32 columns of this warp's 32 rows) and TMA-store it.
@@ -740,6 +739,13 @@ __global__ void __launch_bounds__(32 * (lead_warps(Q) + EW), 1)
         }
         if constexpr (Q != Q_NONE) {
           if (p.c_direct && (p.direct_all || gcol + 32 > p.n_size)) {
+            if (p.c_type == 1) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __half_as_ushort(__float2half_rn(__uint_as_float(w[j])));
+            } else if (p.c_type == 2) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) w[j] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(w[j])));
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               ptx::st_shared_b32(buf + 4u * (uint32_t)(lane * 32 + (j ^ lane)), w[j]);

@@ -298,14 +298,18 @@ def main():
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-cublas", action="store_true")
     ap.add_argument("--workload", default="gemm8192",
-                    choices=["gemm8192", "sharded32768", "contraction5d", "tp_k"],
+                    choices=["gemm8192", "sharded32768", "contraction5d", "tp_k", "linear_q8"],
                     help="gemm8192: BASELINE configs[1] per GPU (the default line); "
                          "contraction5d: BASELINE configs[2] through the contraction entry point "
                          "(C[a,b,i,n] = sum A[a,b,i,j,k] B[j,k,n], a8 b16 i64 j64 k128 n4096); "
                          "sharded32768: BASELINE configs[4], one 32768^3 GEMM as M-row slabs "
                          "over the N GPUs, B broadcast in K panels inside every step; "
                          "tp_k: tensor-parallel K-split GEMM (8192^3 or --shape) whose partials "
-                         "are reduce-scattered over the N GPUs inside every step")
+                         "are reduce-scattered over the N GPUs inside every step; "
+                         "linear_q8: one training step of an 8-bit linear layer on one GPU (RMS norm "
+                         "into 8 bits, scaled product, weight gradient and norm backward from the "
+                         "8-bit checkpoints; 8192 tokens, 8192 -> 8192, or --shape tokens,out,in, "
+                         "--dtype i8 or e4m3)")
     ap.add_argument("--bcast", default="chain", choices=["chain", "nccl"],
                     help="sharded32768: how B reaches the ranks each step (copy-engine chain, "
                          "or ncclBroadcast)")
@@ -320,8 +324,9 @@ def main():
     ap.add_argument("--shape", default=None,
                     help="M,N,K: time this row-major GEMM instead of 8192^3 (device-resident "
                          "kernel loop only; used for the other BASELINE shapes and for profiling)")
-    ap.add_argument("--dtype", default="f16", choices=["f16", "bf16", "e4m3", "e5m2"],
-                    help="operand type (f16 = BASELINE's; the others are secondary lines)")
+    ap.add_argument("--dtype", default="f16", choices=["f16", "bf16", "e4m3", "e5m2", "i8"],
+                    help="operand type (f16 = BASELINE's; the others are secondary lines; i8: "
+                         "linear_q8 only, and its default)")
     ap.add_argument("--out", default="f32", choices=["f32", "f16", "bf16"],
                     help="type C is stored in (the fused epilogue; f32 = BASELINE's). Kernel loop only")
     ap.add_argument("--bias", action="store_true",
@@ -364,6 +369,10 @@ def main():
         b2g.set_option(key, int(val))
     if args.workload == "sharded32768":
         return run_sharded(args, torch, dist, b2g, ws, rank, local, dev)
+    if args.workload == "linear_q8":
+        return run_linear_q8(args, torch, b2g, dev)
+    if args.dtype == "i8":
+        ap.error("--dtype i8 goes with --workload linear_q8")
     if args.workload == "tp_k":
         return run_tp_k(args, torch, dist, b2g, ws, rank, local, dev)
 
@@ -858,6 +867,79 @@ def run_tp_k(args, torch, dist, b2g, ws, rank, local, dev):
                          "peak_source": "%s bf16_tflops_sustained; peer copy 770 GB/s" % src},
             "row0_out_of_tolerance": bad, "device_status": status,
             "gpu_launches": launches}), flush=True)
+    return 0
+
+
+def run_linear_q8(args, torch, b2g, dev):
+    """One training step of an 8-bit linear layer, y = W . norm(x + r): RMS norm with the residual's
+    addition into 8 bits, the residual stream put aside in 8 bits, the scaled product, the weight
+    gradient and the norm's backward pass from the two 8-bit checkpoints.  Weights are quantised
+    once, as an inference engine or a step with frozen 8-bit weights does."""
+    M, N, K = (int(x) for x in args.shape.split(",")) if args.shape else (8192, 8192, 8192)
+    q = b2g.DTYPE_E4M3 if args.dtype == "e4m3" else b2g.DTYPE_I8
+    qt = torch.float8_e4m3fn if q == b2g.DTYPE_E4M3 else torch.int8
+    bf, f32 = torch.bfloat16, torch.float32
+    g = torch.Generator(device=dev).manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev)
+    new = lambda *s, t=f32: torch.empty(*s, dtype=t, device=dev)
+    x, r, da = rnd(M, K).to(bf), rnd(M, K).to(bf), (0.1 * rnd(M, K)).to(bf)
+    dy, w = (0.1 * rnd(M, N)).to(bf), (1 + 0.1 * rnd(K)).to(bf)
+    W, Wq, Ws = (rnd(N, K) / K ** 0.5).to(bf), new(N, K, t=qt), new(N)
+    h, a, sa, rstd = new(M, K, t=bf), new(M, K, t=qt), new(M), new(M)
+    hq, sh, y, dW = new(M, K, t=qt), new(M), new(M, N, t=bf), new(N, K)
+    dx, dw = new(M, K, t=bf), new(K)
+    BF = b2g.DTYPE_BF16
+    b2g.quantize_q8(W, Wq, Ws, N, K, dtype=BF, q_dtype=q)
+    parts = [
+        ("rmsnorm_q8", lambda: b2g.rmsnorm_q8(x, w, a, sa, M, K, dtype=BF, q_dtype=q, R=r, H=h, rstd=rstd, pow2=True)),
+        ("quantize_q8", lambda: b2g.quantize_q8(h, hq, sh, M, K, dtype=BF, q_dtype=q)),
+        ("gemm_q8", lambda: b2g.gemm_q8(a, Wq, y, M, N, K, dtype=q, a_scale=sa, b_scale=Ws, c_dtype=BF)),
+        ("wgrad_q8", lambda: b2g.wgrad_q8(dy, a, sa, dW, M, N, K, dtype=BF, q_dtype=q)),
+        ("rmsnorm_bwd_q8", lambda: b2g.rmsnorm_bwd_q8(da, hq, sh, w, rstd, dx, dw, M, K, dtype=BF, x_dtype=q, dres=da)),
+    ]
+
+    def timed(fns, steps):
+        for _ in range(args.warmup):
+            for f in fns:
+                f()
+        torch.cuda.synchronize()
+        t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        t0.record()
+        for _ in range(steps):
+            for f in fns:
+                f()
+        t1.record()
+        torch.cuda.synchronize()
+        return t0.elapsed_time(t1) / steps
+
+    launches0 = b2g.get_option("launches")
+    clocks = ClockSampler(dev.index) if args.sample_clocks else None
+    if clocks:
+        clocks.start()
+    ms = timed([f for _, f in parts], args.steps)
+    seen = clocks.stop() if clocks else None
+    launches = (b2g.get_option("launches") - launches0) * args.steps // (args.steps + args.warmup)
+    alone = {name: 1e3 * timed([f], args.steps) for name, f in parts}
+    # first token's outputs against 64 bits from the 8-bit operands
+    ref = (a[:1].float().double() * sa[:1].double()) @ (Wq.float().double() * Ws.double()[:, None]).t()
+    bad = int(((y[:1].double() - ref).abs() > 2 ** -7 * ref.abs() + 1e-3).sum())
+    flops = 2 * 2.0 * M * N * K
+    peaks, src = measured_peaks()
+    target = (0.5 * flops / (2 * peaks["bf16_tflops"]) + 0.5 * flops / peaks["bf16_tflops"]) * 1e-9
+    print(json.dumps({
+        "metric": "linear_q8_train_step_tflops_%dx%dx%d" % (M, N, K), "value": flops / ms * 1e-9,
+        "unit": "TFLOP/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": ms,
+        "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
+        "dtype": "%s operands, %s sums, bf16 activations and gradients, f32 weight gradient" % (
+            args.dtype if q == b2g.DTYPE_E4M3 else "i8", "f32" if q == b2g.DTYPE_E4M3 else "i32"),
+        "data": "synthetic: seeded normal activations, weights and gradients",
+        "config": {"workload": "training step of an 8-bit linear layer behind an RMS norm", "tokens": M,
+                   "out": N, "in": K, "l2": "operands and results over 126 MB: no flush needed"},
+        "us_alone": alone,
+        "roofline": {"bound": "tensor", "target_ms": target, "frac": target / ms,
+                     "peak_source": "%s bf16_tflops for the weight gradient, twice that for the 8-bit product" % src},
+        "token0_out_of_tolerance": bad, "device_status": b2g.device_status(), "clocks": seen,
+        "gpu_launches": launches}), flush=True)
     return 0
 
 

@@ -603,3 +603,19 @@ def test_generic_products_agree(b2g, cuda):
         check_wgrad(cuda, b2g, 100, 70, 130, BF16, I8, F32, 3, True)
         check_wgrad(cuda, b2g, 100, 70, 130, F16, E4M3, F16, 0)
         assert b2g.last_path() == b2g.PATH_GENERIC
+
+
+def test_bench_runs_the_layer():
+    """bench.py --workload linear_q8 (the operators one after the other) runs and its output is sound."""
+    import json
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    for dt in ("i8", "e4m3"):
+        run = subprocess.run([sys.executable, os.path.join(ROOT, "bench.py"), "--workload", "linear_q8", "--dtype", dt,
+                              "--shape", "256,512,640", "--steps", "3", "--warmup", "3", "--kernel-only"],
+                             capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0, run.stderr[-2000:]
+        line = json.loads(run.stdout.strip().splitlines()[-1])
+        assert line["token0_out_of_tolerance"] == 0 and line["device_status"] == 0 and line["gpu_launches"] >= 15

@@ -598,8 +598,9 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
     const cudaError_t e = cudaMemsetAsync(p.counters, 0, ctr, stream);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync(split-K counters)");
   }
-  // parallel fix-up only when each CTA group holds at most one split unit (all of them then run
-  // at the same time, so their mutual waits always end)
+  // parallel fix-up only when each CTA group holds at most one split unit: all of them then run at the
+  // same time and wait for one another.  Without a cluster that co-schedules them the launch is
+  // cooperative, so that no other stream's kernels can hold a part of the SMs it needs.
   const int groups = p.cluster_fixup ? p.num_units
                                      : std::max(1, std::min(group_cap, p.num_units / p.k_parts));
   p.fixup_parallel = p.k_splits > 1 && p.num_full % groups == 0 && p.num_units - p.num_full <= groups &&
@@ -618,7 +619,11 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
-  if (opt.pdl) {
+  if (p.fixup_parallel && !p.cluster_fixup) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeCooperative;
+    attr[cfg.numAttrs].val.cooperative = 1;
+    ++cfg.numAttrs;
+  } else if (opt.pdl) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;

@@ -595,6 +595,51 @@ def test_layer_step_eager_captured_and_on_two_streams(b2g, cuda, M, D, F, q):
     del graphs
 
 
+def test_split_products_of_several_streams_at_once(b2g, cuda):
+    """Products whose CTAs wait for one another (K split over them), of different tiles and sizes, queued on four
+    streams at once and replayed from four graphs at once: no wait runs out and no value changes."""
+    torch = cuda
+    shapes = [(300, 5000, 4096), (1000, 1304, 2064), (520, 2048, 4096), (2000, 5120, 4096)]
+    prods = []
+    for i, (M, N, K) in enumerate(shapes):
+        A, B = (q8_matrix(torch, r, K, I8, seed)[0] for r, seed in ((M, 10 + i), (N, 20 + i)))
+        prods.append((A, B, torch.empty(M, N, device="cuda"), M, N, K))
+    def run(p, st=None):
+        b2g.gemm_q8(p[0], p[1], p[2], *p[3:], stream=st)
+    for fix in ({}, {"cluster_fixup": 0}):
+        with options(b2g, **fix):
+            want = []
+            for p in prods:
+                run(p)
+                want.append(p[2].clone())
+            streams = [torch.cuda.Stream() for _ in prods]
+            graphs = []
+            for p, st in zip(prods, streams):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=st):
+                    for _ in range(5):
+                        run(p)
+                graphs.append(g)
+            for p in prods:
+                p[2].zero_()
+            torch.cuda.synchronize()
+            for _ in range(8):
+                for p, st in zip(prods, streams):
+                    run(p, st)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p[2], w) for p, w in zip(prods, want))
+            for p in prods:
+                p[2].zero_()
+            torch.cuda.synchronize()
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p[2], w) for p, w in zip(prods, want))
+            assert b2g.device_status() == 0
+            del graphs
+
+
 def test_generic_products_agree(b2g, cuda):
     """option force_generic: the products' generic kernels meet the same bounds."""
     with options(b2g, force_generic=1):

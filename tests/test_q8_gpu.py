@@ -640,6 +640,54 @@ def test_split_products_of_several_streams_at_once(b2g, cuda):
             del graphs
 
 
+@pytest.mark.parametrize("more", [16, 3], ids=["aligned", "odd"])
+def test_offsets_past_32_bits(b2g, cuda, more):
+    """Rows 2^27 elements apart: every operator gives what it gives for rows close together, bit for bit."""
+    torch = cuda
+    D, M, N, K = dict(device="cuda"), 20, 300, 320
+    def placed(pitch):
+        """x's values at that pitch (one buffer per name and element size, never filled as a whole)."""
+        bufs = {}
+        def place(x, name):
+            key = (name, x.dtype.itemsize)
+            if key not in bufs:
+                bufs[key] = torch.empty((M - 1) * pitch * x.dtype.itemsize + 4096, dtype=torch.uint8, **D)
+            v = bufs[key][:bufs[key].numel() // 16 * 16].view(x.dtype).as_strided(x.shape, (pitch, 1))
+            v.copy_(x)
+            return v
+        return place
+    x = rows(torch, M, K, 1).to(torch.bfloat16)
+    w = torch.randn(K, **D)
+    _, wq = q8_matrix(torch, M, K, I8, 5)  # (20 output channels: weights at the wide pitch too)
+    dy = torch.randn(M, N, **D).to(torch.bfloat16)
+    def step(place):
+        h, q = place(torch.zeros_like(x), "h"), place(torch.zeros(M, K, dtype=torch.int8, **D), "q")
+        s, rstd, dw = torch.empty(M, **D), torch.empty(M, **D), torch.empty(K, **D)
+        b2g.rmsnorm_q8(place(x, "x"), w, q, s, M, K, dtype=BF16, w_dtype=F32, H=h, rstd=rstd, pow2=True)
+        q2 = place(torch.zeros(M, K, dtype=torch.int8, **D), "q2")
+        b2g.quantize_q8(h, q2, s.clone(), M, K, dtype=BF16, pow2=True)
+        v = place(torch.zeros_like(x), "x")
+        b2g.dequantize_q8(q, s, v, M, K, dtype=BF16)
+        c = []
+        for m in (4, M):
+            out = place(torch.zeros(M, M, dtype=torch.bfloat16, **D), "c")
+            b2g.gemm_q8(q, place(wq, "w"), out, m, M, K, a_scale=s, c_dtype=BF16)
+            c.append(out.clone())
+        many = torch.zeros(300, K, dtype=torch.int8, **D).random_(-128, 128, generator=torch.Generator(device="cuda").manual_seed(9))
+        ct = torch.empty(300, M, **D)
+        b2g.gemm_q8(many, place(wq, "w"), ct, 300, M, K)
+        g = place(torch.zeros(M, K, **D), "g")
+        y = place(dy, "c")
+        b2g.wgrad_q8(y, q, s, g, M, M, K)
+        d = place(torch.zeros_like(x), "x")
+        b2g.rmsnorm_bwd_q8(place(rows(torch, M, K, 3).to(torch.bfloat16), "d"), q, s, w, rstd, d, dw, M, K, w_dtype=F32)
+        return [t.clone() for t in (h, q, s, rstd, q2, v, *c, ct, g, d, dw)]
+    near = step(placed(K + more))
+    wide = step(placed((1 << 27) + more))
+    assert b2g.device_status() == 0
+    assert all(torch.equal(a, b) for a, b in zip(near, wide))
+
+
 def test_generic_products_agree(b2g, cuda):
     """option force_generic: the products' generic kernels meet the same bounds."""
     with options(b2g, force_generic=1):

@@ -225,8 +225,9 @@ struct FewArgs {
 
 // gemm_q8_few_kernel takes up to 16 tokens where the weights are up to 12 Mi bytes (K a multiple of 16), as
 // measured against gemm_q8_skinny_kernel (us a call, back to back in a graph, int8): 1 token, N x K =
-// 1024 x 4096 2.7 against 5.2, 8192 x 1024 2.5 against 5.1, 4096 x 4096 6.0 against 6.2, 8192 x 8192
-// 15.5 against 13.8; 16 tokens, 2048 x 2048 3.3 against 6.7, 4096 x 4096 7.6 against 7.1.
+// 1024 x 4096 2.7 against 5.4, 8192 x 1024 2.7 against 4.6, 4096 x 2048 2.8 against 5.4, 8192 x 8192
+// 15.5 against 14.0; 16 tokens, 2048 x 2048 3.3 against 5.5, 4096 x 2048 3.3 against 5.6, 4096 x 4096
+// 7.6 against 6.8.
 bool is_few(const FewArgs& a) { return a.M <= 16 && a.K % 16 == 0 && a.N * a.K <= (int64_t)12 << 20; }
 
 // Warps of a block: as many (4 to 16) as give the GPU about 16 an SM, each with a whole turn of K.
@@ -641,10 +642,11 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
 }
 
 // ------------------------------------------------------------------ decoding batches
-// Up to this many tokens run on gemm_q8_skinny_kernel.  Measured against the tiles of larger batches (us a
-// call, back to back in a graph, int8, N = K = 8192): 1 token 13.8 against 24.0, 32 tokens 15.7
-// against 23.9, 64 tokens 17.7 against 23.9, 128 tokens 21.7 against 24.3; 10240 x 8192, 43 tokens
-// 19.7 against 27.3; 28672 x 8192, 128 tokens 48.7 against 53.0.
+// Up to this many tokens (the kernel's most columns) run on gemm_q8_skinny_kernel.  Measured against the
+// tiles of larger batches (us a call, back to back in a graph, int8, N = K = 8192): 1 token 14.0
+// against 23.6, 32 tokens 15.0 against 23.5, 64 tokens 16.3 against 23.6, 128 tokens 19.1 against
+// 24.1; 10240 x 8192, 43 tokens 18.2 against 26.8; 28672 x 8192, 128 tokens 46.3 against 53.7;
+// 1024 x 1024, 128 tokens 6.5 against 7.4.
 constexpr int64_t kSkinnyTokens = 128;
 
 template <bool I8, int NT>

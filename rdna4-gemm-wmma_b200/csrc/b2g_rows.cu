@@ -32,8 +32,9 @@ using namespace q8;
 constexpr int ERR_WAIT_ROW = 8;  // a row's bulk copy did not arrive
 
 constexpr int kRowThreads = 256;
+constexpr int kLongThreads = 512;  // of a block that passes twice over a long row
 
-// Sum (or integer maximum) over the block, returned to every thread.  `buf` holds one word per
+// Sum over the block, returned to every thread.  `buf` holds one word per
 // warp; the leading barrier lets consecutive calls share it.
 __device__ __forceinline__ float block_sum(float v, float* buf) {
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -42,16 +43,6 @@ __device__ __forceinline__ float block_sum(float v, float* buf) {
   __syncthreads();
   float s = 0.0f;
   for (int i = 0; i < (int)blockDim.x / 32; ++i) s += buf[i];
-  return s;
-}
-
-__device__ __forceinline__ uint32_t block_max(uint32_t v, float* buf) {
-  for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = __uint_as_float(v);
-  __syncthreads();
-  uint32_t s = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) s = max(s, __float_as_uint(buf[i]));
   return s;
 }
 
@@ -81,12 +72,13 @@ __device__ __forceinline__ void from_f(float* d, float v) { *d = v; }
 
 // Elements [n, n + VEC) of a row of N (a multiple of VEC), zeros past the row.  One predicated load: a
 // branch with an element-wise end would make every load wait for the one before it.
-template <typename T, int VEC>
+// AGAIN: the row is read once more (otherwise it must not displace the weights from L1).
+template <typename T, int VEC, bool AGAIN = false>
 __device__ __forceinline__ Vec<T, VEC> load_vec(const T* row, int n, int N) {
   Vec<T, VEC> v;
-  if constexpr (sizeof(v) == 16) {  // read once: do not displace the weights from L1
+  if constexpr (sizeof(v) == 16) {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (n < N) u = __ldcs(reinterpret_cast<const uint4*>(row + n));
+    if (n < N) u = AGAIN ? *reinterpret_cast<const uint4*>(row + n) : __ldcs(reinterpret_cast<const uint4*>(row + n));
     *reinterpret_cast<uint4*>(&v) = u;
   } else if constexpr (sizeof(v) == 8) {
     uint2 u = make_uint2(0, 0);
@@ -541,37 +533,84 @@ __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
-// The same for rows too long for a block's registers: two passes over the row, element by element.
-__global__ void __launch_bounds__(kRowThreads) long_rows_to_q8_kernel(const NormArgs a) {
-  __shared__ float buf[kRowThreads / 32];
-  for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
-    auto value = [&](int64_t n) {
-      float h = load_elem(a.X, m * a.ldx + n, a.dtype);
-      if (a.R) h += load_elem(a.R, m * a.ldr + n, a.dtype);
-      return h;
+// The same for rows too long for a block's registers (over 32768 16-bit or 16384 fp32 elements, aligned; over
+// 16384, unaligned): two passes over the row, the second from L2.  Bound by its loads' latency: bf16,
+// quantize 8192 x 40000 220 us (4.5 TB/s), norm with residual 8192 x 40960 858 us (2.7 TB/s).
+template <typename T, bool NORM, int VEC>
+__global__ void __launch_bounds__(kLongThreads, NORM ? 1 : 2) long_rows_to_q8_kernel(const NormArgs a) {
+  constexpr int P = VEC == 1 ? 8 : NORM ? 2 : 4;  // vectors a thread has in flight
+  constexpr int SPAN = kLongThreads * VEC * P;
+  __shared__ float buf[128];
+  const int tid = (int)threadIdx.x;
+  const bool wvec = NORM && weights_vec(a.W, a.w_dtype);
+  int parity = 0;
+  for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x, parity ^= 1) {
+    const T* X = static_cast<const T*>(a.X) + m * a.ldx;
+    const T* R = NORM && a.R ? static_cast<const T*>(a.R) + m * a.ldr : nullptr;
+    // h of the SPAN elements from n0 on (zeros past the row), and with the norm h * w
+    auto take = [&](int64_t n0, int left, float (&h)[P][VEC], float (&v)[P][VEC]) {
+      Vec<T, VEC> x[P], r[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) x[i] = load_vec<T, VEC, true>(X + n0, (i * kLongThreads + tid) * VEC, left);
+      if (R)
+#pragma unroll
+        for (int i = 0; i < P; ++i) r[i] = load_vec<T, VEC, true>(R + n0, (i * kLongThreads + tid) * VEC, left);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[i][j] = to_f(x[i].e[j]);
+        if (R)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) h[i][j] += to_f(r[i].e[j]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = h[i][j];
+        if constexpr (NORM) {
+          float w[VEC];
+          const char* wp = static_cast<const char*>(a.W) + n0 * (a.w_dtype == B2G_DTYPE_F32 ? 4 : 2);
+          load_weights<VEC>(wp, a.w_dtype, wvec, (i * kLongThreads + tid) * VEC, left, w);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[i][j] *= w[j];
+        }
+      }
     };
-    float ss = 0.0f;
-    uint32_t top = 0;
-    for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) {
-      const float h = value(n);
-      const float v = a.norm ? h * load_elem(a.W, n, a.w_dtype) : h;
-      ss = fmaf(h, h, ss);
-      top = max(top, __float_as_uint(v) & 0x7fffffffu);
+    float ss = 0.0f, ftop = 0.0f;
+    for (int64_t n0 = 0; n0 < a.N; n0 += SPAN) {
+      float h[P][VEC], v[P][VEC];
+      take(n0, (int)min(a.N - n0, (int64_t)SPAN), h, v);
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          if constexpr (NORM) ss = fmaf(h[i][j], h[i][j], ss);
+          ftop = max_abs(ftop, v[i][j]);
+        }
     }
-    top = block_max(top, buf);
-    float rstd = 1.0f;
-    if (a.norm) rstd = 1.0f / sqrtf(block_sum(ss, buf) / (float)a.N + a.eps);
+    uint32_t top = __float_as_uint(ftop);
+    row_reduce<0, NORM>(ss, top, buf, parity);
+    const float rstd = NORM ? 1.0f / sqrtf(ss / (float)a.N + a.eps) : 1.0f;
     const RowQuant rq = row_quant(top, rstd, q_max(a.q_dtype), a.pow2);
-    if (threadIdx.x == 0) {
+    if (tid == 0) {
       a.scale[m] = rq.scale;
-      if (a.rstd) a.rstd[m] = rstd;
+      if (NORM && a.rstd) a.rstd[m] = rstd;
     }
     const bool bad = rq.scale != rq.scale;
-    for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) {
-      const float h = value(n);
-      const float v = a.norm ? h * load_elem(a.W, n, a.w_dtype) : h;
-      static_cast<uint8_t*>(a.Q)[m * a.ldq + n] = bad ? 0 : (uint8_t)to_q8(quotient(v, rq), a.q_dtype);
-      if (a.H) store_elem(a.H, m * a.ldh + n, a.dtype, h);
+    for (int64_t n0 = 0; n0 < a.N; n0 += SPAN) {
+      const int left = (int)min(a.N - n0, (int64_t)SPAN);
+      float h[P][VEC], v[P][VEC];
+      take(n0, left, h, v);
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int n = (i * kLongThreads + tid) * VEC;
+        Vec<uint8_t, VEC> o;
+        pack_q8<VEC>(v[i], rq, a.q_dtype, bad, o.e);
+        store_vec<uint8_t, VEC>(static_cast<uint8_t*>(a.Q) + m * a.ldq + n0, n, left, o);
+        if (NORM && a.H) {
+          Vec<T, VEC> x;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) from_f(&x.e[j], h[i][j]);
+          store_vec<T, VEC>(static_cast<T*>(a.H) + m * a.ldh + n0, n, left, x);
+        }
+      }
     }
   }
 }
@@ -664,28 +703,80 @@ struct BwdArgs {
   int dtype, x_dtype, w_dtype;
 };
 
-// One block per row: mean(g * xh), then dx.
-__global__ void __launch_bounds__(kRowThreads) rmsnorm_bwd_kernel(const BwdArgs a) {
-  __shared__ float buf[kRowThreads / 32];
+// Any size, alignment and checkpoint type, one block a row at a time, element by element: mean(g * xh), then
+// dx, the second pass from L2.  X8: 8-bit checkpoint; else any 16- or 32-bit type.  The block's share of dw
+// is added up in its row of partial sums.  Bound by its loads' latency (bf16, int8 checkpoint: 2048 x
+// 32768 404 us, 4096 x 9001 215 us).
+
+template <typename T, bool X8>
+__global__ void __launch_bounds__(kLongThreads, 2) rmsnorm_bwd_kernel(const BwdArgs a) {
+  constexpr int P = 8, SPAN = kLongThreads * P;  // elements a thread has in flight
+  __shared__ float buf[kLongThreads / 32];
+  const int tid = (int)threadIdx.x;
   for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
-    const float rstd = a.rstd[m];
-    const float xs = a.x_scale ? a.x_scale[m] : 1.0f;
+    const float rstd = __ldg(a.rstd + m), xs = a.x_scale ? __ldg(a.x_scale + m) * rstd : rstd;
+    const T* dY = static_cast<const T*>(a.dY) + m * a.ldy;
+    // dy, w and xh of the SPAN elements from n0 on (zeros past the row)
+    auto take = [&](int64_t n0, int left, float (&dy)[P], float (&w)[P], float (&xh)[P]) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) dy[i] = to_f(load_vec<T, 1>(dY + n0, i * kLongThreads + tid, left).e[0]);
+      if constexpr (X8) {
+        const uint8_t* X = static_cast<const uint8_t*>(a.X) + m * a.ldx + n0;
+        uint8_t b[P];
+#pragma unroll
+        for (int i = 0; i < P; ++i) b[i] = load_vec<uint8_t, 1>(X, i * kLongThreads + tid, left).e[0];
+#pragma unroll
+        for (int i = 0; i < P; ++i) xh[i] = load_elem(&b[i], 0, a.x_dtype);
+      } else {
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const int n = i * kLongThreads + tid;
+          xh[i] = n < left ? load_elem(a.X, m * a.ldx + n0 + n, a.x_dtype) : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        float f[1];
+        load_weights<1>(static_cast<const char*>(a.W) + n0 * (a.w_dtype == B2G_DTYPE_F32 ? 4 : 2), a.w_dtype, false,
+                        i * kLongThreads + tid, left, f);
+        w[i] = f[0];
+        xh[i] *= xs;
+      }
+    };
     float c = 0.0f;
-    for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) {
-      const float xh = load_elem(a.X, m * a.ldx + n, a.x_dtype) * xs * rstd;
-      c = fmaf(load_elem(a.dY, m * a.ldy + n, a.dtype) * load_elem(a.W, n, a.w_dtype), xh, c);
+    for (int64_t n0 = 0; n0 < a.N; n0 += SPAN) {
+      const int left = (int)min(a.N - n0, (int64_t)SPAN);
+      float dy[P], w[P], xh[P];
+      take(n0, left, dy, w, xh);
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+        if (i * kLongThreads + tid < left) c = fmaf(dy[i] * w[i], xh[i], c);
     }
     c = block_sum(c, buf) / (float)a.N;
-    for (int64_t n = threadIdx.x; n < a.N; n += blockDim.x) {
-      const float xh = load_elem(a.X, m * a.ldx + n, a.x_dtype) * xs * rstd;
-      const float dy = load_elem(a.dY, m * a.ldy + n, a.dtype);
-      float dx = rstd * (dy * load_elem(a.W, n, a.w_dtype) - xh * c);
-      if (a.dR) dx += load_elem(a.dR, m * a.ldr + n, a.dtype);
-      if (a.part) {
-        float* p = a.part + (int64_t)blockIdx.x * a.N + n;
-        *p = (m == blockIdx.x ? 0.0f : *p) + dy * xh;
+    for (int64_t n0 = 0; n0 < a.N; n0 += SPAN) {
+      const int left = (int)min(a.N - n0, (int64_t)SPAN);
+      float dy[P], w[P], xh[P], dr[P], dw[P];
+      float* part = a.part ? a.part + (int64_t)blockIdx.x * a.N + n0 : nullptr;
+      take(n0, left, dy, w, xh);
+      if (a.dR) {
+        const T* dR = static_cast<const T*>(a.dR) + m * a.ldr + n0;
+#pragma unroll
+        for (int i = 0; i < P; ++i) dr[i] = to_f(load_vec<T, 1>(dR, i * kLongThreads + tid, left).e[0]);
       }
-      store_elem(a.dX, m * a.lddx + n, a.dtype, dx);
+      const bool add = part && m != blockIdx.x;
+#pragma unroll
+      for (int i = 0; i < P; ++i) dw[i] = add ? load_vec<float, 1>(part, i * kLongThreads + tid, left).e[0] : 0.0f;
+      T* dX = static_cast<T*>(a.dX) + m * a.lddx + n0;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int n = i * kLongThreads + tid;
+        if (n < left) {
+          float dx = rstd * (dy[i] * w[i] - xh[i] * c);
+          if (a.dR) dx += dr[i];
+          if (part) part[n] = fmaf(dy[i], xh[i], dw[i]);
+          from_f(dX + n, dx);
+        }
+      }
     }
   }
 }
@@ -1009,8 +1100,6 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const float* part, float* 
   }
 }
 
-unsigned row_blocks(int64_t M, int sms) { return (unsigned)std::min<int64_t>(M, (int64_t)sms * 8); }
-
 // Checks that every row operator shares: extents and leading dimensions.
 int check_rows(int64_t M, int64_t N, std::initializer_list<int64_t> lds) {
   if (M < 0 || N < 0) return fail(B2G_ERR_INVALID_ARG, "negative dimension");
@@ -1063,8 +1152,11 @@ int raise_smem(F fn, std::atomic<uint64_t>& ready) {
   return e == cudaSuccess ? (int)B2G_OK : cuda_fail(e, "cudaFuncSetAttribute(smem)");
 }
 
-// A launch of rows_ring_kernel, or false where its stages do not fit or a block would have too few
-// rows for the ring to matter.
+// A launch of rows_ring_kernel, or false where its stages do not fit or a block would have too few rows (one
+// with the norm, two without) for the ring to pay.  Against rows_to_q8_kernel (us, bf16, graph): norm with
+// residual, 8192 rows of 8192 81 against 151, 16384 of 1024 27 against 51, 1000 of 4096 11.4 against
+// 13.4, 296 of 8192 7.2 against 8.1, but 296 of 4096 4.8 against 3.9; quantize, 16384 of 8192 78
+// against 99, 1000 of 4096 4.2 against 4.5, but 444 of 16384 8.6 against 6.6.
 template <typename T, bool NORM, int V, int THREADS, int CTAS>
 bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   const uint32_t row_bytes = (uint32_t)(a.N * (int64_t)sizeof(T));
@@ -1072,7 +1164,9 @@ bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   const int64_t nv = a.N * (int64_t)sizeof(T) / 16;
   const int threads = (int)((nv + V * 32 - 1) / (V * 32)) * 32;
   int ctas = 0, stages = 0;  // (blocks of fewer threads than THREADS leave registers for more of them)
-  if (!ring_shape(stage, THREADS * CTAS / threads, &ctas, &stages) || a.M < (int64_t)sms * ctas * 2) return false;
+  if (!ring_shape(stage, THREADS * CTAS / threads, &ctas, &stages) ||
+      a.M < (int64_t)sms * ctas * (NORM ? 1 : 2))
+    return false;
   auto fn = rows_ring_kernel<T, NORM, V, THREADS, CTAS>;
   static std::atomic<uint64_t> ready{0};
   *rc = raise_smem(fn, ready);
@@ -1139,7 +1233,11 @@ int rows_of(const NormArgs& a, int sms, cudaStream_t s) {
                           : false)
       return rc;
   }
-  long_rows_to_q8_kernel<<<row_blocks(a.M, sms), kRowThreads, 0, s>>>(a);
+  const unsigned blocks = (unsigned)std::min<int64_t>(a.M, (int64_t)sms * 2);  // (what is resident at once)
+  if (vec)
+    long_rows_to_q8_kernel<T, NORM, VEC><<<blocks, kLongThreads, 0, s>>>(a);
+  else
+    long_rows_to_q8_kernel<T, NORM, 1><<<blocks, kLongThreads, 0, s>>>(a);
   return launched("long_rows_to_q8_kernel");
 }
 
@@ -1226,7 +1324,7 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
   const bool elems = !ring && (x8 || same) && a.N >= 16 && a.N <= 8192 &&
                      ring_shape((a.dR ? 2 : 1) * y_slot + x_slot, ectas, &ectas, &estages);
   const unsigned blocks = ring || elems ? (unsigned)std::min<int64_t>(a.M, (int64_t)sms * (ring ? ctas : ectas))
-                                        : row_blocks(a.M, sms);
+                                        : (unsigned)std::min<int64_t>(a.M, (int64_t)sms * 2);
   Workspace ws(s);
   int rc = B2G_OK;
   if (dw) {
@@ -1238,7 +1336,10 @@ int bwd_of(BwdArgs a, bool x8, bool same, float* dw, int sms, cudaStream_t s) {
     rc = x8 ? bwd_elems<T, true>(a, ethreads, blocks, estages, y_slot, x_slot, s)
             : bwd_elems<T, false>(a, ethreads, blocks, estages, y_slot, x_slot, s);
   } else if (!ring) {
-    rmsnorm_bwd_kernel<<<blocks, kRowThreads, 0, s>>>(a);
+    if (x8)
+      rmsnorm_bwd_kernel<T, true><<<blocks, kLongThreads, 0, s>>>(a);
+    else
+      rmsnorm_bwd_kernel<T, false><<<blocks, kLongThreads, 0, s>>>(a);
     rc = launched("rmsnorm_bwd_kernel");
   } else if (hold) {
     rc = x8 ? launch_bwd_ring<T, true, V, true>(a, threads, blocks, stages, s)

@@ -199,6 +199,15 @@ def test_norm_weight_types_in_place_and_eps(b2g, cuda, w_dt):
     check_norm(cuda, b2g, 9, 1031, F16, E4M3, True, False, 0, w_dt=w_dt, inplace=True, eps=0.0)
 
 
+@pytest.mark.parametrize("q", [I8, E4M3], ids=NAMES.get)
+@pytest.mark.parametrize("dt", [F16, BF16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("M,N,pad", [(5, 40960, 0), (400, 33024, 8), (5, 33003, 5), (310, 20001, 1)])
+def test_norm_long_rows(b2g, cuda, M, N, pad, dt, q):
+    """Rows too long for registers, with and without a residual, more rows than blocks among them."""
+    check_norm(cuda, b2g, M, N, dt, q, res=True, pow2=False, pad=pad, inplace=pad == 8)
+    check_norm(cuda, b2g, M, N, dt, q, res=False, pow2=True, pad=pad)
+
+
 def test_norm_zero_and_bad_rows(b2g, cuda):
     """A row of zeros gives rstd = 1/sqrt(eps), the least scale and zeros; a NaN or infinity stays
     in its row."""
@@ -470,6 +479,14 @@ def test_norm_backward_variants(b2g, cuda, w_dt):
     check_bwd(cuda, b2g, 40, 1032, BF16, I8, True, 8, w_dt=w_dt, inplace=True)
     check_bwd(cuda, b2g, 40, 1031, F16, E4M3, False, 0, w_dt=w_dt, inplace=True)
     check_bwd(cuda, b2g, 40, 2048, BF16, F16, True, 0, w_dt=w_dt, want_dw=False)
+
+
+@pytest.mark.parametrize("xt", [I8, E4M3, BF16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("M,N,pad", [(3, 40960, 0), (330, 16640, 8), (5, 33003, 5), (310, 9001, 1), (320, 7, 0)])
+def test_norm_backward_long_and_short_rows(b2g, cuda, M, N, pad, xt):
+    """Rows too long, too short or of other types than the ring kernels take, more rows than blocks among them."""
+    check_bwd(cuda, b2g, M, N, BF16, xt, True, pad)
+    check_bwd(cuda, b2g, M, N, F32, xt, False, pad)
 
 
 def test_norm_backward_no_tokens(b2g, cuda):

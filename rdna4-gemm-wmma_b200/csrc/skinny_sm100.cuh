@@ -10,6 +10,10 @@
 // K is split over the CTAs of a cluster.  Each leaves its accumulator in its (idle) stages, and CTA r of
 // S sums columns r, r + S, ... of all of them through distributed shared memory in rank order.
 //
+// Measured (graph, int8): 1 x 8192 x 8192 14.0 us (4.8 TB/s), 43 x 10240 x 8192 18.2 us (4.6 TB/s), 32 x
+// 28672 x 8192 40.1 us (5.9 TB/s), 128 x 28672 x 8192 46.3 us (5.2 TB/s).  A short product's fixed cost
+// (set-up, first loads, epilogue: about 5 us) is what keeps it off the memory's rate.
+//
 // Nothing overlaps the epilogue, and a warp alone on its scheduler issues an instruction every few
 // cycles: so eight warps share it, and loads from several CTAs are in flight together.
 #pragma once

@@ -420,6 +420,21 @@ int b2g_rmsnorm_bwd_q8(const void* dY, const void* X, const float* x_scale, cons
                        int64_t ldy, int64_t ldx, int64_t ldr, int64_t lddx, int dtype, int x_dtype,
                        int w_dtype, void* stream);
 
+/*
+ * The six calls above from an array of 64-bit words, for callers whose foreign-function interface pays
+ * per argument: `args` holds the arguments of the call that `call` names, in order, one word each
+ * (pointers and integers as integers, eps as a double).  Reads exactly that call's arguments.
+ */
+enum {
+  B2G_CALL_QUANTIZE_Q8 = 0,    /* 11 words */
+  B2G_CALL_DEQUANTIZE_Q8 = 1,  /* 10 */
+  B2G_CALL_RMSNORM_Q8 = 2,     /* 19, eps the 17th */
+  B2G_CALL_GEMM_Q8 = 3,        /* 15 */
+  B2G_CALL_WGRAD_Q8 = 4,       /* 15 */
+  B2G_CALL_RMSNORM_BWD_Q8 = 5, /* 18 */
+};
+int b2g_call_q8(int call, const void* args);
+
 /* Balanced contiguous row partition: rank r gets M/world rows, the first M%world ranks one more.
  * No reference counterpart (the reference is single-GPU). */
 int b2g_slab_rows(int64_t M, int world, int rank, int64_t* row0, int64_t* rows);

@@ -11,6 +11,7 @@ and every call goes to the CUDA kernels.
 import ctypes
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -153,6 +154,8 @@ def load(path=None):
     L.b2g_wgrad_q8.argtypes = [vp] * 4 + [i64] * 6 + [c_int] * 4 + [vp]
     L.b2g_rmsnorm_bwd_q8.restype = c_int
     L.b2g_rmsnorm_bwd_q8.argtypes = [vp] * 8 + [i64] * 6 + [c_int] * 3 + [vp]
+    L.b2g_call_q8.restype = c_int
+    L.b2g_call_q8.argtypes = [c_int, ctypes.c_char_p]
     if path is None:
         _lib = L
     return L
@@ -486,7 +489,7 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
     that the call names and on the current device, and a row-major matrix of that size at least,
     whose row stride is the default leading dimension."""
     if x is None or isinstance(x, int) or _torch is None or not isinstance(x, _torch.Tensor):
-        return _ptr(x), (cols or 1) if ld is None else ld
+        return _ptr(x) or 0, (cols or 1) if ld is None else ld
     if x.get_device() != dev or x.dtype not in _torch_types.get(dtype, ()):
         _wrong_tensor(x, dtype, what)
     if ld is None:
@@ -506,7 +509,7 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
 def _vector(x, dtype, what, n, dev):
     """Pointer of a vector of n contiguous values (None: an optional one that is not given)."""
     if x is None or isinstance(x, int) or _torch is None or not isinstance(x, _torch.Tensor):
-        return _ptr(x)
+        return _ptr(x) or 0
     if x.get_device() != dev or x.dtype not in _torch_types.get(dtype, ()):
         _wrong_tensor(x, dtype, what)
     if x.numel() < n or not x.is_contiguous():
@@ -519,7 +522,17 @@ def _stream_of(stream, dev):
     costs as much as the launch)."""
     if stream is None and dev is not None and _raw_stream is not None:
         return _raw_stream(dev)
-    return _stream(stream)
+    return _stream(stream) or 0
+
+
+def _call(call, words, *args):
+    """One of the six operators, its arguments packed into 64-bit words: ctypes converts each argument
+    of a call on its own, which costs more than the launch."""
+    _check(load().b2g_call_q8(call, words(*args)))
+
+
+_WORDS = {n: struct.Struct("%dq" % n).pack for n in (10, 11, 15, 18)}
+_NORM_WORDS = struct.Struct("16qd2q").pack
 
 
 def quantize_q8(X, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, pow2=False, ldx=None,
@@ -530,8 +543,7 @@ def quantize_q8(X, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, pow2=False
     x, ldx = _matrix(X, dtype, "X", M, N, ldx, dev)
     q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
     s = _vector(scale, DTYPE_F32, "scale", M, dev)
-    _check(load().b2g_quantize_q8(x, q, s, M, N, ldx, ldq, dtype, q_dtype, 1 if pow2 else 0,
-                                  _stream_of(stream, dev)))
+    _call(0, _WORDS[11], x, q, s, M, N, ldx, ldq, dtype, q_dtype, 1 if pow2 else 0, _stream_of(stream, dev))
 
 
 def dequantize_q8(Q, scale, X, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, ldq=None, ldx=None,
@@ -541,7 +553,7 @@ def dequantize_q8(Q, scale, X, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, ldq=None
     q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
     s = _vector(scale, DTYPE_F32, "scale", M, dev)
     x, ldx = _matrix(X, dtype, "X", M, N, ldx, dev)
-    _check(load().b2g_dequantize_q8(q, s, x, M, N, ldq, ldx, q_dtype, dtype, _stream_of(stream, dev)))
+    _call(1, _WORDS[10], q, s, x, M, N, ldq, ldx, q_dtype, dtype, _stream_of(stream, dev))
 
 
 def rmsnorm_q8(X, W, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, R=None, H=None, rstd=None,
@@ -558,8 +570,8 @@ def rmsnorm_q8(X, W, Q, scale, M, N, dtype=DTYPE_F16, q_dtype=DTYPE_I8, R=None, 
     q, ldq = _matrix(Q, q_dtype, "Q", M, N, ldq, dev)
     s = _vector(scale, DTYPE_F32, "scale", M, dev)
     rs = _vector(rstd, DTYPE_F32, "rstd", M, dev)
-    _check(load().b2g_rmsnorm_q8(x, r, w, h, q, s, rs, M, N, ldx, ldr, ldh, ldq, dtype, w_dtype,
-                                 q_dtype, float(eps), 1 if pow2 else 0, _stream_of(stream, dev)))
+    _call(2, _NORM_WORDS, x, r, w, h, q, s, rs, M, N, ldx, ldr, ldh, ldq, dtype, w_dtype, q_dtype, eps,
+          1 if pow2 else 0, _stream_of(stream, dev))
 
 
 def gemm_q8(A, B, C, M, N, K, dtype=DTYPE_I8, a_scale=None, b_scale=None, bias=None,
@@ -573,8 +585,7 @@ def gemm_q8(A, B, C, M, N, K, dtype=DTYPE_I8, a_scale=None, b_scale=None, bias=N
     sa = _vector(a_scale, DTYPE_F32, "a_scale", M, dev)
     sb = _vector(b_scale, DTYPE_F32, "b_scale", N, dev)
     bi = _vector(bias, DTYPE_F32, "bias", N, dev)
-    _check(load().b2g_gemm_q8(a, b, c, M, N, K, lda, ldb, ldc, dtype, sa, sb, bi, c_dtype,
-                              _stream_of(stream, dev)))
+    _call(3, _WORDS[15], a, b, c, M, N, K, lda, ldb, ldc, dtype, sa, sb, bi, c_dtype, _stream_of(stream, dev))
 
 
 def wgrad_q8(dY, Q, scale, dW, M, N, K, dtype=DTYPE_BF16, q_dtype=DTYPE_I8, accumulate=False,
@@ -586,8 +597,8 @@ def wgrad_q8(dY, Q, scale, dW, M, N, K, dtype=DTYPE_BF16, q_dtype=DTYPE_I8, accu
     q, ldq = _matrix(Q, q_dtype, "Q", M, K, ldq, dev)
     s = _vector(scale, DTYPE_F32, "scale", M, dev)
     w, ldw = _matrix(dW, c_dtype, "dW", N, K, ldw, dev)
-    _check(load().b2g_wgrad_q8(y, q, s, w, M, N, K, ldy, ldq, ldw, dtype, q_dtype,
-                               1 if accumulate else 0, c_dtype, _stream_of(stream, dev)))
+    _call(4, _WORDS[15], y, q, s, w, M, N, K, ldy, ldq, ldw, dtype, q_dtype, 1 if accumulate else 0, c_dtype,
+          _stream_of(stream, dev))
 
 
 def rmsnorm_bwd_q8(dY, X, x_scale, W, rstd, dX, dw, M, N, dtype=DTYPE_BF16, x_dtype=DTYPE_I8,
@@ -604,8 +615,8 @@ def rmsnorm_bwd_q8(dY, X, x_scale, W, rstd, dX, dw, M, N, dtype=DTYPE_BF16, x_dt
     r, ldr = _matrix(dres, dtype, "dres", M, N, ldr, dev)
     d, lddx = _matrix(dX, dtype, "dX", M, N, lddx, dev)
     g = _vector(dw, DTYPE_F32, "dw", N, dev)
-    _check(load().b2g_rmsnorm_bwd_q8(y, x, xs, w, rs, r, d, g, M, N, ldy, ldx, ldr, lddx, dtype,
-                                     x_dtype, w_dtype, _stream_of(stream, dev)))
+    _call(5, _WORDS[18], y, x, xs, w, rs, r, d, g, M, N, ldy, ldx, ldr, lddx, dtype, x_dtype, w_dtype,
+          _stream_of(stream, dev))
 
 
 def version():

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstring>
 #include <mutex>
 
 #include "../../include/b2g_gemm.h"
@@ -869,4 +870,35 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
   rc = launched("wgrad_q8_generic_kernel");
   if (rc == B2G_OK) set_path(M == 0 ? B2G_PATH_ZERO : B2G_PATH_GENERIC);
   return rc;
+}
+
+extern "C" int b2g_call_q8(int call, const void* args) {
+  clear_error();
+  if (!args) return fail(B2G_ERR_INVALID_ARG, "args is null");
+  const int64_t* a = static_cast<const int64_t*>(args);
+  auto ptr = [a](int i) { return reinterpret_cast<void*>(static_cast<intptr_t>(a[i])); };
+  auto vec = [ptr](int i) { return static_cast<float*>(ptr(i)); };
+  auto num = [a](int i) { return static_cast<int>(a[i]); };
+  switch (call) {
+    case B2G_CALL_QUANTIZE_Q8:
+      return b2g_quantize_q8(ptr(0), ptr(1), vec(2), a[3], a[4], a[5], a[6], num(7), num(8), num(9), ptr(10));
+    case B2G_CALL_DEQUANTIZE_Q8:
+      return b2g_dequantize_q8(ptr(0), vec(1), ptr(2), a[3], a[4], a[5], a[6], num(7), num(8), ptr(9));
+    case B2G_CALL_RMSNORM_Q8: {
+      double eps;
+      std::memcpy(&eps, a + 16, sizeof(eps));
+      return b2g_rmsnorm_q8(ptr(0), ptr(1), ptr(2), ptr(3), ptr(4), vec(5), vec(6), a[7], a[8], a[9], a[10],
+                            a[11], a[12], num(13), num(14), num(15), (float)eps, num(17), ptr(18));
+    }
+    case B2G_CALL_GEMM_Q8:
+      return b2g_gemm_q8(ptr(0), ptr(1), ptr(2), a[3], a[4], a[5], a[6], a[7], a[8], num(9), vec(10), vec(11),
+                         vec(12), num(13), ptr(14));
+    case B2G_CALL_WGRAD_Q8:
+      return b2g_wgrad_q8(ptr(0), ptr(1), vec(2), ptr(3), a[4], a[5], a[6], a[7], a[8], a[9], num(10), num(11),
+                          num(12), num(13), ptr(14));
+    case B2G_CALL_RMSNORM_BWD_Q8:
+      return b2g_rmsnorm_bwd_q8(ptr(0), ptr(1), vec(2), ptr(3), vec(4), ptr(5), ptr(6), vec(7), a[8], a[9],
+                                a[10], a[11], a[12], a[13], num(14), num(15), num(16), ptr(17));
+  }
+  return fail(B2G_ERR_INVALID_ARG, "unknown call %d", call);
 }

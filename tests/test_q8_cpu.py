@@ -61,6 +61,79 @@ def test_refused(b2g, call, bad):
     assert b2g.load().b2g_last_error_string()
 
 
+class Packed:
+    """The library with the six operators called through b2g_call_q8, and the words of the last call."""
+    CALLS = ["b2g_quantize_q8", "b2g_dequantize_q8", "b2g_rmsnorm_q8", "b2g_gemm_q8", "b2g_wgrad_q8",
+             "b2g_rmsnorm_bwd_q8"]
+
+    def __init__(self, b2g):
+        self.lib = b2g.load()
+
+    def load(self):
+        return self
+
+    def __getattr__(self, name):
+        import struct
+        def call(*args):
+            form = "".join("d" if isinstance(a, float) else "q" for a in args)
+            self.words = struct.pack(form, *(a or 0 for a in args))
+            return self.lib.b2g_call_q8(self.CALLS.index(name), self.words)
+        return call
+
+
+@pytest.mark.parametrize("call,bad", REFUSED, ids=["%s-%s" % (c.__name__, "-".join(map(str, k))) for c, k in REFUSED])
+def test_refused_packed(b2g, call, bad):
+    """The packed form refuses what the call itself refuses, with its message."""
+    assert call(b2g, **bad) == b2g.ERR_INVALID_ARG
+    want = b2g.load().b2g_last_error_string()
+    assert call(Packed(b2g), **bad) == b2g.ERR_INVALID_ARG
+    assert b2g.load().b2g_last_error_string() == want
+
+
+def test_packed_calls(b2g):
+    p = Packed(b2g)
+    assert quantize(p, M=0) == b2g.OK and len(p.words) == 8 * 11
+    assert dequantize(p, M=0) == b2g.OK and len(p.words) == 8 * 10
+    assert norm(p, M=0) == b2g.OK and len(p.words) == 8 * 19
+    assert gemm(p, M=0) == b2g.OK and len(p.words) == 8 * 15
+    assert wgrad(p, N=0) == b2g.OK and len(p.words) == 8 * 15
+    assert bwd(p, N=0) == b2g.OK and len(p.words) == 8 * 18
+    assert p.lib.b2g_call_q8(6, p.words) == b2g.ERR_INVALID_ARG
+    assert p.lib.b2g_call_q8(-1, p.words) == b2g.ERR_INVALID_ARG
+    assert p.lib.b2g_call_q8(0, None) == b2g.ERR_INVALID_ARG
+
+
+def test_binding_packs_every_argument_in_its_place(b2g, monkeypatch):
+    """What the binding packs is what the calls take: distinct values, compared word by word."""
+    import struct
+    seen = []
+    class Lib:
+        def b2g_call_q8(self, call, words):
+            seen.append((call, words))
+            return b2g.OK
+    monkeypatch.setattr(b2g, "load", lambda: Lib())
+    monkeypatch.setattr(b2g, "_device", lambda: None)
+    q = lambda *a: struct.pack("%dq" % len(a), *a)
+    b2g.quantize_q8(11, 12, 13, 4, 5, dtype=1, q_dtype=2, pow2=True, ldx=6, ldq=7, stream=99)
+    b2g.dequantize_q8(11, 12, 13, 4, 5, dtype=1, q_dtype=2, ldq=6, ldx=7, stream=99)
+    b2g.rmsnorm_q8(11, 12, 13, 14, 4, 5, dtype=1, q_dtype=2, R=15, H=16, rstd=17, w_dtype=4, eps=0.5, pow2=False,
+                   ldx=21, ldr=22, ldh=23, ldq=24, stream=99)
+    b2g.gemm_q8(11, 12, 13, 4, 5, 6, dtype=2, a_scale=14, b_scale=15, bias=16, c_dtype=1, lda=21, ldb=22, ldc=23, stream=99)
+    b2g.wgrad_q8(11, 12, 13, 14, 4, 5, 6, dtype=0, q_dtype=2, accumulate=True, c_dtype=4, ldy=21, ldq=22, ldw=23, stream=99)
+    b2g.rmsnorm_bwd_q8(11, 12, 13, 14, 15, 16, 17, 4, 5, dtype=0, x_dtype=2, w_dtype=1, dres=18, ldy=21, ldx=22, ldr=23,
+                       lddx=24, stream=99)
+    b2g.gemm_q8(11, 12, 13, 4, 5, 6, stream=99)
+    assert seen == [
+        (0, q(11, 12, 13, 4, 5, 6, 7, 1, 2, 1, 99)),
+        (1, q(11, 12, 13, 4, 5, 6, 7, 2, 1, 99)),
+        (2, q(11, 15, 12, 16, 13, 14, 17, 4, 5, 21, 22, 23, 24, 1, 4, 2) + struct.pack("d", 0.5) + q(0, 99)),
+        (3, q(11, 12, 13, 4, 5, 6, 21, 22, 23, 2, 14, 15, 16, 1, 99)),
+        (4, q(11, 12, 13, 14, 4, 5, 6, 21, 22, 23, 0, 2, 1, 4, 99)),
+        (5, q(11, 12, 13, 14, 15, 18, 16, 17, 4, 5, 21, 22, 23, 24, 0, 2, 1, 99)),
+        (3, q(11, 12, 13, 4, 5, 6, 6, 6, 5, 5, 0, 0, 0, 4, 99)),
+    ]
+
+
 def test_empty_calls_need_no_device(b2g):
     assert quantize(b2g, M=0, X=None, Q=None, s=None) == b2g.OK
     assert dequantize(b2g, M=0, Q=None) == b2g.OK

@@ -386,7 +386,8 @@ int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void* H, void* Q
  * Scaled 8-bit matrix product: C[m,n] = (sum_k A[m*lda+k] * B[n*ldb+k]) * a_scale[m] * b_scale[n]
  * + bias[n].  A is M x K (tokens), B is N x K (one row of weights per output channel), both
  * `dtype` (I8 or E4M3).  int8 products are summed exactly in int32 (K <= 131071, so that no sum
- * overflows), e4m3 products in fp32.  a_scale (M), b_scale (N) and bias (N) are optional fp32
+ * overflows), e4m3 products in fp32 (the tensor core truncates each addition: measured 9.7e-7
+ * relative for 28672 products of one sign, 3.7e-6 for 65536).  a_scale (M), b_scale (N) and bias (N) are optional fp32
  * vectors (NULL: 1, 1 and 0).  C is F32, F16 or BF16, rounded once.
  */
 int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,

@@ -703,6 +703,7 @@ def test_offsets_past_32_bits(b2g, cuda, more):
     wide = step(placed((1 << 27) + more))
     assert b2g.device_status() == 0
     assert all(torch.equal(a, b) for a, b in zip(near, wide))
+    torch.cuda.empty_cache()  # about 40 GB, for the tests that follow
 
 
 def test_generic_products_agree(b2g, cuda):

@@ -8,6 +8,7 @@
 #include "../../include/b2g_gemm.h"
 #include "errors.h"
 #include "host.h"
+#include "plan.h"
 #include "ptx.cuh"
 #include "q8.cuh"
 
@@ -1138,29 +1139,13 @@ int launch_rows(const NormArgs& a, int threads, int sms, cudaStream_t s) {
   return launched("rows_to_q8_kernel");
 }
 
-// Stages and blocks an SM of a ring kernel: as many blocks as `most` if two stages of each fit (one
-// block's copies run while another's row is worked on), then up to four stages.  False where not
-// even two stages of one block fit.
-bool ring_shape(uint32_t stage, int most, int* blocks, int* stages) {
-  constexpr uint32_t kSmem = 224 * 1024;
-  for (int n = most; n >= 1; --n) {
-    const uint32_t fit = (kSmem / n - 2048) / stage;
-    if (fit >= 2) {
-      *blocks = n;
-      *stages = (int)std::min<uint32_t>(4, fit);
-      return true;
-    }
-  }
-  return false;
-}
-
 // Raises a kernel's shared-memory limit once per device.
 template <typename F>
 int raise_smem(F fn, std::atomic<uint64_t>& ready) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && !(ready.load() >> dev & 1)) {
-    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingSmem);
     if (e == cudaSuccess) ready |= 1ull << dev;
   }
   return e == cudaSuccess ? (int)B2G_OK : cuda_fail(e, "cudaFuncSetAttribute(smem)");
@@ -1185,7 +1170,7 @@ bool launch_ring(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   static std::atomic<uint64_t> ready{0};
   *rc = raise_smem(fn, ready);
   if (*rc != B2G_OK) return true;
-  fn<<<(unsigned)(sms * ctas), threads, (uint32_t)stages * (stage + 8), s>>>(
+  fn<<<(unsigned)(sms * ctas), threads, ring_bytes(stages, stage), s>>>(
       a, stages, row_bytes, (uint64_t)launch_options().timeout_ns);
   *rc = launched("rows_ring_kernel");
   return true;
@@ -1201,7 +1186,7 @@ bool launch_ring_elems(const NormArgs& a, int sms, cudaStream_t s, int* rc) {
   static std::atomic<uint64_t> ready{0};
   *rc = raise_smem(fn, ready);
   if (*rc != B2G_OK) return true;
-  fn<<<(unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas), THREADS, (uint32_t)stages * (stage + 8), s>>>(
+  fn<<<(unsigned)std::min<int64_t>(a.M, (int64_t)sms * ctas), THREADS, ring_bytes(stages, stage), s>>>(
       a, stages, slot, (uint64_t)launch_options().timeout_ns);
   *rc = launched("rows_ring_elems_kernel");
   return true;
@@ -1292,7 +1277,7 @@ int launch_bwd_ring(const BwdArgs& a, int threads, unsigned blocks, int stages, 
   static std::atomic<uint64_t> ready{0};
   const int rc = raise_smem(fn, ready);
   if (rc != B2G_OK) return rc;
-  fn<<<blocks, threads, (uint32_t)stages * ((a.dR ? 2 : 1) * yb + xb + 8), s>>>(
+  fn<<<blocks, threads, ring_bytes(stages, (a.dR ? 2 : 1) * yb + xb), s>>>(
       a, stages, yb, xb, (uint64_t)launch_options().timeout_ns);
   return launched("rmsnorm_bwd_ring_kernel");
 }
@@ -1304,7 +1289,7 @@ int launch_bwd_elems(const BwdArgs& a, unsigned blocks, int stages, uint32_t y_s
   static std::atomic<uint64_t> ready{0};
   const int rc = raise_smem(fn, ready);
   if (rc != B2G_OK) return rc;
-  fn<<<blocks, THREADS, (uint32_t)stages * ((a.dR ? 2 : 1) * y_slot + x_slot + 8), s>>>(
+  fn<<<blocks, THREADS, ring_bytes(stages, (a.dR ? 2 : 1) * y_slot + x_slot), s>>>(
       a, stages, y_slot, x_slot, (uint64_t)launch_options().timeout_ns);
   return launched("rmsnorm_bwd_elems_kernel");
 }

@@ -1,6 +1,6 @@
-// Launch planning of the tensor-core GEMM: tile shape and K splitting.  Pure host functions of
-// the problem's tile counts and the GPU's SM count, shared by the launcher (b2g_api.cu) and
-// b2g_plan_preview (which the CPU tests use to pin the choices).
+// Launch planning: tile shape and K splitting of the tensor-core GEMM, and the shape of the row
+// kernels' rings.  Pure host functions of the problem's sizes and the GPU's SM count, shared by the
+// launchers (b2g_api.cu, b2g_q8.cu, b2g_rows.cu), b2g_plan_preview and the CPU tests that pin them.
 #pragma once
 #include <algorithm>
 #include <cstdint>
@@ -140,6 +140,28 @@ inline SplitChoice choose_splits(int num_tiles, int k_iters, int group_cap, int 
   if (c.k_splits < 1) c.k_splits = 1;
   c.num_full = c.k_splits == 1 ? num_tiles : full;
   return c;
+}
+
+// Dynamic shared memory that the row kernels' rings may ask for: what a block can have, less the kernels'
+// static words.
+constexpr uint32_t kRingSmem = 222 * 1024;
+// Bytes of a ring of `stages` buffers of `stage` bytes, each with its barrier.
+inline uint32_t ring_bytes(int stages, uint32_t stage) { return (uint32_t)stages * (stage + 8); }
+
+// Stages and blocks an SM of a ring kernel: as many blocks as `most` if two stages of each fit (one
+// block's copies run while another's row is worked on), then up to four stages.  False where not
+// even two stages of one block fit.
+inline bool ring_shape(uint32_t stage, int most, int* blocks, int* stages) {
+  constexpr uint32_t kPerBlock = 2048;  // of each block: static words, what the driver keeps, rounding
+  for (int n = most; n >= 1; --n) {
+    const uint32_t fit = ((kRingSmem + kPerBlock) / n - kPerBlock) / (stage + 8);
+    if (fit >= 2) {
+      *blocks = n;
+      *stages = (int)std::min<uint32_t>(4, fit);
+      return true;
+    }
+  }
+  return false;
 }
 
 }  // namespace b2g

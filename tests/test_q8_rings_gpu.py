@@ -1,0 +1,42 @@
+"""GPU tests of the 8-bit layer's row kernels where rows pass through a ring of buffers in shared memory."""
+import pytest
+
+from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, check_bwd, check_norm, rows, row_quant64, grid, tt
+
+pytestmark = pytest.mark.gpu
+
+
+def check_quantize(torch, b2g, M, N, dt, q):
+    x = rows(torch, M, N, N).to(tt(torch, dt))
+    Q, s = torch.zeros(M, N, dtype=torch.int8, device="cuda").view(tt(torch, q)), torch.zeros(M, device="cuda")
+    b2g.quantize_q8(x, Q, s, M, N, dtype=dt, q_dtype=q)
+    t, want = row_quant64(torch, x.double(), q, False)
+    assert torch.equal(s.double(), want)
+    r, half = grid(torch, t, q)
+    if dt != F32:
+        assert torch.equal(Q.double(), r)
+    else:  # the product with qmax and the quotient round once each
+        assert bool(((Q.double() - t).abs() <= half * (1 + 2 ** -20) + 4 * 2.0 ** -24 * t.abs()).all())
+
+
+# Stages of 56832, 75776 and 113664 bytes: four, three and two of them fill the shared memory to its
+# last byte, so that there is no room left for their barriers.
+@pytest.mark.parametrize("dt,N", [(BF16, 14208), (BF16, 18944), (F16, 28416), (F32, 7104), (F32, 9472), (F32, 14208)])
+def test_norm_rings_that_fill_shared_memory(b2g, cuda, dt, N):
+    check_norm(cuda, b2g, 300, N, dt, I8, True, False, 0)
+
+
+@pytest.mark.parametrize("N", [14193, 14196, 14200])
+def test_norm_odd_rings_that_fill_shared_memory(b2g, cuda, N):
+    check_norm(cuda, b2g, 5, N, BF16, E4M3, True, False, 5)
+
+
+@pytest.mark.parametrize("dt,N", [(BF16, 28416), (F32, 14208), (F32, 14203)])
+def test_quantize_rings_that_fill_shared_memory(b2g, cuda, dt, N):
+    check_quantize(cuda, b2g, 300, N, dt, I8)
+
+
+@pytest.mark.parametrize("dt,xt,res,N", [(F32, F32, True, 4736), (F32, F32, True, 9472), (BF16, BF16, False, 14208),
+                                         (BF16, BF16, True, 9472), (F32, I8, True, 6307)])
+def test_backward_rings_that_fill_shared_memory(b2g, cuda, dt, xt, res, N):
+    check_bwd(cuda, b2g, 7, N, dt, xt, res)

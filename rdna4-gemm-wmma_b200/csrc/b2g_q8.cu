@@ -383,6 +383,8 @@ struct Product {
   bool accumulate;
   const float *row_scale, *col_scale, *bias;
   int part_blocks;        // Q_WGRAD: K blocks that one accumulator may sum (0: any number)
+  TileChoice tile;        // with part_blocks: the tile and the K splits of plan_parts()
+  int splits;
 };
 
 using KernFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const GemmParams);
@@ -453,30 +455,12 @@ int resident_clusters(int dev, int v, const Variant& var, int q, int size, int s
 
 bool al16(uintptr_t x) { return (x & 15) == 0; }
 
-// The plain product's tiles; where K goes in parts, at most 256 columns (two accumulators in TMEM).
-TileChoice tiles_of(int64_t nmt, int64_t cols, int64_t kit, int sms, const LaunchOptions& opt, int part_blocks) {
-  const TileChoice tc = choose_tiles(nmt, cols, kit, sms, opt.cta_group, opt.tile_n, 128);
-  if (part_blocks > 0 && kit > part_blocks && tc.bn == 512) return {tc.cg, 256, false};
-  return tc;
-}
-
-// K splits of every tile that launch_product plans for a product in parts (1: none).
-int product_splits(int64_t rows, int64_t cols, int64_t k, int q, int part_blocks, int dev, int sms, int* rc) {
-  const LaunchOptions opt = launch_options();
-  const int64_t kb = q == Q_WGRAD ? 64 : 128, nmt = (rows + kBM - 1) / kBM, kit = (k + kb - 1) / kb;
-  const TileChoice tc = tiles_of(nmt, cols, kit, sms, opt, part_blocks);
-  int cap = 0;
-  *rc = resident_clusters(dev, variant_of(tc), variants()[variant_of(tc)], q, tc.cg, sms, &cap);
-  if (*rc != B2G_OK) return 1;
-  const int tiles = (int)((nmt + tc.cg - 1) / tc.cg * ((cols + tc.bn - 1) / tc.bn));
-  return choose_splits(tiles, (int)kit, cap, tc.cg, opt.split_k, false).k_splits;
-}
-
 int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   const LaunchOptions opt = launch_options();
   const int esz = g.q == Q_WGRAD ? 2 : 1, kb = kRowBytes / esz;
   const int64_t nmt = (g.rows + kBM - 1) / kBM, kit = (g.k + kb - 1) / kb;
-  const TileChoice tc = tiles_of(nmt, g.cols, kit, sms, opt, g.part_blocks);
+  const TileChoice tc =
+      g.part_blocks > 0 ? g.tile : choose_tiles(nmt, g.cols, kit, sms, opt.cta_group, opt.tile_n, 128);
   const int v = variant_of(tc);
   const Variant& var = variants()[v];
   const int cg = var.cg, bn = var.bn;
@@ -571,10 +555,9 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   int group_cap = 0;
   int rc = resident_clusters(dev, v, var, g.q, cg, sms, &group_cap);
   if (rc != B2G_OK) return rc;
-  // (a tail wave is split only where no tile is cut into parts)
-  const bool parts = g.part_blocks > 0 && p.k_iters > g.part_blocks;
   const SplitChoice sc =
-      choose_splits(p.num_tiles, p.k_iters, group_cap, cg, opt.split_k, opt.tail_split && !parts);
+      g.part_blocks > 0 ? choose_splits(p.num_tiles, p.k_iters, group_cap, cg, g.splits, false)
+                        : choose_splits(p.num_tiles, p.k_iters, group_cap, cg, opt.split_k, opt.tail_split);
   p.k_per_split = sc.k_per_split;
   p.k_splits = sc.k_splits;
   p.num_full = sc.num_full;
@@ -582,8 +565,7 @@ int launch_product(const Product& g, int dev, int sms, cudaStream_t stream) {
   const bool sum = g.part_blocks > 0 && p.k_splits == 1 && p.k_iters > g.part_blocks;
   const int q = sum ? (int)Q_WGRAD_SUM : g.q;
   if (sum) {
-    p.k_parts = (p.k_iters + g.part_blocks - 1) / g.part_blocks;
-    p.k_per_part = (p.k_iters + p.k_parts - 1) / p.k_parts;
+    p.k_per_part = part_length(p.k_iters, g.part_blocks);
     p.k_parts = (p.k_iters + p.k_per_part - 1) / p.k_per_part;
   }
   const int split_tiles = p.num_tiles - p.num_full;
@@ -797,7 +779,7 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
     }
     if (M <= kSkinnyTokens) return dtype == B2G_DTYPE_I8 ? skinny<true>(f, sms, s) : skinny<false>(f, sms, s);
     const Product g = {dtype == B2G_DTYPE_I8 ? Q_I8 : Q_FP8, A, B, C, M, N, K, lda, ldb, ldc, 0,
-                       c_type_of(c_dtype), false, a_scale, b_scale, bias, 0};
+                       c_type_of(c_dtype), false, a_scale, b_scale, bias, 0, {}, 0};
     return launch_product(g, dev, sms, s);
   }
   const unsigned blocks = tile_blocks(M, N, sms);
@@ -846,21 +828,25 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
     if (rc == B2G_OK) rc = align_rows(&ry, nullptr, static_cast<char*>(ws.get()) + x_bytes, sms, s);
     if (rc != B2G_OK) return rc;
     const int64_t pitch = ry.pitch;
-    // fp32: whole tiles take their tokens in parts of kMaxTokens (launch_product); where K is split
-    // over CTAs, a launch has at most kMaxTokens a split, and the next one adds to it
+    const LaunchOptions opt = launch_options();
     const int part_blocks = c_dtype == B2G_DTYPE_F32 ? (int)(kMaxTokens / 64) : 0;
     int64_t per = M;
+    PartPlan plan{};
     if (part_blocks) {
-      const int splits = product_splits(N, K, M, Q_WGRAD, part_blocks, dev, sms, &rc);
+      const int64_t nmt = (N + kBM - 1) / kBM, kit = (M + 63) / 64;
+      const TileChoice tc = choose_part_tiles(nmt, K, kit, sms, opt.cta_group, opt.tile_n, part_blocks);
+      int cap = 0;
+      rc = resident_clusters(dev, variant_of(tc), variants()[variant_of(tc)], Q_WGRAD, tc.cg, sms, &cap);
       if (rc != B2G_OK) return rc;
-      if (splits > 1) per = std::min(M, splits * kMaxTokens);
+      plan = plan_parts(tc, nmt, K, kit, cap, opt.split_k, part_blocks);
+      per = plan.blocks * 64;
     }
     for (int64_t m0 = 0; m0 < M && rc == B2G_OK; m0 += per) {
       const Product g = {Q_WGRAD, static_cast<const char*>(ry.p) + m0 * pitch,
                          static_cast<const char*>(ws.get()) + m0 * ldx * 2, dW, N, K,
                          std::min(per, M - m0), pitch / 2, ldx, ldw, dtype == B2G_DTYPE_F16 ? 0 : 1,
                          c_type_of(c_dtype), accumulate != 0 || m0 > 0, nullptr, nullptr, nullptr,
-                         part_blocks};
+                         part_blocks, plan.tile, plan.splits};
       rc = launch_product(g, dev, sms, s);
     }
     return rc;

@@ -142,6 +142,44 @@ inline SplitChoice choose_splits(int num_tiles, int k_iters, int group_cap, int 
   return c;
 }
 
+// A product whose accumulators may sum at most `part` K blocks each (fp32 weight gradients: the tensor
+// core's accumulator truncates).  Whole tiles take their K in parts within one launch; where K is split
+// over CTAs, every launch has at most `part` blocks a split, and the next one adds to it.  Tiles
+// and splits are chosen once, for all of K: every launch takes them as they are.
+struct PartPlan {
+  TileChoice tile;
+  int splits;      // of every tile in every launch
+  int64_t blocks;  // K blocks of a launch (the last one may have fewer)
+};
+
+// Tiles as choose_tiles, but at most 256 columns where K goes in parts (two accumulators in TMEM).
+inline TileChoice choose_part_tiles(int64_t nmt, int64_t cols, int64_t kit, int sms, int opt_cg, int opt_bn,
+                                    int64_t part) {
+  const TileChoice tc = choose_tiles(nmt, cols, kit, sms, opt_cg, opt_bn, 128);
+  if (part > 0 && kit > part && tc.bn == 512) return {tc.cg, 256, false};
+  return tc;
+}
+
+// group_cap: CTA groups of `tile` resident at once; opt_split: forced split count (0 = choose).
+inline PartPlan plan_parts(const TileChoice& tile, int64_t nmt, int64_t cols, int64_t kit, int group_cap,
+                           int opt_split, int64_t part) {
+  const int64_t tiles = (nmt + tile.cg - 1) / tile.cg * ((cols + tile.bn - 1) / tile.bn);
+  const int splits = choose_splits((int)tiles, (int)kit, group_cap, tile.cg, opt_split, false).k_splits;
+  if (splits == 1) return {tile, 1, kit};
+  // Launches of equal length.  Where two splits would need several launches, whole tiles in parts are
+  // faster (us, graph: 2048 tokens, dW 1024 x 2048 29.5 against 34.0, 4096 x 2048 x 1024 46.3 against
+  // 51.4); with four splits they are not (4096 x 1024 x 1024 44.8 against 38.0).
+  const int64_t most = splits * part, launches = std::max<int64_t>(1, (kit + most - 1) / most);
+  if (splits == 2 && launches > 1 && opt_split <= 0) return {tile, 1, kit};
+  return {tile, splits, (kit + launches - 1) / launches};
+}
+
+// K blocks of one part of a whole tile's kit blocks.
+inline int part_length(int kit, int part) {
+  const int parts = (kit + part - 1) / part;
+  return (kit + parts - 1) / parts;
+}
+
 // Dynamic shared memory that the row kernels' rings may ask for: what a block can have, less the kernels'
 // static words.
 constexpr uint32_t kRingSmem = 222 * 1024;

@@ -26,7 +26,43 @@ static int ring() {
   return 0;
 }
 
+// No accumulator of an fp32 weight gradient sums more than 12 K blocks (768 tokens), whatever the sizes
+// and the forced tile or split, and the launches cover every block once.
+static int parts() {
+  constexpr int kPart = 12;
+  static const int opts[][3] = {{0, 0, 0}, {1, 0, 0}, {2, 0, 0}, {1, 128, 0}, {2, 512, 0}, {0, 0, 1}, {0, 0, 3}, {2, 256, 16}, {1, 0, 64}};
+  long long tried = 0, split = 0;
+  for (const auto& o : opts)
+    for (int sms : {148, 132, 74})
+      for (long long rows = 64; rows <= 8192; rows += 128)
+        for (long long cols = 64; cols <= 8192; cols += 128)
+          for (long long tokens : {1, 64, 700, 769, 1000, 1536, 1537, 2048, 3000, 4096, 5000, 8192, 16384, 20001, 65536}) {
+            const int64_t nmt = (rows + 127) / 128, kit = (tokens + 63) / 64;
+            const TileChoice tile = choose_part_tiles(nmt, cols, kit, sms, o[0], o[1], kPart);
+            const PartPlan p = plan_parts(tile, nmt, cols, kit, sms / tile.cg, o[2], kPart);
+            const int tiles = (int)((nmt + tile.cg - 1) / tile.cg * ((cols + tile.bn - 1) / tile.bn));
+            int64_t worst = 0, done = 0;
+            ++tried;
+            for (int64_t b = 0; b < kit; b += p.blocks) {  // as the launches are made
+              const int k = (int)std::min(p.blocks, kit - b);
+              const SplitChoice s = choose_splits(tiles, k, sms / tile.cg, tile.cg, p.splits, false);
+              const int sum = s.k_splits > 1 ? s.k_per_split : k > kPart ? part_length(k, kPart) : k;
+              if (s.k_splits > 1 && s.num_full != 0) return printf("a whole tile beside split ones\n"), 1;
+              if (s.k_splits == 1 && k > kPart && p.tile.bn == 512) return printf("parts in a 512-column tile\n"), 1;
+              worst = std::max<int64_t>(worst, sum);
+              done += k;
+              split += s.k_splits > 1;
+            }
+            if (worst > kPart || done != kit)
+              return printf("%lld tokens, dW %lld x %lld, options %d %d %d: %lld blocks in one accumulator, %lld of %lld done\n", tokens,
+                            rows, cols, o[0], o[1], o[2], (long long)worst, (long long)done, (long long)kit), 1;
+          }
+  printf("ok %lld, %lld split launches\n", tried, split);
+  return 0;
+}
+
 int main(int argc, char** argv) {
   if (argc > 1 && !strcmp(argv[1], "ring")) return ring();
+  if (argc > 1 && !strcmp(argv[1], "parts")) return parts();
   return 2;
 }

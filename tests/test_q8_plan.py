@@ -24,3 +24,8 @@ def plan(tmp_path_factory):
 def test_rings_fit_shared_memory(plan):
     run = plan("ring")
     assert run.returncode == 0 and run.stdout.startswith("ok"), run.stdout
+
+
+def test_weight_gradient_sums_at_most_768_tokens_an_accumulator(plan):
+    run = plan("parts")
+    assert run.returncode == 0 and run.stdout.startswith("ok"), run.stdout

@@ -56,6 +56,7 @@ void clear_error() { t_err.clear(); }
 void set_path(int path) { t_path = path; }
 
 int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();  // reported here: the thread's next launch check must not see it again
   return fail(B2G_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 

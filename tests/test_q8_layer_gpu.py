@@ -24,3 +24,29 @@ def test_weight_gradient_split_over_ctas_keeps_fp32(b2g, cuda, M, N, K, dt):
     rel = lambda v: float((v.double() - ref).norm() / ref.norm())
     assert rel(dW) <= max(1e-6, 1.5 * rel(dY.float().t() @ x)), rel(dW)
     assert b2g.device_status() == 0
+
+
+def test_failed_launch_leaves_no_error_behind(b2g, cuda):
+    """A product whose launch the driver refuses (the legacy stream while a blocking stream records a graph)
+    reports it; the next operator of the thread, a row kernel, does not report it again."""
+    torch = cuda
+    runtime = pytest.importorskip("cuda.bindings.runtime")
+    A, B = (torch.ones(n, 2048, dtype=torch.int8, device="cuda") for n in (1, 512))
+    C = torch.zeros(1, 512, device="cuda")
+    x = torch.full((4, 64), 127.0, device="cuda")
+    Q, s = torch.zeros(4, 64, dtype=torch.int8, device="cuda"), torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    err, stream = runtime.cudaStreamCreate()
+    assert int(err) == 0
+    err, = runtime.cudaStreamBeginCapture(stream, runtime.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal)
+    assert int(err) == 0
+    try:
+        with pytest.raises(b2g.B2GError, match="gemm_q8_few_kernel"):
+            b2g.gemm_q8(A, B, C, 1, 512, 2048, stream=0)
+    finally:
+        runtime.cudaStreamEndCapture(stream)
+        runtime.cudaStreamDestroy(stream)
+    b2g.quantize_q8(x, Q, s, 4, 64, dtype=b2g.DTYPE_F32, stream=0)
+    b2g.gemm_q8(A, B, C, 1, 512, 2048, stream=0)
+    torch.cuda.synchronize()
+    assert bool((Q == 127).all()) and bool((s == 1).all()) and bool((C == 2048).all())

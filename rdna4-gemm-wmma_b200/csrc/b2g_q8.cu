@@ -14,6 +14,7 @@
 #include "host.h"
 #include "plan.h"
 #include "q8.cuh"
+#include "sched.h"
 #include "skinny_sm100.cuh"
 
 namespace b2g {
@@ -278,8 +279,9 @@ struct RepackJob {
 
 // A warp copies a piece of a row: each lane loads whole 4-byte words from the word that holds its first
 // byte on, takes the next word from its neighbour and shifts the two together.  A row's piece may
-// begin up to 3 bytes before the row and end as far behind it, inside the matrix; in its first and last
-// row words are put together from bytes where they would reach out of it.  Memory-bound: all of a
+// begin up to 3 bytes before the row and end as far behind it; in the rows from which that could reach out of
+// the matrix (the first and the last, and more of them where pitches are below 3 bytes) words are put
+// together from bytes where they would.  Memory-bound: all of a
 // piece's loads are issued before the first is used.  It costs 30 us for 64 MiB of weights (4.4 TB/s, read
 // and written), which a product of 16 tokens with them, 14.8 us, pays in every call.
 constexpr int kRepackWords = 8;  // words a lane
@@ -298,7 +300,7 @@ __global__ void __launch_bounds__(256) repack_kernel(const RepackJob a, const Re
     const uint8_t* p = row - off + at0;
     const int64_t left = g.bytes + off - at0;  // bytes of the row from p on
     uint32_t w[U], last = 0;
-    if (r > 0 && r < g.rows - 1) {
+    if (b2g_row_words_inside(r, g.rows, g.sp)) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         w[u] = u * 128 < left ? __ldcs(reinterpret_cast<const uint32_t*>(p + u * 128)) : 0u;

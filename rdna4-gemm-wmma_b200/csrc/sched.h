@@ -27,3 +27,10 @@ B2G_HD void b2g_sched_tile(int t, int num_m, int num_n, int group, int* tm, int*
   *tm = first_m + r % rows;
   *tn = r / rows;
 }
+
+// The aligning copy of an operand (repack_kernel, b2g_q8.cu) reads row r in whole 4-byte words, which reach
+// up to 3 bytes beyond either end of the row.  Whether they lie inside the matrix, `rows` rows of
+// pitch `pitch` bytes: where pitches are narrow, not only for rows other than the first and last.
+B2G_HD bool b2g_row_words_inside(long long r, long long rows, long long pitch) {
+  return r * pitch >= 3 && (rows - 1 - r) * pitch >= 3;
+}

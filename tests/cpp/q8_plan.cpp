@@ -3,6 +3,7 @@
 #include <cstring>
 
 #include "plan.h"
+#include "sched.h"
 
 using namespace b2g;
 
@@ -61,8 +62,33 @@ static int parts() {
   return 0;
 }
 
+// The words that the aligning copy reads without a check lie inside the matrix, for every row, base
+// alignment, length and pitch.
+static int words() {
+  long long tried = 0;
+  for (int base = 4; base < 8; ++base)
+    for (int rows = 1; rows <= 12; ++rows)
+      for (int bytes = 1; bytes <= 40; ++bytes)
+        for (int pitch = bytes; pitch <= bytes + 9; ++pitch)
+          for (int r = 0; r < rows; ++r) {
+            if (!b2g_row_words_inside(r, rows, pitch)) continue;
+            const int row = base + r * pitch, first = row & ~3, last = (row + bytes - 1) | 3;  // first and last byte read
+            const int end = base + (rows - 1) * pitch + bytes;
+            ++tried;
+            if (first < base || last >= end)
+              return printf("base %d, row %d of %d, %d bytes, pitch %d: reads [%d, %d] of [%d, %d)\n", base, r, rows, bytes, pitch, first,
+                            last, base, end), 1;
+          }
+  // and the rows in the middle of an ordinary matrix go without the check
+  for (int r = 1; r < 99; ++r)
+    if (!b2g_row_words_inside(r, 100, 3)) return printf("row %d of 100 is checked\n", r), 1;
+  printf("ok %lld\n", tried);
+  return 0;
+}
+
 int main(int argc, char** argv) {
   if (argc > 1 && !strcmp(argv[1], "ring")) return ring();
   if (argc > 1 && !strcmp(argv[1], "parts")) return parts();
+  if (argc > 1 && !strcmp(argv[1], "words")) return words();
   return 2;
 }

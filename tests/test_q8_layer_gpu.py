@@ -1,7 +1,7 @@
 """GPU tests of the 8-bit layer's products: sums of many tokens, scales, and launches that fail."""
 import pytest
 
-from test_q8_gpu import BF16, F16, NAMES, scales, tt
+from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, scales, tt
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,31 @@ def test_failed_launch_leaves_no_error_behind(b2g, cuda):
     b2g.gemm_q8(A, B, C, 1, 512, 2048, stream=0)
     torch.cuda.synchronize()
     assert bool((Q == 127).all()) and bool((s == 1).all()) and bool((C == 2048).all())
+
+
+@pytest.mark.parametrize("q", [I8, E4M3], ids=NAMES.get)
+@pytest.mark.parametrize("K", [1, 2, 3])
+@pytest.mark.parametrize("M", [9, 200])
+def test_products_of_narrow_operands_at_odd_bases(b2g, cuda, M, K, q):
+    """Contiguous operands of one to three columns, one byte past a word's start: sums of up to three products of
+    small integers, exact in every type."""
+    torch = cuda
+    def narrow(rows, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        buf = torch.zeros(rows * K + 16, dtype=torch.int8, device="cuda").view(tt(torch, q))
+        v = buf[1:1 + rows * K].view(rows, K)
+        v.copy_(torch.randint(-8, 9, (rows, K), generator=g, device="cuda").float())
+        return v
+    N = 130
+    A, B = narrow(M, 1), narrow(N, 2)
+    C = torch.zeros(M, N, device="cuda")
+    b2g.gemm_q8(A, B, C, M, N, K, dtype=q)
+    assert torch.equal(C, A.float() @ B.float().t())
+    # the same in the weight gradient: dY of one to three columns, two bytes past a word's start
+    y = torch.zeros(M * K + 8, dtype=torch.bfloat16, device="cuda")[1:1 + M * K].view(M, K)
+    y.copy_(torch.randint(-3, 4, (M, K), device="cuda"))
+    X = torch.randint(-8, 9, (M, 24), device="cuda").float().to(tt(torch, q))
+    dW = torch.zeros(K, 24, device="cuda")
+    b2g.wgrad_q8(y, X, torch.ones(M, device="cuda"), dW, M, K, 24, q_dtype=q)
+    assert torch.equal(dW, y.float().t() @ X.float())
+    assert b2g.device_status() == 0

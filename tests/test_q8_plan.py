@@ -29,3 +29,8 @@ def test_rings_fit_shared_memory(plan):
 def test_weight_gradient_sums_at_most_768_tokens_an_accumulator(plan):
     run = plan("parts")
     assert run.returncode == 0 and run.stdout.startswith("ok"), run.stdout
+
+
+def test_aligning_copy_reads_inside_its_operand(plan):
+    run = plan("words")
+    assert run.returncode == 0 and run.stdout.startswith("ok"), run.stdout

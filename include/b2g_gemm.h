@@ -352,7 +352,10 @@ int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t 
  *   - b2g_last_path() is set by the two products and not by the row operators.
  *   - The products obey the options cta_group, tile_n, split_k, tail_split, cluster_fixup,
  *     serial_fixup, pdl, raster_group, force_generic, timeout_ns and fault_flags; the row operators
- *     obey timeout_ns.
+ *     obey timeout_ns and fault_flags.
+ *   - Where a wait of a row operator runs out (b2g_device_status() code 8), the rows of that block from there
+ *     on come out with the scale and rstd NaN and zeros, or as a NaN dX, and H is NaN in all of
+ *     that block's rows.
  *
  * b2g_quantize_q8: rows of X (dtype F16, BF16 or F32) into Q.  Per row, with a = max|x|:
  *   scale = max(a / qmax, 2^-126), q = round(x * qmax / a) (to nearest, ties to even; x / scale

@@ -55,6 +55,7 @@ struct NormArgs {
   int dtype, w_dtype, q_dtype;
   float eps;
   bool norm, pow2;
+  bool fault;  // test-only: a ring's copies are left out, so that its waits run out
 };
 
 // ------------------------------------------------------------------ vectors of a row
@@ -293,8 +294,9 @@ __device__ __forceinline__ void unpack(const uint8_t* p, float (&v)[VEC]) {
 // A ring of row buffers in shared memory, filled by bulk copies.  `full` barriers count the bytes of each
 // buffer; thread 0 refills a buffer once every thread has read it.  Copies run ahead of the rows by
 // up to `stages`, which keeps the memory busy however long a row's reduction takes, and costs no
-// registers.  A wait that runs out marks the block, later waits return at once, and its rows come
-// out as NaN.
+// registers.  A wait that runs out raises the block's flag, and every row from there on comes out as NaN:
+// each thread looks at the flag after its wait, not at the wait's answer, because a buffer that is not
+// refilled shows every other of its later phases as complete.
 struct Ring {
   uint32_t base, bars, stage_bytes;
   int stages;
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   };
   int issued = 0;
   if (tid == 0)
-    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+    for (int64_t m = first + (a.fault ? a.M : 0); m < a.M && issued < stages; m += step) fill(m, issued++);
   const bool wvec = NORM && weights_vec(a.W, a.w_dtype);
   float wreg[WREG ? V : 1][VEC];
   if constexpr (WREG)
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     for (int i = 0; i < V; ++i) load_weights<VEC>(a.W, a.w_dtype, wvec, (i * threads + tid) * VEC, N, wreg[i]);
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
-    const bool ok = ring.wait(k);
+    ring.wait(k);
     const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     float v[V][VEC];
     F2 ss = f2(0.0f, 0.0f);
@@ -403,7 +405,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     float s0, s1;
     f2_get(ss, s0, s1);
     float sum = s0 + s1;
-    uint32_t bits = ok ? __float_as_uint(top) : 0x7fffffffu;
+    uint32_t bits = __float_as_uint(top);
+    if (*ring.abort_flag) {
+      bits = 0x7fffffffu;
+      sum = __int_as_float(0x7fc00000);
+    }
     row_reduce<0, NORM>(sum, bits, buf, k & 1);
     if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
       fill(m + step * stages, k + stages);  // every thread has read this row (row_reduce)
@@ -427,6 +433,9 @@ __global__ void __launch_bounds__(THREADS, CTAS)
       }
     }
   }
+  if (NORM && a.H && *ring.abort_flag)  // H was stored before its row was known to be lost
+    for (int64_t m = first; m < a.M; m += step)
+      for (int n = tid; n < N; n += (int)blockDim.x) from_f(static_cast<T*>(a.H) + m * a.ldh + n, __int_as_float(0x7fc00000));
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
@@ -475,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
   };
   int issued = 0;
   if (tid == 0)
-    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+    for (int64_t m = first + (a.fault ? a.M : 0); m < a.M && issued < stages; m += step) fill(m, issued++);
   float w[NORM ? V : 1];
   if constexpr (NORM)
 #pragma unroll
@@ -486,7 +495,8 @@ __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
     }
   int k = 0;
   for (int64_t m = first; m < a.M; m += step, ++k) {
-    const bool ok = ring.wait(k), end = at_end(m);
+    ring.wait(k);
+    const bool end = at_end(m);
     const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     const T* gx = X + m * a.ldx;
     const T* gr = R ? R + m * a.ldr : nullptr;
@@ -520,7 +530,11 @@ __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
       }
       top = max_abs(top, v[i]);
     }
-    uint32_t bits = ok ? __float_as_uint(top) : 0x7fffffffu;
+    uint32_t bits = __float_as_uint(top);
+    if (*ring.abort_flag) {
+      bits = 0x7fffffffu;
+      sum = __int_as_float(0x7fc00000);
+    }
     row_reduce<0, NORM>(sum, bits, buf, k & 1);
     if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
       fill(m + step * stages, k + stages);  // every thread has read this row (row_reduce)
@@ -540,6 +554,9 @@ __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
     for (int i = 0; i < V; ++i)
       if (i * THREADS < count) q[i * THREADS] = (uint8_t)o[i];
   }
+  if (NORM && a.H && *ring.abort_flag)  // H was stored before its row was known to be lost
+    for (int64_t m = first; m < a.M; m += step)
+      for (int n = tid; n < N; n += (int)blockDim.x) from_f(static_cast<T*>(a.H) + m * a.ldh + n, __int_as_float(0x7fc00000));
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 
@@ -712,6 +729,7 @@ struct BwdArgs {
   float* part;  // [blocks][N] partial sums of dw, or null
   int64_t M, N, ldy, ldx, ldr, lddx;
   int dtype, x_dtype, w_dtype;
+  bool fault;  // as NormArgs::fault
 };
 
 // Any size, alignment and checkpoint type, one block a row at a time, element by element: mean(g * xh), then
@@ -852,7 +870,7 @@ __global__ void __launch_bounds__(512, 1)
   };
   int issued = 0;
   if (tid == 0)
-    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+    for (int64_t m = first + (a.fault ? a.M : 0); m < a.M && issued < stages; m += step) fill(m, issued++);
   const bool wvec = weights_vec(a.W, a.w_dtype);
   auto weights = [&](int i, F2 (&w)[P]) {
     float f[VEC];
@@ -879,7 +897,7 @@ __global__ void __launch_bounds__(512, 1)
       if (a.x_scale) next_scale = __ldg(a.x_scale + m + step);
     }
     const F2 xs2 = f2(xs, xs);
-    const bool ok = ring.wait(k);
+    ring.wait(k);
     const uint8_t* st = smem + (uint32_t)(k % stages) * stage_bytes;
     Vec<T, VEC> y[V], r[V];
     XV x[V];
@@ -911,7 +929,7 @@ __global__ void __launch_bounds__(512, 1)
     float c0, c1;
     f2_get(c2, c0, c1);
     float c = c0 + c1;
-    uint32_t late = ok ? 0u : 1u;
+    uint32_t late = (uint32_t)*ring.abort_flag;
     row_reduce<0, true>(c, late, buf, k & 1);
     if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
       fill(m + step * stages, k + stages);  // every thread holds its part of this row (row_reduce)
@@ -1005,7 +1023,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS)
   };
   int issued = 0;
   if (tid == 0)
-    for (int64_t m = first; m < a.M && issued < stages; m += step) fill(m, issued++);
+    for (int64_t m = first + (a.fault ? a.M : 0); m < a.M && issued < stages; m += step) fill(m, issued++);
   float w[V], dw[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -1023,7 +1041,8 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS)
       next_rstd = __ldg(a.rstd + m + step);
       if (a.x_scale) next_scale = __ldg(a.x_scale + m + step);
     }
-    const bool ok = ring.wait(k), end = at_end(m);
+    ring.wait(k);
+    const bool end = at_end(m);
     const uint8_t* st = smem + (uint32_t)(k % stages) * ring.stage_bytes;
     float g[V], xh[V], dr[V];
     float c = 0.0f;
@@ -1065,7 +1084,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS)
       g[i] *= w[i];
       c = fmaf(g[i], xh[i], c);
     }
-    uint32_t late = ok ? 0u : 1u;
+    uint32_t late = (uint32_t)*ring.abort_flag;
     row_reduce<0, true>(c, late, buf, k & 1);
     if (tid == 0 && m + step * stages < a.M && !*ring.abort_flag) {
       fill(m + step * stages, k + stages);  // every thread holds its part of this row (row_reduce)
@@ -1400,6 +1419,7 @@ extern "C" int b2g_quantize_q8(const void* X, void* Q, float* scale, int64_t M, 
   a.M = M; a.N = N; a.ldx = ldx; a.ldq = ldq;
   a.dtype = dtype; a.w_dtype = dtype; a.q_dtype = q_dtype;
   a.pow2 = pow2 != 0;
+  a.fault = (launch_options().fault_flags & 1) != 0;
   return rows_to_q8(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -1440,6 +1460,7 @@ extern "C" int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void*
   a.eps = eps;
   a.norm = true;
   a.pow2 = pow2 != 0;
+  a.fault = (launch_options().fault_flags & 1) != 0;
   return rows_to_q8(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -1476,6 +1497,7 @@ extern "C" int b2g_rmsnorm_bwd_q8(const void* dY, const void* X, const float* x_
   a.dX = dX;
   a.M = M; a.N = N; a.ldy = ldy; a.ldx = ldx; a.ldr = ldr; a.lddx = lddx;
   a.dtype = dtype; a.x_dtype = x_dtype; a.w_dtype = w_dtype;
+  a.fault = (launch_options().fault_flags & 1) != 0;
   const bool x8 = is_q8(x_dtype), same = x_dtype == dtype;
   switch (dtype) {
     case B2G_DTYPE_F16: return bwd_of<__half>(a, x8, same, dw, sms, s);

@@ -1,6 +1,7 @@
 """GPU tests of the 8-bit layer's row kernels where rows pass through a ring of buffers in shared memory."""
 import pytest
 
+from gpu_util import options
 from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, check_bwd, check_norm, rows, row_quant64, grid, tt
 
 pytestmark = pytest.mark.gpu
@@ -40,3 +41,41 @@ def test_quantize_rings_that_fill_shared_memory(b2g, cuda, dt, N):
                                          (BF16, BF16, True, 9472), (F32, I8, True, 6307)])
 def test_backward_rings_that_fill_shared_memory(b2g, cuda, dt, xt, res, N):
     check_bwd(cuda, b2g, 7, N, dt, xt, res)
+
+
+def lost_copies(torch, b2g, call):
+    """Runs `call` with the rings' copies left out (test option): its waits run out after 2 ms, it ends and
+    says so, and the next call is sound."""
+    with options(b2g, fault_flags=1, timeout_ns=2000000):
+        call()
+        assert b2g.device_status() == 8
+    assert b2g.device_status() == 0
+
+
+# (M, N, pitch): aligned rows and rows of any alignment, over a hundred of them a block
+RINGS = [(60000, 1024, 1024), (60000, 1027, 1029)]
+
+
+@pytest.mark.parametrize("M,N,pitch", RINGS)
+def test_rows_behind_a_lost_copy_are_marked(b2g, cuda, M, N, pitch):
+    """Every row whose copy did not arrive, or that came after one in its block, has the scale NaN and zeros,
+    or a NaN gradient: also those whose buffer would have been filled several times by then."""
+    torch = cuda
+    x = torch.ones(M, pitch, dtype=torch.bfloat16, device="cuda")[:, :N]
+    w = torch.ones(N, dtype=torch.bfloat16, device="cuda")
+    Q, s = torch.ones(M, pitch, dtype=torch.int8, device="cuda")[:, :N], torch.ones(M, device="cuda")
+    h, rstd = torch.ones(M, pitch, dtype=torch.bfloat16, device="cuda")[:, :N], torch.ones(M, device="cuda")
+    for res in (None, x):
+        Q.fill_(1)
+        lost_copies(torch, b2g, lambda: b2g.rmsnorm_q8(x, w, Q, s, M, N, dtype=BF16, R=res, H=h, rstd=rstd))
+        assert bool(torch.isnan(s).all()) and bool(torch.isnan(rstd).all()) and not Q.any()
+        assert bool(torch.isnan(h).all())
+        h.fill_(1)
+    Q.fill_(1)
+    lost_copies(torch, b2g, lambda: b2g.quantize_q8(x, Q, s, M, N, dtype=BF16))
+    assert bool(torch.isnan(s).all()) and not Q.any()
+    d, ones = torch.ones(M, pitch, dtype=torch.bfloat16, device="cuda")[:, :N], torch.ones(M, device="cuda")
+    lost_copies(torch, b2g, lambda: b2g.rmsnorm_bwd_q8(x, Q, ones, w, ones, d, None, M, N, dtype=BF16))
+    assert bool(torch.isnan(d).all())
+    b2g.quantize_q8(x, Q, s, M, N, dtype=BF16)
+    assert bool((Q == 127).all()) and b2g.device_status() == 0

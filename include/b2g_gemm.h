@@ -354,8 +354,8 @@ int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t 
  *     serial_fixup, pdl, raster_group, force_generic, timeout_ns and fault_flags; the row operators
  *     obey timeout_ns and fault_flags.
  *   - Where a wait of a row operator runs out (b2g_device_status() code 8), the rows of that block from there
- *     on come out with the scale and rstd NaN and zeros, or as a NaN dX, and H is NaN in all of
- *     that block's rows.
+ *     on come out with the scale and rstd NaN and zeros, or as a NaN dX, H is NaN in all of that
+ *     block's rows, and dw is NaN.
  *
  * b2g_quantize_q8: rows of X (dtype F16, BF16 or F32) into Q.  Per row, with a = max|x|:
  *   scale = max(a / qmax, 2^-126), q = round(x * qmax / a) (to nearest, ties to even; x / scale

@@ -972,6 +972,7 @@ __global__ void __launch_bounds__(512, 1)
     }
   }
   if (a.part) {
+    const bool lost = *ring.abort_flag;  // dw took in a row whose copy did not arrive
     float* p = a.part + (int64_t)blockIdx.x * a.N;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -982,6 +983,7 @@ __global__ void __launch_bounds__(512, 1)
           float4 v;
           f2_get(dw[i][j / 2], v.x, v.y);
           f2_get(dw[i][j / 2 + 1], v.z, v.w);
+          if (lost) v.x = v.y = v.z = v.w = __int_as_float(0x7fc00000);
           *reinterpret_cast<float4*>(p + n + j) = v;
         }
     }
@@ -1102,10 +1104,11 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS)
     for (int i = 0; i < V; ++i)
       if (i * THREADS < count) from_f(dX + i * THREADS, g[i]);
   }
+  const bool lost = *ring.abort_flag;
   if (a.part)
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i * THREADS + tid < N) a.part[(int64_t)blockIdx.x * N + i * THREADS + tid] = dw[i];
+      if (i * THREADS + tid < N) a.part[(int64_t)blockIdx.x * N + i * THREADS + tid] = lost ? __int_as_float(0x7fc00000) : dw[i];
   if (tid == 0 && *ring.abort_flag) ring.drain(issued);
 }
 

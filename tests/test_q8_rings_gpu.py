@@ -79,3 +79,19 @@ def test_rows_behind_a_lost_copy_are_marked(b2g, cuda, M, N, pitch):
     assert bool(torch.isnan(d).all())
     b2g.quantize_q8(x, Q, s, M, N, dtype=BF16)
     assert bool((Q == 127).all()) and b2g.device_status() == 0
+
+
+# the kernels that hold a row in registers, that unpack it twice, and that take any alignment
+@pytest.mark.parametrize("N,pitch", [(1024, 1024), (16384, 16384), (1027, 1029)])
+def test_weight_gradient_of_the_norm_tells_of_a_lost_copy(b2g, cuda, N, pitch):
+    """dw is a sum over all rows: NaN where one of them did not arrive."""
+    torch = cuda
+    M = 3000
+    y = torch.ones(M, pitch, dtype=torch.bfloat16, device="cuda")[:, :N]
+    x = torch.ones(M, pitch, dtype=torch.int8, device="cuda")[:, :N]
+    w, ones, dw = torch.ones(N, dtype=torch.bfloat16, device="cuda"), torch.ones(M, device="cuda"), torch.zeros(N, device="cuda")
+    d = torch.ones(M, pitch, dtype=torch.bfloat16, device="cuda")[:, :N]
+    lost_copies(torch, b2g, lambda: b2g.rmsnorm_bwd_q8(y, x, ones, w, ones, d, dw, M, N, dtype=BF16))
+    assert bool(torch.isnan(dw).all()) and bool(torch.isnan(d).all())
+    b2g.rmsnorm_bwd_q8(y, x, ones, w, ones, d, dw, M, N, dtype=BF16)
+    assert bool((dw == M).all()) and not d.any() and b2g.device_status() == 0

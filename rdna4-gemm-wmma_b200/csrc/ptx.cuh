@@ -142,14 +142,17 @@ __device__ __forceinline__ uint32_t ld_shared_cluster_b32(uint32_t addr) {
 }
 
 // Teardown variant: ignores the abort flag (the copies or MMAs being waited for finish
-// on their own) and is bounded by time only.
+// on their own) and is bounded by time only: by kDrainNs at least, however short a limit the
+// waits before it were given (b2g_set_option "timeout_ns"), since shared memory or TMEM that is
+// given up under a copy or an MMA is another block's by the time it lands.
+constexpr uint64_t kDrainNs = 2000000;
 __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity, int* err, int code,
                                                 uint64_t limit_ns) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer();
   for (uint32_t n = 1;; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((n & 63u) == 0 && globaltimer() - t0 > limit_ns) {
+    if ((n & 63u) == 0 && globaltimer() - t0 > (limit_ns < kDrainNs ? kDrainNs : limit_ns)) {
       atomicCAS(err, 0, code);
       return false;
     }

@@ -95,3 +95,29 @@ def test_weight_gradient_of_the_norm_tells_of_a_lost_copy(b2g, cuda, N, pitch):
     assert bool(torch.isnan(dw).all()) and bool(torch.isnan(d).all())
     b2g.rmsnorm_bwd_q8(y, x, ones, w, ones, d, dw, M, N, dtype=BF16)
     assert bool((dw == M).all()) and not d.any() and b2g.device_status() == 0
+
+
+def test_least_time_limit(b2g, cuda):
+    """With a limit of 1 ns a wait may give up at any time, with copies in flight: calls then end with code 8
+    (or a product's) or with the right rows, and no later call is disturbed."""
+    torch = cuda
+    from test_q8_gpu import check_gemm
+    M, N = 4000, 2048
+    x, w = rows(torch, M, N, 1).to(torch.bfloat16), torch.ones(N, dtype=torch.bfloat16, device="cuda")
+    Q, s, rstd = torch.zeros(M, N, dtype=torch.int8, device="cuda"), torch.zeros(M, device="cuda"), torch.ones(M, device="cuda")
+    d, dw = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda"), torch.zeros(N, device="cuda")
+    A, C = torch.ones(100, N, dtype=torch.int8, device="cuda"), torch.zeros(100, M, device="cuda")
+    def step():
+        b2g.rmsnorm_q8(x, w, Q, s, M, N, dtype=BF16, R=x, rstd=rstd)
+        b2g.rmsnorm_bwd_q8(x, Q, s, w, rstd, d, dw, M, N, dtype=BF16)
+        b2g.gemm_q8(A, Q, C, 100, M, N)
+        return [t.clone() for t in (Q, s, rstd, d, dw, C)]
+    want = step()
+    assert b2g.device_status() == 0
+    with options(b2g, timeout_ns=1):
+        for _ in range(20):
+            got = step()
+            assert b2g.device_status() != 0 or all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    check_gemm(torch, b2g, 100, 520, 1184, I8, F32)
+    assert b2g.device_status() == 0

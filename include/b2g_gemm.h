@@ -341,8 +341,8 @@ int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t 
  * Conventions of the b2g_*_q8 entry points:
  *   - An 8-bit matrix is row-major, B2G_DTYPE_I8 (qmax 127) or B2G_DTYPE_E4M3 (qmax 448), with
  *     one fp32 scale per row; element (m, n) stands for Q[m*ldq + n] * scale[m].
- *   - Any leading dimension >= the row length (in elements) and any alignment of the element type
- *     are accepted.  Row pitches and base addresses that are multiples of 16 bytes run fastest:
+ *   - Any leading dimension >= the row length (in elements) and any address that is aligned to the
+ *     element type are accepted (others are refused).  Row pitches and base addresses that are multiples of 16 bytes run fastest:
  *     elsewhere the row kernels load elements one by one and the products copy the operand into
  *     an aligned workspace first.  Elements between the row length and the pitch are not written,
  *     and their values are never used.

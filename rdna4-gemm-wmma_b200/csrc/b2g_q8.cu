@@ -759,8 +759,11 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
   }
   if (!C) return fail(B2G_ERR_INVALID_ARG, "C is null");
   if (K > 0 && (!A || !B)) return fail(B2G_ERR_INVALID_ARG, "A or B is null");
+  int rc = check_alignment({{"C", C, c_dtype}, {"a_scale", a_scale, B2G_DTYPE_F32},
+                            {"b_scale", b_scale, B2G_DTYPE_F32}, {"bias", bias, B2G_DTYPE_F32}});
+  if (rc != B2G_OK) return rc;
   int dev = 0, sms = 0, cc = 0;
-  int rc = current_device(&dev, &sms, &cc);
+  rc = current_device(&dev, &sms, &cc);
   if (rc != B2G_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (tensor_ok(cc, M, N, K)) {
@@ -815,9 +818,11 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
   }
   if (!dW) return fail(B2G_ERR_INVALID_ARG, "dW is null");
   if (M > 0 && (!dY || !Q || !scale)) return fail(B2G_ERR_INVALID_ARG, "dY, Q or scale is null");
+  int rc = check_alignment({{"dY", dY, dtype}, {"scale", scale, B2G_DTYPE_F32}, {"dW", dW, c_dtype}});
+  if (rc != B2G_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int dev = 0, sms = 0, cc = 0;
-  int rc = current_device(&dev, &sms, &cc);
+  rc = current_device(&dev, &sms, &cc);
   if (rc != B2G_OK) return rc;
   if (tensor_ok(cc, N, K, M)) {
     // the checkpoint's rows in dY's type, then the product of two token-major matrices

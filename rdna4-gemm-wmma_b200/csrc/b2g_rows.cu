@@ -1410,11 +1410,13 @@ extern "C" int b2g_quantize_q8(const void* X, void* Q, float* scale, int64_t M, 
   clear_error();
   if (!is_real(dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported input type code %d", dtype);
   if (!is_q8(q_dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported 8-bit type code %d", q_dtype);
-  const int rc = check_rows(M, N, {ldx, ldq});
+  int rc = check_rows(M, N, {ldx, ldq});
   if (rc != B2G_OK) return rc;
   if (M == 0) return B2G_OK;
   if (N == 0) return fail(B2G_ERR_INVALID_ARG, "rows of no elements have no scale");
   if (!X || !Q || !scale) return fail(B2G_ERR_INVALID_ARG, "X, Q or scale is null");
+  rc = check_alignment({{"X", X, dtype}, {"scale", scale, B2G_DTYPE_F32}});
+  if (rc != B2G_OK) return rc;
   NormArgs a{};
   a.X = X;
   a.Q = Q;
@@ -1431,10 +1433,12 @@ extern "C" int b2g_dequantize_q8(const void* Q, const float* scale, void* X, int
   clear_error();
   if (!is_real(dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported output type code %d", dtype);
   if (!is_q8(q_dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported 8-bit type code %d", q_dtype);
-  const int rc = check_rows(M, N, {ldx, ldq});
+  int rc = check_rows(M, N, {ldx, ldq});
   if (rc != B2G_OK) return rc;
   if (M == 0 || N == 0) return B2G_OK;
   if (!X || !Q || !scale) return fail(B2G_ERR_INVALID_ARG, "X, Q or scale is null");
+  rc = check_alignment({{"X", X, dtype}, {"scale", scale, B2G_DTYPE_F32}});
+  if (rc != B2G_OK) return rc;
   return dequantize_rows(Q, scale, X, M, N, ldq, ldx, q_dtype, dtype,
                          static_cast<cudaStream_t>(stream));
 }
@@ -1447,12 +1451,15 @@ extern "C" int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void*
   if (!is_real(dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported input type code %d", dtype);
   if (!is_real(w_dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported weight type code %d", w_dtype);
   if (!is_q8(q_dtype)) return fail(B2G_ERR_INVALID_ARG, "unsupported 8-bit type code %d", q_dtype);
-  const int rc = check_rows(M, N, {ldx, R ? ldr : ldx, H ? ldh : ldx, ldq});
+  int rc = check_rows(M, N, {ldx, R ? ldr : ldx, H ? ldh : ldx, ldq});
   if (rc != B2G_OK) return rc;
   if (!(eps >= 0.0f)) return fail(B2G_ERR_INVALID_ARG, "eps is negative or NaN");
   if (M == 0) return B2G_OK;
   if (N == 0) return fail(B2G_ERR_INVALID_ARG, "rows of no elements have no norm");
   if (!X || !W || !Q || !scale) return fail(B2G_ERR_INVALID_ARG, "X, W, Q or scale is null");
+  rc = check_alignment({{"X", X, dtype}, {"R", R, dtype}, {"W", W, w_dtype}, {"H", H, dtype},
+                        {"scale", scale, B2G_DTYPE_F32}, {"rstd", rstd, B2G_DTYPE_F32}});
+  if (rc != B2G_OK) return rc;
   if (H && ((H == X && ldh != ldx) || (H == R && ldh != ldr)))
     return fail(B2G_ERR_INVALID_ARG, "H in place needs the leading dimension of what it replaces");
   NormArgs a{};
@@ -1489,6 +1496,10 @@ extern "C" int b2g_rmsnorm_bwd_q8(const void* dY, const void* X, const float* x_
     return fail(B2G_ERR_INVALID_ARG, "dY, X, W, rstd or dX is null");
   if (is_q8(x_dtype) != (x_scale != nullptr))
     return fail(B2G_ERR_INVALID_ARG, "x_scale goes with an 8-bit checkpoint, and only with one");
+  rc = check_alignment({{"dY", dY, dtype}, {"X", X, x_dtype}, {"x_scale", x_scale, B2G_DTYPE_F32},
+                        {"W", W, w_dtype}, {"rstd", rstd, B2G_DTYPE_F32}, {"dR", dR, dtype}, {"dX", dX, dtype},
+                        {"dw", dw, B2G_DTYPE_F32}});
+  if (rc != B2G_OK) return rc;
   if ((dX == dY && lddx != ldy) || (dX == dR && lddx != ldr))
     return fail(B2G_ERR_INVALID_ARG, "dX in place needs the leading dimension of what it replaces");
   int dev = 0, sms = 0, cc = 0;

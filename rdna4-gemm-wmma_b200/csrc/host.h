@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/b2g_gemm.h"
 
@@ -51,6 +52,22 @@ inline bool is_real(int dt) {
   return dt == B2G_DTYPE_F16 || dt == B2G_DTYPE_BF16 || dt == B2G_DTYPE_F32;
 }
 inline bool is_q8(int dt) { return dt == B2G_DTYPE_I8 || dt == B2G_DTYPE_E4M3; }
+
+// Refuses pointers below the alignment of their element type, which the kernels' accesses rely on
+// (null: an optional argument that is not given).
+struct Operand {
+  const char* name;
+  const void* p;
+  int dtype;
+};
+inline int check_alignment(std::initializer_list<Operand> ops) {
+  for (const Operand& o : ops) {
+    const uintptr_t size = o.dtype == B2G_DTYPE_F32 ? 4 : is_real(o.dtype) ? 2 : 1;
+    if ((uintptr_t)o.p % size != 0)
+      return fail(B2G_ERR_INVALID_ARG, "%s is not aligned to its element type", o.name);
+  }
+  return B2G_OK;
+}
 
 // b2g_dequantize_q8 without its argument checks (b2g_rows.cu).
 int dequantize_rows(const void* Q, const float* scale, void* X, int64_t M, int64_t N, int64_t ldq,

@@ -487,7 +487,7 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
     """(pointer, leading dimension) of a rows x cols operand of the 8-bit operators.  A raw pointer is
     taken as it is (leading dimension `cols` unless given).  A torch tensor has to be of the type
     that the call names and on the current device, and a row-major matrix of that size at least,
-    whose row stride is the default leading dimension."""
+    whose row stride is the default leading dimension; with another one, its storage has to hold the rows."""
     if x is None or isinstance(x, int) or _torch is None or not isinstance(x, _torch.Tensor):
         return _ptr(x) or 0, (cols or 1) if ld is None else ld
     if x.get_device() != dev or x.dtype not in _torch_types.get(dtype, ()):
@@ -503,6 +503,8 @@ def _matrix(x, dtype, what, rows, cols, ld, dev):
                 _refuse("%s is no row-major matrix of %d x %d", what, rows, cols)
             elif rows > 1:
                 ld = st[0]
+    elif rows and cols and (rows - 1) * ld + cols > x.untyped_storage().nbytes() // x.element_size() - x.storage_offset():
+        _refuse("%s ends before %d rows of %d at leading dimension %d", what, rows, cols, ld)
     return x.data_ptr(), ld
 
 

@@ -478,7 +478,9 @@ def _refuse(msg, *args):
 
 
 def _wrong_tensor(x, dtype, what):
-    if x.dtype not in _torch_types.get(dtype, (x.dtype,)):
+    if dtype not in _torch_types:
+        _refuse("%s: unsupported type code %r", what, dtype)
+    if x.dtype not in _torch_types[dtype]:
         _refuse("%s is %s, not of type code %r", what, x.dtype, dtype)
     _refuse("%s is not on %s", what, "the current device" if x.is_cuda else "a GPU")
 

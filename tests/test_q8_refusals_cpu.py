@@ -83,3 +83,12 @@ def test_binding_checks_a_given_leading_dimension(b2g, host_tensors):
         with pytest.raises(b2g.B2GError, match="leading dimension"):
             call()
         assert len(calls) == len(ok), i
+
+
+def test_binding_names_an_unknown_type_code(b2g, host_tensors):
+    torch, calls = host_tensors
+    x, q, s = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)
+    for kw in (dict(dtype=b2g.DTYPE_E5M2), dict(dtype=77), dict(dtype=b2g.DTYPE_BF16, q_dtype=b2g.DTYPE_E5M2)):
+        with pytest.raises(b2g.B2GError, match="unsupported type code"):
+            b2g.quantize_q8(x, q, s, 4, 8, stream=1, **kw)
+    assert not calls

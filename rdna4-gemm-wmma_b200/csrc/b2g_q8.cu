@@ -759,6 +759,8 @@ extern "C" int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int
   }
   if (!C) return fail(B2G_ERR_INVALID_ARG, "C is null");
   if (K > 0 && (!A || !B)) return fail(B2G_ERR_INVALID_ARG, "A or B is null");
+  if (M == 1) lda = std::max<int64_t>(K, 1), ldc = N;  // the pitch of a single row is not used: any is as good
+  if (N == 1) ldb = std::max<int64_t>(K, 1);
   int rc = check_alignment({{"C", C, c_dtype}, {"a_scale", a_scale, B2G_DTYPE_F32},
                             {"b_scale", b_scale, B2G_DTYPE_F32}, {"bias", bias, B2G_DTYPE_F32}});
   if (rc != B2G_OK) return rc;
@@ -818,6 +820,8 @@ extern "C" int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, v
   }
   if (!dW) return fail(B2G_ERR_INVALID_ARG, "dW is null");
   if (M > 0 && (!dY || !Q || !scale)) return fail(B2G_ERR_INVALID_ARG, "dY, Q or scale is null");
+  if (M == 1) ldy = N, ldq = K;  // as in b2g_gemm_q8
+  if (N == 1) ldw = K;
   int rc = check_alignment({{"dY", dY, dtype}, {"scale", scale, B2G_DTYPE_F32}, {"dW", dW, c_dtype}});
   if (rc != B2G_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

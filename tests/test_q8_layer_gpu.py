@@ -78,3 +78,25 @@ def test_products_of_narrow_operands_at_odd_bases(b2g, cuda, M, K, q):
     b2g.wgrad_q8(y, X, torch.ones(M, device="cuda"), dW, M, K, 24, q_dtype=q)
     assert torch.equal(dW, y.float().t() @ X.float())
     assert b2g.device_status() == 0
+
+
+@pytest.mark.parametrize("ld", [1 << 41, (1 << 41) + 3])
+def test_the_pitch_of_a_single_row_does_not_matter(b2g, cuda, ld):
+    """One token, one output channel, one row of dY or dW: any leading dimension, past what TMA can address."""
+    torch = cuda
+    ones = lambda *s, t=torch.int8: torch.ones(*s, dtype=t, device="cuda")
+    C = torch.zeros(1, 4096, device="cuda")
+    b2g.gemm_q8(ones(1, 4096), ones(4096, 4096), C, 1, 4096, 4096, lda=ld, ldc=ld)
+    assert bool((C == 4096).all())
+    C = torch.zeros(300, 1, device="cuda")
+    b2g.gemm_q8(ones(300, 520), ones(1, 520), C, 300, 1, 520, ldb=ld)
+    assert bool((C == 520).all())
+    dW = torch.zeros(264, 520, device="cuda")
+    b2g.wgrad_q8(ones(1, 264, t=torch.bfloat16), ones(1, 520), torch.ones(1, device="cuda"), dW, 1, 264, 520, ldy=ld, ldq=ld)
+    assert bool((dW == 1).all())
+    dW = torch.zeros(1, 520, device="cuda")
+    b2g.wgrad_q8(ones(300, 1, t=torch.bfloat16), ones(300, 520), torch.ones(300, device="cuda"), dW, 300, 1, 520, ldw=ld)
+    assert bool((dW == 300).all())
+    x, q, s = ones(1, 520, t=torch.bfloat16), ones(1, 520), torch.ones(1, device="cuda")
+    b2g.quantize_q8(x, q, s, 1, 520, dtype=BF16, ldx=ld, ldq=ld)
+    assert bool((q == 127).all()) and b2g.device_status() == 0

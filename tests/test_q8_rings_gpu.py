@@ -2,14 +2,14 @@
 import pytest
 
 from gpu_util import options
-from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, check_bwd, check_norm, rows, row_quant64, grid, tt
+from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, check_bwd, check_norm, grid, pad_untouched, padded, row_quant64, rows, tt
 
 pytestmark = pytest.mark.gpu
 
 
-def check_quantize(torch, b2g, M, N, dt, q):
-    x = rows(torch, M, N, N).to(tt(torch, dt))
-    Q, s = torch.zeros(M, N, dtype=torch.int8, device="cuda").view(tt(torch, q)), torch.zeros(M, device="cuda")
+def check_quantize(torch, b2g, M, N, dt, q, pad=0):
+    _, x = padded(torch, M, N, dt, pad, rows(torch, M, N, N))
+    (buf, Q), s = padded(torch, M, N, q, pad), torch.zeros(M, device="cuda")
     b2g.quantize_q8(x, Q, s, M, N, dtype=dt, q_dtype=q)
     t, want = row_quant64(torch, x.double(), q, False)
     assert torch.equal(s.double(), want)
@@ -18,6 +18,7 @@ def check_quantize(torch, b2g, M, N, dt, q):
         assert torch.equal(Q.double(), r)
     else:  # the product with qmax and the quotient round once each
         assert bool(((Q.double() - t).abs() <= half * (1 + 2 ** -20) + 4 * 2.0 ** -24 * t.abs()).all())
+    assert pad_untouched(torch, buf, N)
 
 
 # Stages of 56832, 75776 and 113664 bytes: four, three and two of them fill the shared memory to its
@@ -120,4 +121,71 @@ def test_least_time_limit(b2g, cuda):
             assert b2g.device_status() != 0 or all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(torch.equal(a, b) for a, b in zip(step(), want))
     check_gemm(torch, b2g, 100, 520, 1184, I8, F32)
+    assert b2g.device_status() == 0
+
+
+# (most blocks an SM, N, pad): nine rows and more a block, so that each of up to four buffers is refilled twice; rows of
+# whole 16-byte vectors of every kernel width, and rows of any alignment
+MANY = [(14, 1024, 0), (9, 1544, 0), (7, 4096, 8), (4, 8192, 0), (2, 16384, 0), (8, 1001, 5), (8, 2047, 0), (4, 4001, 2), (2, 8191, 0),
+        (1, 16001, 0)]
+
+
+def rows_of_many(torch, blocks):
+    return 9 * blocks * torch.cuda.get_device_properties(0).multi_processor_count + 7
+
+
+@pytest.mark.parametrize("dt", [F16, BF16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("blocks,N,pad", MANY)
+def test_many_rows_into_8_bits(b2g, cuda, blocks, N, pad, dt):
+    M = rows_of_many(cuda, blocks)
+    q = I8 if dt != F16 else E4M3
+    check_norm(cuda, b2g, M, N, dt, q, True, False, pad)
+    check_norm(cuda, b2g, M, N, dt, q, True, False, pad, inplace=True, seed=3)
+    check_norm(cuda, b2g, M, N, dt, q, False, True, pad, seed=6)
+    check_quantize(cuda, b2g, M, N, dt, q, pad)
+    assert b2g.device_status() == 0
+
+
+@pytest.mark.parametrize("xt", [I8, E4M3, None], ids=["i8", "e4m3", "same"])
+@pytest.mark.parametrize("dt", [BF16, F32], ids=NAMES.get)
+@pytest.mark.parametrize("blocks,N,pad", MANY)
+def test_many_rows_backward(b2g, cuda, blocks, N, pad, dt, xt):
+    M, xt = rows_of_many(cuda, blocks), dt if xt is None else xt
+    check_bwd(cuda, b2g, M, N, dt, xt, True, pad)
+    check_bwd(cuda, b2g, M, N, dt, xt, False, pad, inplace=True)
+    assert b2g.device_status() == 0
+
+
+@pytest.mark.parametrize("blocks,N,pad", [(14, 1024, 0), (4, 8192, 0), (8, 1001, 5), (2, 8191, 0)])
+def test_many_rows_in_place_and_again(b2g, cuda, blocks, N, pad):
+    """H in X, dX in dY (with dR) and dX in dR give what separate outputs do, bit for bit, time after time."""
+    torch = cuda
+    M = rows_of_many(torch, blocks)
+    bf = torch.bfloat16
+    new = lambda t=bf: torch.zeros(M, N + pad, dtype=t, device="cuda")[:, :N]
+    x, y, r = (new() for _ in range(3))
+    for i, t in enumerate((x, y, r)):
+        t.copy_(rows(torch, M, N, i))
+    w = (1 + 0.2 * torch.randn(N, device="cuda")).to(bf)
+    def norm(src, dst):
+        q, s, rstd = new(torch.int8), torch.zeros(M, device="cuda"), torch.zeros(M, device="cuda")
+        b2g.rmsnorm_q8(src, w, q, s, M, N, dtype=BF16, H=dst, rstd=rstd)
+        return q, s, rstd
+    h = new()
+    q, s, rstd = norm(x, h)
+    assert torch.equal(h, x)
+    def bwd(dy, dr, dst):
+        dw = torch.zeros(N, device="cuda")
+        b2g.rmsnorm_bwd_q8(dy, q, s, w, rstd, dst, dw, M, N, dtype=BF16, dres=dr)
+        return dst.clone(), dw
+    want = bwd(y, r, new())
+    for _ in range(3):
+        again = new()
+        again.copy_(x)
+        assert all(torch.equal(a, b) for a, b in zip(norm(again, again), (q, s, rstd))) and torch.equal(again, x)
+        for at in (0, 1):
+            a, b = new(), new()
+            a.copy_(y)
+            b.copy_(r)
+            assert all(torch.equal(g, v) for g, v in zip(bwd(a, b, (a, b)[at]), want))
     assert b2g.device_status() == 0

@@ -1,7 +1,7 @@
 """GPU tests of the 8-bit layer's products: sums of many tokens, scales, and launches that fail."""
 import pytest
 
-from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, scales, tt
+from test_q8_gpu import BF16, E4M3, F16, F32, I8, NAMES, half_step, q8_matrix, scales, tt
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,25 @@ def test_the_pitch_of_a_single_row_does_not_matter(b2g, cuda, ld):
     x, q, s = ones(1, 520, t=torch.bfloat16), ones(1, 520), torch.ones(1, device="cuda")
     b2g.quantize_q8(x, q, s, 1, 520, dtype=BF16, ldx=ld, ldq=ld)
     assert bool((q == 127).all()) and b2g.device_status() == 0
+
+
+@pytest.mark.parametrize("q", [I8, E4M3], ids=NAMES.get)
+@pytest.mark.parametrize("dt,c", [(BF16, F32), (F16, F32), (BF16, BF16), (F16, F16)], ids=["bf16-f32", "f16-f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(70, 130, 264), (1500, 520, 392), (5000, 264, 1040)])
+def test_weight_gradient_with_ordinary_scales(b2g, cuda, M, N, K, dt, c, q):
+    """Scales that are no powers of two: q * scale is rounded to dY's type before the product, half a step of it
+    (2^-8 relative in bf16, 2^-11 in fp16, whose subnormals add 2^-25) in every term, and no more."""
+    torch = cuda
+    u = 2.0 ** -24
+    dY = (torch.randn(M, N, device="cuda") * 0.1).to(tt(torch, dt))
+    _, Q = q8_matrix(torch, M, K, q, 7)
+    s = scales(torch, M, 3)
+    dW = torch.zeros(N, K, dtype=tt(torch, c), device="cuda")
+    b2g.wgrad_q8(dY, Q, s, dW, M, N, K, dtype=dt, q_dtype=q, c_dtype=c)
+    x, y = Q.double() * s.double()[:, None], dY.double()
+    ref, size = y.t() @ x, y.abs().t() @ x.abs()
+    tol = (half_step(torch, dt) + u) * size + (2.0 ** -25 * y.abs().sum(0)[:, None] if dt == F16 else 0)  # the rounding of q * scale
+    tol = tol + 2 * (M + 1) * u * size * 1.01 + half_step(torch, c) * ref.abs() + (2.0 ** -25 if c == F16 else 0)
+    err = (dW.double() - ref).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+    assert b2g.device_status() == 0

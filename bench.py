@@ -306,9 +306,9 @@ def main():
                          "over the N GPUs, B broadcast in K panels inside every step; "
                          "tp_k: tensor-parallel K-split GEMM (8192^3 or --shape) whose partials "
                          "are reduce-scattered over the N GPUs inside every step; "
-                         "linear_q8: one training step of an 8-bit linear layer on one GPU (RMS norm "
-                         "into 8 bits, scaled product, weight gradient and norm backward from the "
-                         "8-bit checkpoints; 8192 tokens, 8192 -> 8192, or --shape tokens,out,in, "
+                         "linear_q8: one training step of an 8-bit linear layer on one GPU without its "
+                         "data gradient (RMS norm into 8 bits, scaled product, weight gradient and norm "
+                         "backward from the 8-bit checkpoints; 8192 tokens, 8192 -> 8192, or --shape tokens,out,in, "
                          "--dtype i8 or e4m3)")
     ap.add_argument("--bcast", default="chain", choices=["chain", "nccl"],
                     help="sharded32768: how B reaches the ranks each step (copy-engine chain, "
@@ -873,8 +873,9 @@ def run_tp_k(args, torch, dist, b2g, ws, rank, local, dev):
 def run_linear_q8(args, torch, b2g, dev):
     """One training step of an 8-bit linear layer, y = W . norm(x + r): RMS norm with the residual's
     addition into 8 bits, the residual stream put aside in 8 bits, the scaled product, the weight
-    gradient and the norm's backward pass from the two 8-bit checkpoints.  Weights are quantised
-    once, as an inference engine or a step with frozen 8-bit weights does."""
+    gradient and the norm's backward pass from the two 8-bit checkpoints.  The data gradient, a plain
+    product with 16-bit weights, is neither run nor counted (its result is an input here).  Weights are
+    quantised once, as an inference engine or a step with frozen 8-bit weights does."""
     M, N, K = (int(x) for x in args.shape.split(",")) if args.shape else (8192, 8192, 8192)
     q = b2g.DTYPE_E4M3 if args.dtype == "e4m3" else b2g.DTYPE_I8
     qt = torch.float8_e4m3fn if q == b2g.DTYPE_E4M3 else torch.int8
@@ -933,7 +934,7 @@ def run_linear_q8(args, torch, b2g, dev):
         "dtype": "%s operands, %s sums, bf16 activations and gradients, f32 weight gradient" % (
             args.dtype if q == b2g.DTYPE_E4M3 else "i8", "f32" if q == b2g.DTYPE_E4M3 else "i32"),
         "data": "synthetic: seeded normal activations, weights and gradients",
-        "config": {"workload": "training step of an 8-bit linear layer behind an RMS norm", "tokens": M,
+        "config": {"workload": "training step of an 8-bit linear layer behind an RMS norm, without its data gradient", "tokens": M,
                    "out": N, "in": K, "l2": "operands and results over 126 MB: no flush needed"},
         "us_alone": alone,
         "roofline": {"bound": "tensor", "target_ms": target, "frac": target / ms,

@@ -350,9 +350,12 @@ int b2g_gemm_batched(const void* A, const void* B, float* C, int64_t L, int64_t 
  *     unless it is said to be optional.  M == 0 is valid everywhere.
  *   - Outputs may not overlap inputs or each other, except where said.
  *   - b2g_last_path() is set by the two products and not by the row operators.
- *   - The products obey the options cta_group, tile_n, split_k, tail_split, cluster_fixup,
- *     serial_fixup, pdl, raster_group, force_generic, timeout_ns and fault_flags; the row operators
- *     obey timeout_ns and fault_flags.
+ *   - Options.  All products: pdl and force_generic.  Products of more than 128 tokens and weight gradients:
+ *     cta_group, tile_n, split_k, tail_split (not fp32 weight gradients), cluster_fixup, serial_fixup,
+ *     raster_group, timeout_ns and fault_flags.  Products of up to 128 tokens choose their own tiles: of
+ *     these they obey split_k (at most 8), timeout_ns and fault_flags, and with up to 16 tokens and
+ *     12 Mi weights (B2G_PATH_FEW) none.  b2g_last_path() is B2G_PATH_TC_1CTA for a product of up to
+ *     128 tokens that is not B2G_PATH_FEW.  The row operators obey timeout_ns and fault_flags.
  *   - Where a wait of a row operator runs out (b2g_device_status() code 8), the rows of that block from there
  *     on come out with the scale and rstd NaN and zeros, or as a NaN dX, H is NaN in all of that
  *     block's rows, and dw is NaN.
@@ -378,7 +381,10 @@ int b2g_dequantize_q8(const void* Q, const float* scale, void* X, int64_t M, int
  * R is optional (NULL: h = x); H is optional and receives h rounded to dtype; H may be X or R
  * itself (same leading dimension), for a residual stream updated in place.  rstd is optional
  * (M values, for b2g_rmsnorm_bwd_q8).  X, R and H have type dtype (F16, BF16 or F32), W (N
- * values) w_dtype (the same three).  The sum of squares of a row has to stay below 2^128.
+ * values) w_dtype (the same three).  The sum of squares of a row has to stay below 2^128, and with
+ * eps == 0 above 2^-126 (a row of zeros then has the scale NaN: its norm is 0 / 0).  y is not rounded
+ * before its row's largest value is known, so a value within fp32 rounding of a border between
+ * two 8-bit values may fall to either side of it, and so may a pow2 scale next to a power of two.
  */
 int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void* H, void* Q, float* scale,
                    float* rstd, int64_t M, int64_t N, int64_t ldx, int64_t ldr, int64_t ldh,
@@ -391,7 +397,8 @@ int b2g_rmsnorm_q8(const void* X, const void* R, const void* W, void* H, void* Q
  * `dtype` (I8 or E4M3).  int8 products are summed exactly in int32 (K <= 131071, so that no sum
  * overflows), e4m3 products in fp32 (the tensor core truncates each addition: measured 9.7e-7
  * relative for 28672 products of one sign, 3.7e-6 for 65536).  a_scale (M), b_scale (N) and bias (N) are optional fp32
- * vectors (NULL: 1, 1 and 0).  C is F32, F16 or BF16, rounded once.
+ * vectors (NULL: 1, 1 and 0), applied in fp32 from left to right as the formula is written (so sum *
+ * a_scale has to stay in fp32's range).  C is F32, F16 or BF16, rounded once.
  */
 int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int64_t N, int64_t K, int64_t lda,
                 int64_t ldb, int64_t ldc, int dtype, const float* a_scale, const float* b_scale,
@@ -402,9 +409,11 @@ int b2g_gemm_q8(const void* A, const void* B, void* C, int64_t M, int64_t N, int
  *   dW[n*ldw + k] = sum_{m < M} dY[m*ldy + n] * (Q[m*ldq + k] * scale[m])   (+ dW if accumulate)
  * dY is M x N (dtype F16 or BF16), Q M x K (q_dtype) with its row scales, dW N x K of type
  * c_dtype: F32, or (accumulate == 0 only) F16 or BF16.  Q * scale is rounded to dY's type
- * (saturating): with power-of-two scales it is exact in BF16, and in F16 while it lies in
- * F16's range.  Products are exact in fp32 and summed in fp32; an fp32 dW sums at most 768
- * tokens in one tensor-core accumulator, and such partial sums in fp32.
+ * (saturating): with power-of-two scales (pow2 of b2g_quantize_q8 and b2g_rmsnorm_q8) it is exact in BF16,
+ * and in F16 while it lies in F16's range; with others each term is off by up to half a step
+ * of dY's type (2^-8 in BF16, 2^-11 in F16; measured over whole gradients, 2-norm, 1.6e-3 and 2.0e-4).
+ * Products are exact in fp32 and summed in fp32; an fp32 dW sums at most 768 tokens in one
+ * tensor-core accumulator (which truncates), and such partial sums in fp32; a 16-bit dW sums any number.
  */
 int b2g_wgrad_q8(const void* dY, const void* Q, const float* scale, void* dW, int64_t M, int64_t N,
                  int64_t K, int64_t ldy, int64_t ldq, int64_t ldw, int dtype, int q_dtype,

@@ -331,8 +331,8 @@ __device__ __forceinline__ Ring make_ring(uint8_t* smem, int stages, uint32_t st
 // rows_to_q8_kernel with its rows in a ring: rows of whole 16-byte vectors, one row at a time a block of
 // up to THREADS threads, which hold V vectors each.  The norm's weights stay in registers where V <= 4.
 // CTAS blocks share an SM, so that one's reduction overlaps the others' arithmetic.  Bound by memory: bf16,
-// norm with residual 8192 x 8192 81 us and 16384 x 4096 80 us (5.8 TB/s), quantize 16384 x 8192 75 us
-// (5.4 TB/s); rows of 1024 by instructions, norm 16384 x 1024 27 us (4.3 TB/s).
+// norm with residual 8192 x 8192 82 us and 16384 x 4096 82 us (5.7 TB/s), quantize 16384 x 8192 77 us
+// (5.2 TB/s); rows of 1024 by instructions, norm 16384 x 1024 27.5 us (4.3 TB/s).
 template <typename T, bool NORM, int V, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS)
     rows_ring_kernel(const NormArgs a, int stages, uint32_t row_bytes, uint64_t limit_ns) {
@@ -454,8 +454,8 @@ __device__ __forceinline__ uint32_t low4(const void* p) { return (uint32_t)(uint
 // thread's, so that shared and global accesses of a warp are consecutive.  Q, H and the first and
 // last row go through ordinary accesses.  Instructions are the limit here (one access an element and
 // operand), so THREADS is a constant: every address is one base with a constant offset.  bf16, norm with
-// residual 8192 x 8191 140 us (3.4 TB/s); aligned rows through it 132 us at 8192 x 8192, where
-// rows_ring_kernel takes 81, quantize 16384 x 8192 114 against 75.
+// residual 8192 x 8191 129 us (3.6 TB/s); 8192 x 8192 at an odd pitch 129 us, where rows_ring_kernel
+// takes 82 for aligned rows, quantize 16384 x 8192 116 against 77.
 template <typename T, bool NORM, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS, V <= 16 ? 1024 / THREADS : 1)
     rows_ring_elems_kernel(const NormArgs a, int stages, uint32_t slot, uint64_t limit_ns) {
@@ -841,8 +841,8 @@ struct XVec {
 // traffic but one partial row a block.  HOLD (up to 16 elements a thread): the weights, and a row's
 // dy * w and xh, stay in fp32 registers; else a row stays packed between the reduction and the
 // output and is unpacked twice, with the weights read from L1.  bf16, int8 checkpoint, residual:
-// 8192 x 8192 91 us (5.1 TB/s), 8192 x 4096 50 us (packed 102), 16384 x 1024 31 us (packed 57),
-// 4096 x 16384, packed, 190 us (2.5 TB/s, instructions).
+// 8192 x 8192 86 us (5.5 TB/s), 8192 x 4096 52 us (packed, when compared, 102 against 50), 16384 x 1024 30 us
+// (packed 57 against 31), 4096 x 16384, packed, 154 us (3.0 TB/s, instructions).
 template <typename T, bool X8, int V, bool HOLD>
 __global__ void __launch_bounds__(512, 1)
     rmsnorm_bwd_ring_kernel(const BwdArgs a, int stages, uint32_t y_bytes, uint32_t x_bytes,
@@ -992,8 +992,8 @@ __global__ void __launch_bounds__(512, 1)
 }
 
 // The same for rows of any alignment, element by element (as rows_ring_elems_kernel).  Bound by
-// instructions: aligned rows through it 175 us at 8192 x 8192 (the kernel above 91), 48 us at 16384 x 256
-// (16).
+// instructions: at an odd pitch 174 us at 8192 x 8192 (the kernel above, aligned, 86), 50 us at 16384 x 256
+// (14).
 template <typename T, bool X8, int THREADS, int V>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS)
     rmsnorm_bwd_elems_kernel(const BwdArgs a, int stages, uint32_t y_slot, uint32_t x_slot, uint64_t limit_ns) {
@@ -1175,7 +1175,7 @@ int raise_smem(F fn, std::atomic<uint64_t>& ready) {
 
 // A launch of rows_ring_kernel, or false where its stages do not fit or a block would have too few rows (one
 // with the norm, two without) for the ring to pay.  Against rows_to_q8_kernel (us, bf16, graph): norm with
-// residual, 8192 rows of 8192 81 against 151, 16384 of 1024 27 against 51, 1000 of 4096 11.4 against
+// residual, 8192 rows of 8192 82 against 151, 16384 of 1024 27 against 51, 1000 of 4096 11.4 against
 // 13.4, 296 of 8192 7.2 against 8.1, but 296 of 4096 4.8 against 3.9; quantize, 16384 of 8192 78
 // against 99, 1000 of 4096 4.2 against 4.5, but 444 of 16384 8.6 against 6.6.
 template <typename T, bool NORM, int V, int THREADS, int CTAS>
